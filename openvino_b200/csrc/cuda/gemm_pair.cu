@@ -112,13 +112,6 @@ __device__ __forceinline__ PairTile pair_tile(const PairParams& p, int idx) {
     return r;
 }
 
-// Tensor load into this CTA's shared memory, bytes reported on the barrier at the same offset in the even CTA of the pair.
-__device__ __forceinline__ void pair_load_2d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar & 0xFEFFFFFFu), "r"(c0), "r"(c1)
-        : "memory");
-}
 __device__ __forceinline__ void pair_mma_elect(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p, q;\n\t"
@@ -126,15 +119,6 @@ __device__ __forceinline__ void pair_mma_elect(uint32_t tmem_d, uint64_t da, uin
         "elect.sync _|q, 0xffffffff;\n\t"
         "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
         ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-// Arrive on the barrier at this offset in both CTAs once the MMAs issued so far are done.
-__device__ __forceinline__ void pair_commit_elect(uint64_t* bar) {
-    asm volatile(
-        "{\n\t.reg .pred q;\n\t"
-        "elect.sync _|q, 0xffffffff;\n\t"
-        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}"
-        ::"r"(smem_u32(bar)), "h"((uint16_t)3)
         : "memory");
 }
 template <bool F16, int FORM>

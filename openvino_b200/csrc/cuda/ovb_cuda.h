@@ -139,6 +139,41 @@ int ovb_pack_w16(const void* w, void* w_out, int N, int K, ovb_stream_t stream);
 int ovb_pack_f8(const void* w, void* w_out, long long words, ovb_stream_t stream);
 
 // ---------------------------------------------------------------------------------------------
+// Products of 8-bit whole numbers (gemm_i8.cu, quantize_rows.cu): rows quantised with a scale each, weights with a scale (and a zero point) per channel.
+//   out[t, n] = act((sum_k x[t, k] w[n, k] - w_zp[n] * x_sum[t]) * x_scale[t] * w_scale[n] + bias[n]) + residual[t, n]
+typedef struct {
+    const void* x;            // 16-bit rows (row row_idx[r] where given; an index outside [0, x_rows) reads row 0), pitch ldx
+    const void* gamma;        // RMS norm of the rows on the way: y = x * rsqrt(mean(x^2) + eps) * gamma; or NULL
+    const int* row_idx;
+    void* q;                  // signed bytes, pitch ldq: round(y * (127 / max|y|)), halves to even
+    float* scale;             // [rows] max|y| / 127; 0 where max|y| < 2^-119, NaN where a value is not finite (codes 0)
+    int* sum;                 // [rows] sum of the codes
+    int64_t ldx;
+    int rows, cols, x_rows, ldq, f16;      // f16: x and gamma are fp16, otherwise bf16
+    float eps;
+} ovb_quant_rows_args;
+int ovb_quantize_rows(const ovb_quant_rows_args* a, ovb_stream_t stream);
+// [N, K] bytes of pitch ldw -> chunks of 128 rows x 128 columns in the swizzled order of the MMA, zeros behind N and K; unsigned bytes become b - 128.
+int64_t ovb_pack_i8_bytes(int N, int K);
+int ovb_pack_i8(const void* w, int is_unsigned, void* w_out, int N, int K, int64_t ldw, ovb_stream_t stream);
+typedef struct {
+    const void* x;            // signed bytes in [-127, 127], 16-byte aligned, pitch ldx (a multiple of 16)
+    const float* x_scale;     // [T]
+    const int* x_sum;         // [T]
+    const void* w;            // made by ovb_pack_i8, 128-byte aligned
+    const float* w_scale;     // [N]
+    const int* w_zp;          // [N] in [-128, 127], in the signed form of the bytes; or NULL
+    const void* bias;         // [N] in the 16-bit type, or NULL
+    const void* residual;     // 16-bit, pitch ldr, or NULL (may be out itself)
+    void* out;                // 16-bit or fp32, pitch ldo
+    int T, N, K, ldx, ldo, ldr;            // K <= 65536
+    int act;                  // OVB_ACT_*; gated ones as in ovb_gemm
+    int f16, out_f32;         // the 16-bit type is fp16, otherwise bf16; out is fp32
+    float act_limit, act_slope, act_shift;
+} ovb_gemm_i8_args;
+int ovb_gemm_i8(const ovb_gemm_i8_args* a, ovb_stream_t stream);
+
+// ---------------------------------------------------------------------------------------------
 // Normalisation / elementwise
 // y = rmsnorm(x (+ residual)) * gamma ;  if residual_out != NULL it receives x + residual.
 int ovb_rmsnorm(const void* x, const void* residual, const void* gamma, void* y, void* residual_out, int rows,
@@ -254,6 +289,31 @@ int ovb_rope_kv_write(void* qkv, const int* positions, const int* slot_map, void
    to k_meta / v_meta (see ovb_pa_args). */
 int ovb_rope_kv_write_u8(void* qkv, const int* positions, const int* slot_map, void* k_cache, void* v_cache, void* k_meta, void* v_meta, int T,
                          int Hq, int Hkv, int D, float theta, int block_size, ovb_stream_t stream);
+
+// Head norms and rotation in one pass (head_rope.cu): q [B, S, Hq, D] and k [B, S, Hkv, D] (element strides per batch, token and head; the elements
+// of a head lie side by side) to q_out and k_out of the same form, which may be q and k themselves; or, with caches, k and v to the rows of
+// slot_map[b * S + s] in the paged caches (negative: not kept; one at or above `slots` is not kept and records status 5; the slots of a call differ).
+typedef struct {
+    const void* q;
+    const void* k;
+    const void* v;            // with caches
+    void* q_out;
+    void* k_out;              // without
+    void* k_cache;            // [num_blocks, Hkv, block_size, D] 16-bit, or bytes (kv_u8) with (scale, zero point) pairs in k_meta / v_meta
+    void* v_cache;
+    void* k_meta;
+    void* v_meta;
+    const int* positions;     // + b * pos_batch + s
+    const int* slot_map;
+    const float* inv_freq;    // [rot / 2]
+    const void* q_norm;       // [D] in the 16-bit type, or NULL
+    const void* k_norm;
+    int64_t q_batch, q_token, q_head, k_batch, k_token, k_head, v_batch, v_token, v_head, qo_batch, qo_token, qo_head, ko_batch, ko_token, ko_head, pos_batch;
+    int64_t slots;            // num_blocks * block_size
+    int B, S, Hq, Hkv, D, rot, block_size, interleaved, f16, kv_u8;
+    float eps, mult;          // cos and sin are multiplied by mult
+} ovb_qk_rope_args;
+int ovb_qk_norm_rope(const ovb_qk_rope_args* a, ovb_stream_t stream);
 
 // ---------------------------------------------------------------------------------------------
 // Paged attention. Cache layout [num_blocks, Hkv, block_size, D]; ragged batch described like the

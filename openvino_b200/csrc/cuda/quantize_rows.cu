@@ -1,0 +1,209 @@
+// Rows of 16-bit values -> signed bytes with one scale per row, the RMS norm of the row on the way where there is one.
+//
+//   y = x, or x * rsqrt(mean(x^2) + eps) * gamma;  a = max |y|;  q = round_half_even(y * (127 / a));  scale = a / 127;  sum = sum q
+//
+// Quotients and products are rounded to 32 bits once each, the norm's sums are held in 32 bits. |y| * (127 / a) is at most 127 (1 + 2^-23), so no value
+// has to be clamped. A row whose largest magnitude is below 2^-119, where 127 / a would not be finite, counts as zero (scale 0); one with a value that
+// is not finite gets the scale NaN and codes of zero, so that every result of the row is NaN. The magnitudes are compared as integers, where NaN is the
+// largest.
+//
+// What bounds it: memory, three bytes per value (two of them usually from L2). A row stays in registers between the passes: every thread holds HOLD
+// pieces of eight columns.
+#include "gemm_common.cuh"
+
+namespace ovb {
+
+struct QuantParams {
+    const void* x;
+    const void* gamma;            // or NULL
+    const int* row_idx;           // or NULL: rows 0 .. rows
+    uint8_t* q;
+    float* scale;
+    int* sum;
+    int rows, cols, x_rows;
+    int64_t ldx;
+    int ldq;
+    float eps;
+};
+
+constexpr uint32_t kNotFinite = 0x7F800000u;
+constexpr float kQuantFloor = 1.5046327690525280e-36f;      // 2^-119
+
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+
+// The sum (largest) over the warps that share a row; every thread gets it.
+template <int WPR, class T, class F>
+__device__ __forceinline__ T over_row(T v, T* box, F&& f) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if (WPR == 1) return v;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (lane == 0) box[warp] = v;
+    __syncthreads();
+    v = box[lane % WPR];
+#pragma unroll
+    for (int o = WPR / 2; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+__device__ __forceinline__ void row_result(const QuantParams& p, int row, uint32_t top, int sum) {
+    const float a = __uint_as_float(top);
+    p.scale[row] = top >= kNotFinite ? __int_as_float(0x7FFFFFFF) : a < kQuantFloor ? 0.f : __fdiv_rn(a, 127.f);
+    p.sum[row] = sum;
+}
+// 127 / a, or 0 where the row has no codes
+__device__ __forceinline__ float row_factor(uint32_t top) {
+    const float a = __uint_as_float(top);
+    return top >= kNotFinite || a < kQuantFloor ? 0.f : __fdiv_rn(127.f, a);
+}
+
+__device__ __forceinline__ int source_row(const QuantParams& p, int row) {
+    if (p.row_idx == nullptr) return row;
+    const int r = p.row_idx[row];
+    return r < 0 || r >= p.x_rows ? 0 : r;
+}
+
+// Rows of whole, aligned pieces of eight columns. WPR warps share a row; blocks of max(4, WPR) warps.
+template <class E, int WPR, int HOLD>
+__global__ void __launch_bounds__(WPR < 4 ? 128 : WPR * 32) quantize_rows_kernel(const QuantParams p) {
+    constexpr int RPB = WPR < 4 ? 4 / WPR : 1, SPAN = WPR * 32;
+    __shared__ float box_f[16];
+    __shared__ uint32_t box_u[16];
+    __shared__ int box_i[16];
+    const int row = blockIdx.x * RPB + (RPB > 1 ? (int)threadIdx.x / SPAN : 0), at = threadIdx.x % SPAN;
+    const int pieces = p.cols >> 3;
+    constexpr bool HELD = HOLD <= 4;            // with more pieces the weights do not fit the registers beside the row: they are read again
+    uint4 g[HELD ? HOLD : 1];
+    pdl_enter();
+    if (row >= p.rows) return;              // whole warps, and only where rows do not share a block's barriers
+    if (HELD && p.gamma != nullptr) {
+#pragma unroll
+        for (int h = 0; h < HOLD; ++h)
+            if (at + h * SPAN < pieces) g[h] = __ldg(static_cast<const uint4*>(p.gamma) + at + h * SPAN);
+    }
+    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const E*>(p.x) + (size_t)source_row(p, row) * p.ldx);
+    uint4 x[HOLD];
+#pragma unroll
+    for (int h = 0; h < HOLD; ++h) x[h] = at + h * SPAN < pieces ? __ldcg(src + at + h * SPAN) : make_uint4(0, 0, 0, 0);
+    float inv = 1.f;
+    if (p.gamma != nullptr) {
+        float ss = 0.f;
+#pragma unroll
+        for (int h = 0; h < HOLD; ++h) {
+            const E* e = reinterpret_cast<const E*>(&x[h]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) ss = fmaf(to_float(e[j]), to_float(e[j]), ss);
+        }
+        ss = over_row<WPR>(ss, box_f, [](float a, float b) { return a + b; });
+        inv = rsqrtf(ss / (float)p.cols + p.eps);
+    }
+    auto value = [&](int h, int j) {
+        const float v = to_float(reinterpret_cast<const E*>(&x[h])[j]);
+        return p.gamma != nullptr ? v * inv * to_float(reinterpret_cast<const E*>(&g[HELD ? h : 0])[j]) : v;
+    };
+    auto weights = [&](int h) {
+        if (!HELD && p.gamma != nullptr) g[0] = __ldg(static_cast<const uint4*>(p.gamma) + at + h * SPAN);
+    };
+    uint32_t top = 0;
+#pragma unroll
+    for (int h = 0; h < HOLD; ++h)
+        if (at + h * SPAN < pieces) {
+            weights(h);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = max(top, magnitude(value(h, j)));
+        }
+    top = over_row<WPR>(top, box_u, [](uint32_t a, uint32_t b) { return max(a, b); });
+    const float f = row_factor(top);
+    const bool codes = f != 0.f;
+    uint2* dst = reinterpret_cast<uint2*>(p.q + (size_t)row * p.ldq);
+    int sum = 0;
+#pragma unroll
+    for (int h = 0; h < HOLD; ++h)
+        if (at + h * SPAN < pieces) {
+            uint32_t w[2] = {0, 0};
+            if (codes) {
+                weights(h);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int c = __float2int_rn(__fmul_rn(value(h, j), f));
+                    sum += c;
+                    w[j >> 2] |= (uint32_t)(c & 0xFF) << (8 * (j & 3));
+                }
+            }
+            dst[at + h * SPAN] = make_uint2(w[0], w[1]);
+        }
+    sum = over_row<WPR>(sum, box_i, [](int a, int b) { return a + b; });
+    if (at == 0) row_result(p, row, top, sum);
+}
+
+// Any width, pitch and alignment: a block per row, which is read once for each pass.
+template <class E>
+__global__ void __launch_bounds__(256) quantize_rows_any_kernel(const QuantParams p) {
+    __shared__ float box_f[16];
+    __shared__ uint32_t box_u[16];
+    __shared__ int box_i[16];
+    pdl_enter();
+    const int row = blockIdx.x;
+    const E* src = static_cast<const E*>(p.x) + (size_t)source_row(p, row) * p.ldx;
+    const E* gamma = static_cast<const E*>(p.gamma);
+    float inv = 1.f;
+    if (gamma != nullptr) {
+        float ss = 0.f;
+        for (int k = threadIdx.x; k < p.cols; k += 256) ss = fmaf(to_float(src[k]), to_float(src[k]), ss);
+        ss = over_row<8>(ss, box_f, [](float a, float b) { return a + b; });
+        inv = rsqrtf(ss / (float)p.cols + p.eps);
+    }
+    auto value = [&](int k) { return gamma != nullptr ? to_float(src[k]) * inv * to_float(gamma[k]) : to_float(src[k]); };
+    uint32_t top = 0;
+    for (int k = threadIdx.x; k < p.cols; k += 256) top = max(top, magnitude(value(k)));
+    top = over_row<8>(top, box_u, [](uint32_t a, uint32_t b) { return max(a, b); });
+    const float f = row_factor(top);
+    int sum = 0;
+    for (int k = threadIdx.x; k < p.cols; k += 256) {
+        const int c = f != 0.f ? __float2int_rn(__fmul_rn(value(k), f)) : 0;
+        sum += c;
+        p.q[(size_t)row * p.ldq + k] = (uint8_t)(c & 0xFF);
+    }
+    sum = over_row<8>(sum, box_i, [](int a, int b) { return a + b; });
+    if (threadIdx.x == 0) row_result(p, row, top, sum);
+}
+
+template <class E>
+static cudaError_t run_quantize(const QuantParams& p, cudaStream_t stream) {
+    const bool whole = p.cols % 8 == 0 && p.ldx % 8 == 0 && p.ldq % 8 == 0 &&
+                       ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.gamma)) & 15) == 0 && (reinterpret_cast<uintptr_t>(p.q) & 7) == 0;
+    if (!whole || p.cols > 32768) return launch_pdl(quantize_rows_any_kernel<E>, dim3(p.rows), dim3(256), 0, stream, p);
+    auto go = [&](auto kern, int wpr) { return launch_pdl(kern, dim3(wpr < 4 ? (p.rows + 4 / wpr - 1) / (4 / wpr) : p.rows), dim3(wpr < 4 ? 128 : wpr * 32), 0, stream, p); };
+    if (p.cols <= 512) return go(quantize_rows_kernel<E, 1, 2>, 1);
+    if (p.cols <= 1024) return go(quantize_rows_kernel<E, 1, 4>, 1);
+    if (p.cols <= 4096) return go(quantize_rows_kernel<E, 8, 2>, 8);
+    if (p.cols <= 8192) return go(quantize_rows_kernel<E, 16, 2>, 16);
+    if (p.cols <= 16384) return go(quantize_rows_kernel<E, 16, 4>, 16);
+    return go(quantize_rows_kernel<E, 16, 8>, 16);
+}
+
+}  // namespace ovb
+
+extern "C" int ovb_quantize_rows(const ovb_quant_rows_args* a, ovb_stream_t stream_) {
+    using namespace ovb;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    OVB_REQUIRE(a && a->x && a->q && a->scale && a->sum, "ovb_quantize_rows: null operand");
+    OVB_REQUIRE(a->rows > 0 && a->cols > 0 && a->ldq >= a->cols && a->ldx >= 0, "ovb_quantize_rows: %d rows of %d columns, pitches %lld and %d", a->rows, a->cols,
+                (long long)a->ldx, a->ldq);
+    OVB_REQUIRE(a->row_idx == nullptr || a->x_rows > 0, "ovb_quantize_rows: row indices need the number of rows of x");
+    QuantParams p;
+    p.x = a->x;
+    p.gamma = a->gamma;
+    p.row_idx = a->row_idx;
+    p.q = static_cast<uint8_t*>(a->q);
+    p.scale = a->scale;
+    p.sum = a->sum;
+    p.rows = a->rows;
+    p.cols = a->cols;
+    p.x_rows = a->x_rows;
+    p.ldx = a->ldx;
+    p.ldq = a->ldq;
+    p.eps = a->eps;
+    OVB_CHECK_CUDA(a->f16 ? run_quantize<__half>(p, stream) : run_quantize<__nv_bfloat16>(p, stream));
+    return 0;
+}

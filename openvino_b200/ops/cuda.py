@@ -6,6 +6,7 @@ There is no eager/PyTorch fallback: if the library cannot be loaded, calls raise
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import math
 import os
@@ -20,12 +21,13 @@ _PKG = Path(__file__).resolve().parent.parent
 _LIB_PATH = Path(os.environ["OVB_CUDA_LIB"]) if os.environ.get("OVB_CUDA_LIB") else _PKG / "lib" / "libovb_cuda.so"
 
 W_BF16, W_U4, W_U8, W_F16, W_F8 = 0, 1, 2, 3, 4
+W_I8 = 5                       # bytes multiplied as whole numbers with quantised rows (ovb_gemm_i8)
 W_F32 = 16                     # fp32 weights: products without tensor cores (ovb_gemm_f32)
 DT_F32, DT_BF16 = 0, 2         # storage types of the layered decoders' kernels
 ACT_NONE, ACT_GELU_ERF, ACT_RELU, ACT_SILU, ACT_SWIGLU, ACT_GELU_TANH, ACT_GLU_LIMITED, ACT_RELU2, ACT_SOFTCAP = 0, 1, 2, 3, 4, 5, 6, 7, 8
 
 STATUS_NAMES = {0: "ok", 1: "mbarrier wait timed out", 2: "peer flag wait timed out", 3: "bad argument seen on device",
-                4: "local flag wait timed out", 5: "index out of range (debug build; the access was skipped)"}
+                4: "local flag wait timed out", 5: "index out of range (the access was skipped)"}
 
 
 class GemmArgs(C.Structure):
@@ -136,6 +138,23 @@ class RgLruArgs(C.Structure):
                        ("B", "T", "N", "taps", "bw", "ub_pitch", "gb_pitch", "gi_off", "ldx", "ldy", "ldu", "ldg", "ldo", "max_q_len", "dtype"))
 
 
+class QuantRowsArgs(C.Structure):
+    _fields_ = (_fields(("x", "gamma", "row_idx", "q", "scale", "sum"), ()) + [("ldx", C.c_int64)]
+                + _fields((), ("rows", "cols", "x_rows", "ldq", "f16"), ("eps",)))
+
+
+class GemmI8Args(C.Structure):
+    _fields_ = _fields(("x", "x_scale", "x_sum", "w", "w_scale", "w_zp", "bias", "residual", "out"),
+                       ("T", "N", "K", "ldx", "ldo", "ldr", "act", "f16", "out_f32"), ("act_limit", "act_slope", "act_shift"))
+
+
+class QkRopeArgs(C.Structure):
+    _fields_ = (_fields(("q", "k", "v", "q_out", "k_out", "k_cache", "v_cache", "k_meta", "v_meta", "positions", "slot_map", "inv_freq", "q_norm", "k_norm"), ())
+                + [(t + "_" + d, C.c_int64) for t in ("q", "k", "v", "qo", "ko") for d in ("batch", "token", "head")]
+                + [("pos_batch", C.c_int64), ("slots", C.c_int64)]
+                + _fields((), ("B", "S", "Hq", "Hkv", "D", "rot", "block_size", "interleaved", "f16", "kv_u8"), ("eps", "mult")))
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -167,6 +186,11 @@ def lib():
             l.ovb_llm_scratch_bytes.restype = C.c_int64
             l.ovb_llm_scratch_bytes.argtypes = [C.POINTER(LlmStep)]
             l.ovb_llm_step_run.argtypes = [C.POINTER(LlmStep), C.c_void_p]
+        if hasattr(l, "ovb_gemm_i8"):
+            l.ovb_pack_i8_bytes.restype = C.c_int64
+            l.ovb_gemm_i8.argtypes = [C.POINTER(GemmI8Args), C.c_void_p]
+            l.ovb_quantize_rows.argtypes = [C.POINTER(QuantRowsArgs), C.c_void_p]
+            l.ovb_qk_norm_rope.argtypes = [C.POINTER(QkRopeArgs), C.c_void_p]
         l.ovb_pa_scratch_bytes.restype = C.c_int64
         l.ovb_channel_delta_record_floats.restype = C.c_int64
         l.ovb_gemm.argtypes = [C.POINTER(GemmArgs), C.c_void_p]
@@ -345,8 +369,110 @@ class PackedWeight:
         sz = torch.cat([sz.reshape(-1), torch.zeros(256, dtype=sz.dtype, device=sz.device)])   # slack for 128-row copies
         return PackedWeight(W_F8, w8, N, K, sz, None, block, bias)
 
+    @staticmethod
+    def from_ir_i8(w: torch.Tensor, scales: torch.Tensor, zps: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None) -> "PackedWeight":
+        """[N, K] int8 or uint8 weight with one scale per row, and a zero point per row of the weight's own type (None: 0, and 128 for uint8), for the
+        product of whole numbers: ``gemm`` quantises the rows that it meets, each with a scale of its own. Any N; K up to 65536. ``bias`` [N] is of
+        the 16-bit type of the rows."""
+        _need(w.dim() == 2 and w.numel() > 0 and w.dtype in (torch.int8, torch.uint8), "an int8 or uint8 weight [N, K] is expected, not %s %s", w.dtype, tuple(w.shape))
+        N, Kd = w.shape
+        _need(Kd <= 65536, "K = %d: 32-bit sums of products of bytes are exact up to 65536", Kd)
+        _need(scales.numel() == N and scales.is_floating_point(), "one scale per output channel is expected, not %d %s values for %d channels", scales.numel(), scales.dtype, N)
+        _need(zps is None or (zps.numel() == N and zps.dtype == w.dtype), "zero points are one value of the weight's type per output channel")
+        _need(bias is None or (bias.numel() == N and bias.dtype in (torch.bfloat16, torch.float16)), "the bias is one 16-bit value per output channel")
+        with _on(w, scales, zps, bias):
+            if w.stride(1) != 1 or w.stride(0) < Kd:
+                w = w.contiguous()
+            out = torch.empty(int(lib().ovb_pack_i8_bytes(C.c_int(N), C.c_int(Kd))), dtype=torch.uint8, device=w.device)
+            unsigned = w.dtype == torch.uint8
+            _check(lib().ovb_pack_i8(C.c_void_p(w.data_ptr()), C.c_int(1 if unsigned else 0), C.c_void_p(out.data_ptr()), C.c_int(N), C.c_int(Kd),
+                                     C.c_int64(w.stride(0)), C.c_void_p(_stream())), "ovb_pack_i8")
+            z = None if zps is None else zps.reshape(-1).to(torch.int32) - (128 if unsigned else 0)
+            return PackedWeight(W_I8, out, N, Kd, scales.reshape(-1).float().contiguous(), z, Kd, None if bias is None else bias.reshape(-1).contiguous(), tiled=True)
+
 
 # ------------------------------------------------------------------------------------------ ops
+def _need(ok: bool, message: str, *args) -> None:
+    if not ok:
+        raise ValueError(message % args)
+
+
+def _on(first: torch.Tensor, *others):
+    """The device of the operands, which have to share one, as the current device."""
+    for t in (first,) + others:
+        _need(t is None or (t.is_cuda and t.device == first.device), "the operands have to be on one CUDA device")
+    return contextlib.nullcontext() if first.device.index == torch.cuda.current_device() else torch.cuda.device(first.device)
+
+
+class QuantizedRows:
+    """Rows as signed bytes with one scale each: value = ``q`` * ``scales``. ``sums`` are the sums of the codes, ``dtype`` the 16-bit type that the rows had
+    (products of them have it again). The row pitch of ``q`` is a multiple of 16."""
+
+    __slots__ = ("q", "scales", "sums", "dtype")
+
+    def __init__(self, q, scales, sums, dtype):
+        self.q, self.scales, self.sums, self.dtype = q, scales, sums, dtype
+
+    @property
+    def shape(self):
+        return self.q.shape
+
+
+def quantize_rows(x: torch.Tensor, norm=None) -> QuantizedRows:
+    """bf16 or fp16 rows -> signed bytes: with a = max |row|, code = round(value * (127 / a)), halves to even, scale = a / 127.
+
+    ``norm`` (weights, eps[, row indices]): RMS norm of the rows (of the indexed rows) of ``x`` first, in 32 bits. A row without a value of at least 2^-119 is
+    zero; one with a value that is not finite has the scale NaN, and so have all products with it."""
+    _need(x.dim() == 2 and x.dtype in (torch.bfloat16, torch.float16), "bf16 or fp16 rows [T, K] are expected, not %s %s", x.dtype, tuple(x.shape))
+    gamma, eps, idx = (None, 0.0, None) if norm is None else (norm[0], norm[1], norm[2] if len(norm) > 2 else None)
+    rows, cols = x.shape if idx is None else (idx.numel(), x.shape[1])
+    _need(0 < cols and (cols == 1 or x.stride(1) == 1), "the values of a row have to lie side by side")
+    _need(gamma is None or (gamma.numel() == cols and gamma.dtype == x.dtype and gamma.is_contiguous()), "the norm's weights are %d values of the rows' type", cols)
+    _need(idx is None or (idx.dtype == torch.int32 and idx.is_contiguous() and x.shape[0] > 0), "row indices are int32, and x has rows")
+    with _on(x, gamma, idx):
+        q = torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.int8, device=x.device)[:, :cols]
+        scales, sums = torch.empty(rows, dtype=torch.float32, device=x.device), torch.empty(rows, dtype=torch.int32, device=x.device)
+        if rows:
+            a = QuantRowsArgs(x.data_ptr(), _ptr(gamma), _ptr(idx), q.data_ptr(), scales.data_ptr(), sums.data_ptr(), x.stride(0), rows, cols, x.shape[0],
+                              q.stride(0), 1 if x.dtype == torch.float16 else 0, eps)
+            _check(lib().ovb_quantize_rows(C.byref(a), C.c_void_p(_stream())), "ovb_quantize_rows")
+    return QuantizedRows(q, scales, sums, x.dtype)
+
+
+def _gemm_i8(x, w: "PackedWeight", out, residual, act, out_f32, glu, cap, norm) -> torch.Tensor:
+    if isinstance(x, QuantizedRows):
+        _need(norm is None, "rows are normed before they are quantised: give quantize_rows the norm")
+        rows = x
+    else:
+        rows = None
+        _need(x.dim() == 2 and x.dtype in (torch.bfloat16, torch.float16), "bf16 or fp16 rows [T, K] are expected, not %s %s", x.dtype, tuple(x.shape))
+    _need(x.shape[1] == w.K, "rows of %d values for weights of K = %d", x.shape[1], w.K)
+    T = norm[2].numel() if norm is not None and len(norm) > 2 else x.shape[0]
+    cols = w.N // 2 if act in (ACT_SWIGLU, ACT_GLU_LIMITED) else w.N
+    kind = torch.float32 if out_f32 else x.dtype
+    _need(w.bias is None or w.bias.dtype == x.dtype, "the bias is %s, the rows are %s", None if w.bias is None else w.bias.dtype, x.dtype)
+    _need(act != ACT_GLU_LIMITED or (glu is not None and len(glu) == 3), "ACT_GLU_LIMITED needs its limit, slope and shift")
+    for name, t, d in (("out", out, kind), ("residual", residual, x.dtype)):
+        _need(t is None or (t.shape == (T, cols) and t.dtype == d and (cols == 1 or t.stride(1) == 1) and (T == 1 or t.stride(0) >= cols)),
+              "%s has to be %s [%d, %d] with the values of a row side by side", name, d, T, cols)
+    with _on(w.w, out, residual, *((rows.q,) if rows is not None else (x,))):
+        if out is None:
+            out = torch.empty((T, cols), dtype=kind, device=w.w.device)
+        if T == 0:
+            return out
+        if rows is None:
+            rows = quantize_rows(x, norm)
+        a = GemmI8Args(rows.q.data_ptr(), rows.scales.data_ptr(), rows.sums.data_ptr(), w.w.data_ptr(), w.scales.data_ptr(), _ptr(w.zps), _ptr(w.bias), _ptr(residual),
+                       out.data_ptr(), T, w.N, w.K, rows.q.stride(0), max(out.stride(0), cols), max(residual.stride(0), cols) if residual is not None else 0, act,
+                       1 if rows.dtype == torch.float16 else 0, 1 if out_f32 else 0)
+        if act == ACT_GLU_LIMITED:
+            a.act_limit, a.act_slope, a.act_shift = glu
+        elif act == ACT_SOFTCAP:
+            a.act_limit = cap
+        _check(lib().ovb_gemm_i8(C.byref(a), C.c_void_p(_stream())), "ovb_gemm_i8")
+    return out
+
+
 def gemm(x: torch.Tensor, w: PackedWeight, out: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
          act: int = ACT_NONE, out_f32: bool = False, ws: Optional[Workspace] = None, splits: int = 0,
          block_t: int = 0, comm=None, glu=None, cap: float = 0.0, norm=None) -> torch.Tensor:
@@ -356,7 +482,12 @@ def gemm(x: torch.Tensor, w: PackedWeight, out: Optional[torch.Tensor] = None, r
     ``norm`` (weights, eps[, row indices]): RMS norm of the rows (of the indexed rows) of ``x`` before the product, in the product's launch where its kernel takes
     it in and in one of its own otherwise.
     ``glu`` (limit, slope, shift): parameters of ``ACT_GLU_LIMITED``; ``cap``: bound of ``ACT_SOFTCAP``. fp32 weights (``W_F32``) take the product without
-    tensor cores; ``x`` and ``out`` are then fp32."""
+    tensor cores; ``x`` and ``out`` are then fp32. Weights of ``from_ir_i8`` (``W_I8``) are multiplied in whole numbers: ``x`` holds 16-bit rows, which are
+    quantised on the way (after their norm, in 32 bits), or the ``QuantizedRows`` that several products share; such products need no workspace and are not
+    summed over ranks."""
+    if w.mode == W_I8:
+        _need(comm is None and not splits and not block_t, "products of whole numbers take no communicator, split count or token tile")
+        return _gemm_i8(x, w, out, residual, act, out_f32, glu, cap, norm)
     assert x.dim() == 2 and x.stride(1) == 1
     if norm is not None and len(norm) > 2:
         T, K = norm[2].numel(), x.shape[1]
@@ -900,6 +1031,87 @@ def rope_kv_write_u8(qkv, positions, slot_map, k_cache, v_cache, k_meta, v_meta,
                                       C.c_void_p(k_cache.data_ptr()), C.c_void_p(v_cache.data_ptr()), C.c_void_p(k_meta.data_ptr()),
                                       C.c_void_p(v_meta.data_ptr()), C.c_int(T), C.c_int(Hq), C.c_int(Hkv), C.c_int(D), C.c_float(theta),
                                       C.c_int(block_size), C.c_void_p(_stream())), "ovb_rope_kv_write_u8")
+
+
+def _rope_operands(a: QkRopeArgs, dtype, D, inv_freq, q_norm, k_norm, eps, mult, interleaved) -> None:
+    _need(dtype in (torch.bfloat16, torch.float16), "bf16 or fp16 heads are expected, not %s", dtype)
+    _need(inv_freq.dtype == torch.float32 and inv_freq.is_contiguous() and 2 * inv_freq.numel() <= D, "frequencies are fp32, one for each pair of at most %d dimensions", D)
+    for w in (q_norm, k_norm):
+        _need(w is None or (w.numel() == D and w.dtype == dtype and w.is_contiguous()), "a head norm has %d weights of the heads' type", D)
+    a.inv_freq, a.q_norm, a.k_norm = inv_freq.data_ptr(), _ptr(q_norm), _ptr(k_norm)
+    a.D, a.rot, a.interleaved, a.f16, a.eps, a.mult = D, 2 * inv_freq.numel(), 1 if interleaved else 0, 1 if dtype == torch.float16 else 0, eps, mult
+
+
+def qk_norm_rope(q, k, positions, inv_freq, q_norm=None, k_norm=None, eps=1e-6, interleaved=False, mult=1.0, q_out=None, k_out=None):
+    """RMS norm of every query and key head (where it has weights [D]) and rotation by the position, one launch. Returns (q_out, k_out).
+
+    q [B, S, Hq, D] and k [B, S, Hkv, D], bf16 or fp16 (or [S, H, D]): views with any strides whose heads are contiguous; ``positions`` int32 [B, S] or [S].
+    The first 2 * len(``inv_freq``) dimensions turn by positions * inv_freq (fp32; the product is formed in 64 bits), halves paired, or neighbours with
+    ``interleaved``; cos and sin are multiplied by ``mult``. The outputs may be q and k themselves."""
+    if q.dim() == 3:
+        _need(k.dim() == 3 and positions.dim() == 1, "queries [S, H, D] need keys of that form and positions [S]")
+        outs = qk_norm_rope(q[None], k[None], positions, inv_freq, q_norm, k_norm, eps, interleaved, mult, None if q_out is None else q_out[None],
+                            None if k_out is None else k_out[None])
+        return outs[0][0], outs[1][0]
+    _need(q.dim() == 4 and k.dim() == 4 and k.shape[:2] == q.shape[:2] and k.shape[3] == q.shape[3] and k.dtype == q.dtype and min(q.shape[2:]) > 0 and k.shape[2] > 0,
+          "queries [B, S, Hq, D] and keys [B, S, Hkv, D] of one type are expected")
+    B, S, Hq, D = q.shape
+    _need(positions.dtype == torch.int32 and positions.shape in ((S,), (B, S)) and (S == 1 or positions.stride(-1) == 1), "positions are int32 [S] or [B, S]")
+    a = QkRopeArgs()
+    _rope_operands(a, q.dtype, D, inv_freq, q_norm, k_norm, eps, mult, interleaved)
+    with _on(q, k, positions, inv_freq, q_norm, k_norm, q_out, k_out):
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device) if k_out is None else k_out
+        for name, t, like in (("q", q, q), ("k", k, k), ("qo", q_out, q), ("ko", k_out, k)):
+            _need(t.shape == like.shape and t.dtype == like.dtype and t.stride(3) == 1, "heads have to be contiguous, and outputs of their inputs' shape and type")
+            _need(name in ("q", "k") or all(n == 1 or st > 0 for n, st in zip(t.shape, t.stride())), "outputs must not repeat memory")
+            setattr(a, name + "_batch", t.stride(0)), setattr(a, name + "_token", t.stride(1)), setattr(a, name + "_head", t.stride(2))
+        a.q, a.k, a.q_out, a.k_out, a.positions = q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), positions.data_ptr()
+        a.pos_batch = positions.stride(0) if positions.dim() == 2 else 0
+        a.B, a.S, a.Hq, a.Hkv = B, S, Hq, k.shape[2]
+        if B * S:
+            _check(lib().ovb_qk_norm_rope(C.byref(a), C.c_void_p(_stream())), "ovb_qk_norm_rope")
+    return q_out, k_out
+
+
+def qk_norm_rope_kv_write(qkv, positions, slot_map, k_cache, v_cache, inv_freq, Hq, Hkv, D, block_size, q_norm=None, k_norm=None, eps=1e-6, interleaved=False,
+                          mult=1.0, q_out=None, k_meta=None, v_meta=None) -> None:
+    """``qk_norm_rope`` of the rows of a fused projection ``qkv`` [T, (Hq + 2 Hkv) * D], keys and values going to the paged cache.
+
+    Queries go to ``q_out`` [T, Hq * D], by default their own place in ``qkv``; key and value rows to the slots ``slot_map`` (int32, block * block_size +
+    offset; negative: not kept; the slots of a call differ) of the caches [num_blocks, Hkv, block_size, D], which are of the type of ``qkv``, or uint8 with
+    the fp16 (scale, zero point) tables ``k_meta`` / ``v_meta`` [num_blocks, Hkv, block_size, 2] (D and the rotation multiples of 8, D up to 256).
+    A slot behind the cache is not written and shows in the status word."""
+    _need(qkv.dim() == 2 and min(Hq, Hkv, D, block_size) > 0 and qkv.shape[1] >= (Hq + 2 * Hkv) * D and qkv.stride(1) == 1,
+          "rows [T, %d] with their values side by side are expected, not %s", (Hq + 2 * Hkv) * D, tuple(qkv.shape))
+    T = qkv.shape[0]
+    u8 = k_cache.dtype == torch.uint8
+    for name, t in (("positions", positions), ("slot_map", slot_map)):
+        _need(t.dtype == torch.int32 and t.dim() == 1 and t.numel() >= T and t.is_contiguous(), "%s has to hold %d int32 values", name, T)
+    for t in (k_cache, v_cache):
+        _need(t.dim() == 4 and t.shape == (k_cache.shape[0], Hkv, block_size, D) and t.is_contiguous() and t.dtype == (torch.uint8 if u8 else qkv.dtype),
+              "caches are [num_blocks, %d, %d, %d] of the type of qkv, or uint8", Hkv, block_size, D)
+    for t in (k_meta, v_meta):
+        _need(not u8 or (t is not None and t.dtype == torch.float16 and t.shape == (k_cache.shape[0], Hkv, block_size, 2) and t.is_contiguous()),
+              "a uint8 cache needs fp16 tables [num_blocks, %d, %d, 2]", Hkv, block_size)
+    _need(q_out is None or (q_out.dim() == 2 and q_out.shape[0] == T and q_out.shape[1] >= Hq * D and q_out.stride(1) == 1 and q_out.dtype == qkv.dtype
+                            and (T <= 1 or q_out.stride(0) >= Hq * D)), "q_out has to be [%d, %d] of the type of qkv", T, Hq * D)
+    _need(q_out is not None or T <= 1 or qkv.stride(0) >= (Hq + 2 * Hkv) * D, "rows that are written in place must not overlap")
+    a = QkRopeArgs()
+    _rope_operands(a, qkv.dtype, D, inv_freq, q_norm, k_norm, eps, mult, interleaved)
+    with _on(qkv, positions, slot_map, k_cache, v_cache, inv_freq, q_norm, k_norm, q_out, *((k_meta, v_meta) if u8 else ())):
+        q_out = qkv if q_out is None else q_out
+        item = qkv.element_size()
+        a.q, a.k, a.v = (qkv.data_ptr() + n * D * item for n in (0, Hq, Hq + Hkv))
+        a.q_out, a.k_cache, a.v_cache, a.positions, a.slot_map = q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), positions.data_ptr(), slot_map.data_ptr()
+        if u8:
+            a.kv_u8, a.k_meta, a.v_meta = 1, k_meta.data_ptr(), v_meta.data_ptr()
+        a.q_token = a.k_token = a.v_token = qkv.stride(0)
+        a.qo_token = q_out.stride(0)
+        a.q_head = a.k_head = a.v_head = a.qo_head = D
+        a.B, a.S, a.Hq, a.Hkv, a.block_size, a.slots = 1, T, Hq, Hkv, block_size, k_cache.shape[0] * block_size
+        if T:
+            _check(lib().ovb_qk_norm_rope(C.byref(a), C.c_void_p(_stream())), "ovb_qk_norm_rope")
 
 
 def paged_attention(q, k_cache, v_cache, past_lens, subsequence_begins, block_indices, block_indices_begins, Hq, Hkv, D,
