@@ -248,7 +248,7 @@ static int set_up_i8_tile() {
     return 0;
 }
 
-static int run_i8_tile(const ovb_gemm_i8_args* a, I8Params& base, cudaStream_t stream) {
+static int run_i8_tile(const ovb_gemm_i8_args* a, const I8Params& base, cudaStream_t stream) {
     I8TileParams p;
     static_cast<I8Params&>(p) = base;
     p.bt = a->T <= 256 ? (a->T + 15) / 16 * 16 : 256;
@@ -332,6 +332,11 @@ int ovb_gemm_i8(const ovb_gemm_i8_args* a, ovb_stream_t stream_) {
     OVB_REQUIRE(a->residual == nullptr || !a->out_f32, "ovb_gemm_i8: a residual belongs to a 16-bit output");
     const int cols = gated ? a->N / 2 : a->N;
     OVB_REQUIRE(a->ldo >= cols && (a->residual == nullptr || a->ldr >= cols), "ovb_gemm_i8: row pitch of the output %d or residual %d below %d columns", a->ldo, a->ldr, cols);
+    if (a->raw != nullptr) {
+        const ovb_quant_rows_args rows = {a->raw, a->gamma, a->row_idx, const_cast<void*>(a->x), const_cast<float*>(a->x_scale), const_cast<int*>(a->x_sum), a->ld_raw, a->T, a->K,
+                                          a->raw_rows, a->ldx, a->f16, a->eps};
+        if (int rc = ovb_quantize_rows(&rows, stream_)) return rc;
+    }
     I8Params p;
     p.w = static_cast<const uint8_t*>(a->w);
     p.x_scale = a->x_scale;
@@ -347,7 +352,7 @@ int ovb_gemm_i8(const ovb_gemm_i8_args* a, ovb_stream_t stream_) {
     p.ldo = a->ldo; p.ldr = a->ldr;
     p.act = a->act; p.out_f32 = a->out_f32;
     p.act_limit = a->act_limit; p.act_slope = a->act_slope; p.act_shift = a->act_shift;
-    return run_i8_tile(a, p, stream);
+    return a->T > 256 ? gemm_i8_pair(a, p, stream) : run_i8_tile(a, p, stream);
 }
 
 }  // extern "C"

@@ -32,4 +32,7 @@ struct I8Params {
 __device__ __forceinline__ float i8_value(int acc, int zp, int sum, float scale) { return float(acc - zp * sum) * scale; }
 __device__ __forceinline__ bool is_gated(int act) { return act == OVB_ACT_SWIGLU || act == OVB_ACT_GLU_LIMITED; }
 
+// gemm_i8_pair.cu: many tokens, pairs of CTAs.
+int gemm_i8_pair(const ovb_gemm_i8_args* a, const I8Params& p, cudaStream_t stream);
+
 }  // namespace ovb

@@ -166,10 +166,16 @@ typedef struct {
     const void* bias;         // [N] in the 16-bit type, or NULL
     const void* residual;     // 16-bit, pitch ldr, or NULL (may be out itself)
     void* out;                // 16-bit or fp32, pitch ldo
+    /* 16-bit rows that are quantised first, as ovb_quantize_rows does it, or NULL; x, x_scale and x_sum are then memory for the quantised rows */
+    const void* raw;
+    const void* gamma;        // norm on the way, or NULL
+    const int* row_idx;
+    int64_t ld_raw;
     int T, N, K, ldx, ldo, ldr;            // K <= 65536
     int act;                  // OVB_ACT_*; gated ones as in ovb_gemm
     int f16, out_f32;         // the 16-bit type is fp16, otherwise bf16; out is fp32
-    float act_limit, act_slope, act_shift;
+    int raw_rows;             // with row_idx
+    float act_limit, act_slope, act_shift, eps;
 } ovb_gemm_i8_args;
 int ovb_gemm_i8(const ovb_gemm_i8_args* a, ovb_stream_t stream);
 

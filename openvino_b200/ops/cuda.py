@@ -10,6 +10,7 @@ import contextlib
 import ctypes as C
 import math
 import os
+import struct
 import threading
 from pathlib import Path
 from typing import Optional
@@ -144,8 +145,14 @@ class QuantRowsArgs(C.Structure):
 
 
 class GemmI8Args(C.Structure):
-    _fields_ = _fields(("x", "x_scale", "x_sum", "w", "w_scale", "w_zp", "bias", "residual", "out"),
-                       ("T", "N", "K", "ldx", "ldo", "ldr", "act", "f16", "out_f32"), ("act_limit", "act_slope", "act_shift"))
+    _fields_ = (_fields(("x", "x_scale", "x_sum", "w", "w_scale", "w_zp", "bias", "residual", "out", "raw", "gamma", "row_idx"), ()) + [("ld_raw", C.c_int64)]
+                + _fields((), ("T", "N", "K", "ldx", "ldo", "ldr", "act", "f16", "out_f32", "raw_rows"), ("act_limit", "act_slope", "act_shift", "eps")))
+
+
+# The same structures packed by hand: a call of a few microseconds on the device is not to wait for ctypes to fill fields one by one.
+_QUANT_ROWS = struct.Struct("@6Pq5if")
+_GEMM_I8 = struct.Struct("@12Pq10i4f")
+_QK_ROPE = struct.Struct("@14P17q10i2f")
 
 
 class QkRopeArgs(C.Structure):
@@ -188,9 +195,8 @@ def lib():
             l.ovb_llm_step_run.argtypes = [C.POINTER(LlmStep), C.c_void_p]
         if hasattr(l, "ovb_gemm_i8"):
             l.ovb_pack_i8_bytes.restype = C.c_int64
-            l.ovb_gemm_i8.argtypes = [C.POINTER(GemmI8Args), C.c_void_p]
-            l.ovb_quantize_rows.argtypes = [C.POINTER(QuantRowsArgs), C.c_void_p]
-            l.ovb_qk_norm_rope.argtypes = [C.POINTER(QkRopeArgs), C.c_void_p]
+            for fn in (l.ovb_gemm_i8, l.ovb_quantize_rows, l.ovb_qk_norm_rope):
+                fn.argtypes = [C.c_void_p, C.c_void_p]
         l.ovb_pa_scratch_bytes.restype = C.c_int64
         l.ovb_channel_delta_record_floats.restype = C.c_int64
         l.ovb_gemm.argtypes = [C.POINTER(GemmArgs), C.c_void_p]
@@ -380,7 +386,7 @@ class PackedWeight:
         _need(scales.numel() == N and scales.is_floating_point(), "one scale per output channel is expected, not %d %s values for %d channels", scales.numel(), scales.dtype, N)
         _need(zps is None or (zps.numel() == N and zps.dtype == w.dtype), "zero points are one value of the weight's type per output channel")
         _need(bias is None or (bias.numel() == N and bias.dtype in (torch.bfloat16, torch.float16)), "the bias is one 16-bit value per output channel")
-        with _on(w, scales, zps, bias):
+        with torch.cuda.device(_one_device(w, scales, zps, bias)):
             if w.stride(1) != 1 or w.stride(0) < Kd:
                 w = w.contiguous()
             out = torch.empty(int(lib().ovb_pack_i8_bytes(C.c_int(N), C.c_int(Kd))), dtype=torch.uint8, device=w.device)
@@ -397,11 +403,28 @@ def _need(ok: bool, message: str, *args) -> None:
         raise ValueError(message % args)
 
 
-def _on(first: torch.Tensor, *others):
-    """The device of the operands, which have to share one, as the current device."""
-    for t in (first,) + others:
-        _need(t is None or (t.is_cuda and t.device == first.device), "the operands have to be on one CUDA device")
-    return contextlib.nullcontext() if first.device.index == torch.cuda.current_device() else torch.cuda.device(first.device)
+def _one_device(first: torch.Tensor, *others) -> int:
+    """The device of the operands (None among them: not given), which have to share one."""
+    d = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != d:
+            d = -1
+    _need(d >= 0, "the operands have to be on one CUDA device")
+    return d
+
+
+def _call(fn, packed: bytes, device: int, what: str) -> None:
+    """An entry point of the library on ``device``'s current stream."""
+    if device == torch._C._cuda_getDevice():
+        rc = fn(packed, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(packed, torch._C._cuda_getCurrentRawStream(device))
+    if rc:
+        _check(rc, what)
+
+
+_HALVES = (torch.bfloat16, torch.float16)
 
 
 class QuantizedRows:
@@ -418,58 +441,79 @@ class QuantizedRows:
         return self.q.shape
 
 
+def _raw_rows(x: torch.Tensor, norm):
+    """(rows, weights of the norm, eps, row indices) of rows that are to be quantised."""
+    if x.dim() != 2 or x.dtype not in _HALVES:
+        raise ValueError("bf16 or fp16 rows [T, K] are expected, not %s %s" % (x.dtype, tuple(x.shape)))
+    T, cols = x.shape
+    _need(cols > 0 and (x.stride(1) == 1 or cols == 1), "the values of a row have to lie side by side")
+    if norm is None:
+        return T, None, 0.0, None
+    gamma, eps, idx = norm[0], norm[1], norm[2] if len(norm) > 2 else None
+    _need(gamma.numel() == cols and gamma.dtype == x.dtype and gamma.is_contiguous(), "the norm's weights are %d values of the rows' type", cols)
+    if idx is not None:
+        _need(idx.dtype == torch.int32 and idx.is_contiguous() and T > 0, "row indices are int32, and x has rows")
+        T = idx.numel()
+    return T, gamma, eps, idx
+
+
 def quantize_rows(x: torch.Tensor, norm=None) -> QuantizedRows:
     """bf16 or fp16 rows -> signed bytes: with a = max |row|, code = round(value * (127 / a)), halves to even, scale = a / 127.
 
     ``norm`` (weights, eps[, row indices]): RMS norm of the rows (of the indexed rows) of ``x`` first, in 32 bits. A row without a value of at least 2^-119 is
     zero; one with a value that is not finite has the scale NaN, and so have all products with it."""
-    _need(x.dim() == 2 and x.dtype in (torch.bfloat16, torch.float16), "bf16 or fp16 rows [T, K] are expected, not %s %s", x.dtype, tuple(x.shape))
-    gamma, eps, idx = (None, 0.0, None) if norm is None else (norm[0], norm[1], norm[2] if len(norm) > 2 else None)
-    rows, cols = x.shape if idx is None else (idx.numel(), x.shape[1])
-    _need(0 < cols and (cols == 1 or x.stride(1) == 1), "the values of a row have to lie side by side")
-    _need(gamma is None or (gamma.numel() == cols and gamma.dtype == x.dtype and gamma.is_contiguous()), "the norm's weights are %d values of the rows' type", cols)
-    _need(idx is None or (idx.dtype == torch.int32 and idx.is_contiguous() and x.shape[0] > 0), "row indices are int32, and x has rows")
-    with _on(x, gamma, idx):
-        q = torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.int8, device=x.device)[:, :cols]
-        scales, sums = torch.empty(rows, dtype=torch.float32, device=x.device), torch.empty(rows, dtype=torch.int32, device=x.device)
-        if rows:
-            a = QuantRowsArgs(x.data_ptr(), _ptr(gamma), _ptr(idx), q.data_ptr(), scales.data_ptr(), sums.data_ptr(), x.stride(0), rows, cols, x.shape[0],
-                              q.stride(0), 1 if x.dtype == torch.float16 else 0, eps)
-            _check(lib().ovb_quantize_rows(C.byref(a), C.c_void_p(_stream())), "ovb_quantize_rows")
+    T, gamma, eps, idx = _raw_rows(x, norm)
+    d = _one_device(x, gamma, idx)
+    cols = x.shape[1]
+    q = torch.empty((T, (cols + 15) // 16 * 16), dtype=torch.int8, device=x.device)[:, :cols]
+    scales, sums = torch.empty(T, dtype=torch.float32, device=x.device), torch.empty(T, dtype=torch.int32, device=x.device)
+    if T:
+        _call(lib().ovb_quantize_rows, _QUANT_ROWS.pack(x.data_ptr(), _ptr(gamma) or 0, _ptr(idx) or 0, q.data_ptr(), scales.data_ptr(), sums.data_ptr(), x.stride(0), T, cols,
+                                                        x.shape[0], q.stride(0), x.dtype == torch.float16, eps), d, "ovb_quantize_rows")
     return QuantizedRows(q, scales, sums, x.dtype)
 
 
 def _gemm_i8(x, w: "PackedWeight", out, residual, act, out_f32, glu, cap, norm) -> torch.Tensor:
-    if isinstance(x, QuantizedRows):
+    gamma = idx = None
+    eps = 0.0
+    quantized = isinstance(x, QuantizedRows)
+    if quantized:
         _need(norm is None, "rows are normed before they are quantised: give quantize_rows the norm")
-        rows = x
+        T, like = x.shape[0], x.q
     else:
-        rows = None
-        _need(x.dim() == 2 and x.dtype in (torch.bfloat16, torch.float16), "bf16 or fp16 rows [T, K] are expected, not %s %s", x.dtype, tuple(x.shape))
-    _need(x.shape[1] == w.K, "rows of %d values for weights of K = %d", x.shape[1], w.K)
-    T = norm[2].numel() if norm is not None and len(norm) > 2 else x.shape[0]
-    cols = w.N // 2 if act in (ACT_SWIGLU, ACT_GLU_LIMITED) else w.N
-    kind = torch.float32 if out_f32 else x.dtype
-    _need(w.bias is None or w.bias.dtype == x.dtype, "the bias is %s, the rows are %s", None if w.bias is None else w.bias.dtype, x.dtype)
+        T, gamma, eps, idx = _raw_rows(x, norm)
+        like = x
+    N, Kd, dtype, bias, zps = w.N, w.K, x.dtype, w.bias, w.zps
+    if x.shape[1] != Kd:
+        raise ValueError("rows of %d values for weights of K = %d" % (x.shape[1], Kd))
+    cols = N // 2 if act in (ACT_SWIGLU, ACT_GLU_LIMITED) else N
+    kind = torch.float32 if out_f32 else dtype
+    if bias is not None and bias.dtype != dtype:
+        raise ValueError("the bias is %s, the rows are %s" % (bias.dtype, dtype))
     _need(act != ACT_GLU_LIMITED or (glu is not None and len(glu) == 3), "ACT_GLU_LIMITED needs its limit, slope and shift")
-    for name, t, d in (("out", out, kind), ("residual", residual, x.dtype)):
-        _need(t is None or (t.shape == (T, cols) and t.dtype == d and (cols == 1 or t.stride(1) == 1) and (T == 1 or t.stride(0) >= cols)),
-              "%s has to be %s [%d, %d] with the values of a row side by side", name, d, T, cols)
-    with _on(w.w, out, residual, *((rows.q,) if rows is not None else (x,))):
-        if out is None:
-            out = torch.empty((T, cols), dtype=kind, device=w.w.device)
-        if T == 0:
-            return out
-        if rows is None:
-            rows = quantize_rows(x, norm)
-        a = GemmI8Args(rows.q.data_ptr(), rows.scales.data_ptr(), rows.sums.data_ptr(), w.w.data_ptr(), w.scales.data_ptr(), _ptr(w.zps), _ptr(w.bias), _ptr(residual),
-                       out.data_ptr(), T, w.N, w.K, rows.q.stride(0), max(out.stride(0), cols), max(residual.stride(0), cols) if residual is not None else 0, act,
-                       1 if rows.dtype == torch.float16 else 0, 1 if out_f32 else 0)
-        if act == ACT_GLU_LIMITED:
-            a.act_limit, a.act_slope, a.act_shift = glu
-        elif act == ACT_SOFTCAP:
-            a.act_limit = cap
-        _check(lib().ovb_gemm_i8(C.byref(a), C.c_void_p(_stream())), "ovb_gemm_i8")
+    for name, t, of in (("out", out, kind), ("residual", residual, dtype)):
+        if t is not None and not (t.shape == (T, cols) and t.dtype == of and (cols == 1 or t.stride(1) == 1) and (T == 1 or t.stride(0) >= cols)):
+            raise ValueError("%s has to be %s [%d, %d] with the values of a row side by side" % (name, of, T, cols))
+    d = _one_device(like, w.w, gamma, idx, out, residual)
+    if out is None:
+        out = torch.empty((T, cols), dtype=kind, device=like.device)
+    if T == 0:
+        return out
+    if quantized:
+        pitch, q, scales, sums, raw, ld_raw = x.q.stride(0), x.q.data_ptr(), x.scales.data_ptr(), x.sums.data_ptr(), 0, 0
+    else:
+        # the quantised rows, their scales and sums: memory of the caching allocator, which belongs to the stream
+        pitch = (Kd + 15) // 16 * 16
+        rows = torch.empty(T * (pitch + 8), dtype=torch.uint8, device=like.device)
+        q = rows.data_ptr()
+        scales, raw, ld_raw = q + T * pitch, x.data_ptr(), x.stride(0)
+        sums = scales + 4 * T
+    limit, slope, shift = glu if act == ACT_GLU_LIMITED else (cap, 0.0, 0.0)
+    _call(lib().ovb_gemm_i8, _GEMM_I8.pack(q, scales, sums, w.w.data_ptr(), w.scales.data_ptr(), 0 if zps is None else zps.data_ptr(), 0 if bias is None else bias.data_ptr(),
+                                           0 if residual is None else residual.data_ptr(), out.data_ptr(), raw, 0 if gamma is None else gamma.data_ptr(),
+                                           0 if idx is None else idx.data_ptr(), ld_raw, T, N, Kd, pitch, max(out.stride(0), cols),
+                                           0 if residual is None else max(residual.stride(0), cols), act, dtype == torch.float16, bool(out_f32), x.shape[0], limit, slope, shift,
+                                           eps), d, "ovb_gemm_i8")
     return out
 
 
@@ -1033,13 +1077,27 @@ def rope_kv_write_u8(qkv, positions, slot_map, k_cache, v_cache, k_meta, v_meta,
                                       C.c_int(block_size), C.c_void_p(_stream())), "ovb_rope_kv_write_u8")
 
 
-def _rope_operands(a: QkRopeArgs, dtype, D, inv_freq, q_norm, k_norm, eps, mult, interleaved) -> None:
-    _need(dtype in (torch.bfloat16, torch.float16), "bf16 or fp16 heads are expected, not %s", dtype)
-    _need(inv_freq.dtype == torch.float32 and inv_freq.is_contiguous() and 2 * inv_freq.numel() <= D, "frequencies are fp32, one for each pair of at most %d dimensions", D)
+def _rope_operands(dtype, D, inv_freq, q_norm, k_norm) -> int:
+    """Checks what both forms share; the dimensions that turn."""
+    if dtype not in _HALVES:
+        raise ValueError("bf16 or fp16 heads are expected, not %s" % dtype)
+    rot = 2 * inv_freq.numel()
+    _need(inv_freq.dtype == torch.float32 and inv_freq.is_contiguous() and rot <= D, "frequencies are fp32, one for each pair of at most %d dimensions", D)
     for w in (q_norm, k_norm):
-        _need(w is None or (w.numel() == D and w.dtype == dtype and w.is_contiguous()), "a head norm has %d weights of the heads' type", D)
-    a.inv_freq, a.q_norm, a.k_norm = inv_freq.data_ptr(), _ptr(q_norm), _ptr(k_norm)
-    a.D, a.rot, a.interleaved, a.f16, a.eps, a.mult = D, 2 * inv_freq.numel(), 1 if interleaved else 0, 1 if dtype == torch.float16 else 0, eps, mult
+        if w is not None and not (w.numel() == D and w.dtype == dtype and w.is_contiguous()):
+            raise ValueError("a head norm has %d weights of the heads' type" % D)
+    return rot
+
+
+def _written_once(t: torch.Tensor) -> bool:
+    """No two elements of a tensor with contiguous heads share memory, by its strides alone: every dimension steps over all that the smaller ones span."""
+    span = 0
+    for st, n in sorted(zip(t.stride(), t.shape)):
+        if n > 1:
+            if st <= span:
+                return False
+            span += st * (n - 1)
+    return True
 
 
 def qk_norm_rope(q, k, positions, inv_freq, q_norm=None, k_norm=None, eps=1e-6, interleaved=False, mult=1.0, q_out=None, k_out=None):
@@ -1053,24 +1111,28 @@ def qk_norm_rope(q, k, positions, inv_freq, q_norm=None, k_norm=None, eps=1e-6, 
         outs = qk_norm_rope(q[None], k[None], positions, inv_freq, q_norm, k_norm, eps, interleaved, mult, None if q_out is None else q_out[None],
                             None if k_out is None else k_out[None])
         return outs[0][0], outs[1][0]
-    _need(q.dim() == 4 and k.dim() == 4 and k.shape[:2] == q.shape[:2] and k.shape[3] == q.shape[3] and k.dtype == q.dtype and min(q.shape[2:]) > 0 and k.shape[2] > 0,
-          "queries [B, S, Hq, D] and keys [B, S, Hkv, D] of one type are expected")
-    B, S, Hq, D = q.shape
-    _need(positions.dtype == torch.int32 and positions.shape in ((S,), (B, S)) and (S == 1 or positions.stride(-1) == 1), "positions are int32 [S] or [B, S]")
-    a = QkRopeArgs()
-    _rope_operands(a, q.dtype, D, inv_freq, q_norm, k_norm, eps, mult, interleaved)
-    with _on(q, k, positions, inv_freq, q_norm, k_norm, q_out, k_out):
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device) if k_out is None else k_out
-        for name, t, like in (("q", q, q), ("k", k, k), ("qo", q_out, q), ("ko", k_out, k)):
-            _need(t.shape == like.shape and t.dtype == like.dtype and t.stride(3) == 1, "heads have to be contiguous, and outputs of their inputs' shape and type")
-            _need(name in ("q", "k") or all(n == 1 or st > 0 for n, st in zip(t.shape, t.stride())), "outputs must not repeat memory")
-            setattr(a, name + "_batch", t.stride(0)), setattr(a, name + "_token", t.stride(1)), setattr(a, name + "_head", t.stride(2))
-        a.q, a.k, a.q_out, a.k_out, a.positions = q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), positions.data_ptr()
-        a.pos_batch = positions.stride(0) if positions.dim() == 2 else 0
-        a.B, a.S, a.Hq, a.Hkv = B, S, Hq, k.shape[2]
-        if B * S:
-            _check(lib().ovb_qk_norm_rope(C.byref(a), C.c_void_p(_stream())), "ovb_qk_norm_rope")
+    dtype = q.dtype
+    _need(q.dim() == 4 and k.dim() == 4 and k.dtype == dtype, "queries [B, S, Hq, D] and keys [B, S, Hkv, D] of one type are expected")
+    (B, S, Hq, D), (kB, kS, Hkv, kD) = q.shape, k.shape
+    _need(kB == B and kS == S and kD == D and Hq > 0 and Hkv > 0 and D > 0, "queries [B, S, Hq, D] and keys [B, S, Hkv, D] are expected, not %s and %s", tuple(q.shape), tuple(k.shape))
+    many = positions.dim() == 2
+    _need(positions.dtype == torch.int32 and positions.shape == ((B, S) if many else (S,)) and (S == 1 or positions.stride(-1) == 1), "positions are int32 [S] or [B, S]")
+    rot = _rope_operands(dtype, D, inv_freq, q_norm, k_norm)
+    for t, like in ((q_out, q), (k_out, k)):
+        if t is not None and not (t.shape == like.shape and t.dtype == dtype and _written_once(t)):
+            raise ValueError("outputs have their inputs' shape and type, and no two elements in one place")
+    d = _one_device(q, k, positions, inv_freq, q_norm, k_norm, q_out, k_out)
+    if q_out is None:
+        q_out = torch.empty((B, S, Hq, D), dtype=dtype, device=q.device)
+    if k_out is None:
+        k_out = torch.empty((B, S, Hkv, D), dtype=dtype, device=q.device)
+    qs, ks, qo, ko = q.stride(), k.stride(), q_out.stride(), k_out.stride()
+    _need(qs[3] == 1 and ks[3] == 1 and qo[3] == 1 and ko[3] == 1, "heads have to be contiguous")
+    if B * S:
+        _call(lib().ovb_qk_norm_rope, _QK_ROPE.pack(q.data_ptr(), k.data_ptr(), 0, q_out.data_ptr(), k_out.data_ptr(), 0, 0, 0, 0, positions.data_ptr(), 0, inv_freq.data_ptr(),
+                                                    0 if q_norm is None else q_norm.data_ptr(), 0 if k_norm is None else k_norm.data_ptr(), qs[0], qs[1], qs[2], ks[0], ks[1], ks[2],
+                                                    0, 0, 0, qo[0], qo[1], qo[2], ko[0], ko[1], ko[2], positions.stride(0) if many else 0, 0, B, S, Hq, Hkv, D, rot, 0,
+                                                    bool(interleaved), dtype == torch.float16, 0, eps, mult), d, "ovb_qk_norm_rope")
     return q_out, k_out
 
 
@@ -1082,36 +1144,36 @@ def qk_norm_rope_kv_write(qkv, positions, slot_map, k_cache, v_cache, inv_freq, 
     offset; negative: not kept; the slots of a call differ) of the caches [num_blocks, Hkv, block_size, D], which are of the type of ``qkv``, or uint8 with
     the fp16 (scale, zero point) tables ``k_meta`` / ``v_meta`` [num_blocks, Hkv, block_size, 2] (D and the rotation multiples of 8, D up to 256).
     A slot behind the cache is not written and shows in the status word."""
-    _need(qkv.dim() == 2 and min(Hq, Hkv, D, block_size) > 0 and qkv.shape[1] >= (Hq + 2 * Hkv) * D and qkv.stride(1) == 1,
-          "rows [T, %d] with their values side by side are expected, not %s", (Hq + 2 * Hkv) * D, tuple(qkv.shape))
-    T = qkv.shape[0]
-    u8 = k_cache.dtype == torch.uint8
-    for name, t in (("positions", positions), ("slot_map", slot_map)):
-        _need(t.dtype == torch.int32 and t.dim() == 1 and t.numel() >= T and t.is_contiguous(), "%s has to hold %d int32 values", name, T)
+    dtype, u8 = qkv.dtype, k_cache.dtype == torch.uint8
+    width = (Hq + 2 * Hkv) * D
+    _need(qkv.dim() == 2 and min(Hq, Hkv, D, block_size) > 0 and qkv.shape[1] >= width and qkv.stride(1) == 1, "rows [T, %d] with their values side by side are expected, not %s",
+          width, tuple(qkv.shape))
+    T, pitch = qkv.shape[0], qkv.stride(0)
+    for t in (positions, slot_map):
+        if not (t.dtype == torch.int32 and t.dim() == 1 and t.numel() >= T and t.is_contiguous()):
+            raise ValueError("positions and slots are int32, %d values at least" % T)
+    blocks = k_cache.shape[0]
     for t in (k_cache, v_cache):
-        _need(t.dim() == 4 and t.shape == (k_cache.shape[0], Hkv, block_size, D) and t.is_contiguous() and t.dtype == (torch.uint8 if u8 else qkv.dtype),
-              "caches are [num_blocks, %d, %d, %d] of the type of qkv, or uint8", Hkv, block_size, D)
-    for t in (k_meta, v_meta):
-        _need(not u8 or (t is not None and t.dtype == torch.float16 and t.shape == (k_cache.shape[0], Hkv, block_size, 2) and t.is_contiguous()),
-              "a uint8 cache needs fp16 tables [num_blocks, %d, %d, 2]", Hkv, block_size)
-    _need(q_out is None or (q_out.dim() == 2 and q_out.shape[0] == T and q_out.shape[1] >= Hq * D and q_out.stride(1) == 1 and q_out.dtype == qkv.dtype
-                            and (T <= 1 or q_out.stride(0) >= Hq * D)), "q_out has to be [%d, %d] of the type of qkv", T, Hq * D)
-    _need(q_out is not None or T <= 1 or qkv.stride(0) >= (Hq + 2 * Hkv) * D, "rows that are written in place must not overlap")
-    a = QkRopeArgs()
-    _rope_operands(a, qkv.dtype, D, inv_freq, q_norm, k_norm, eps, mult, interleaved)
-    with _on(qkv, positions, slot_map, k_cache, v_cache, inv_freq, q_norm, k_norm, q_out, *((k_meta, v_meta) if u8 else ())):
-        q_out = qkv if q_out is None else q_out
-        item = qkv.element_size()
-        a.q, a.k, a.v = (qkv.data_ptr() + n * D * item for n in (0, Hq, Hq + Hkv))
-        a.q_out, a.k_cache, a.v_cache, a.positions, a.slot_map = q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), positions.data_ptr(), slot_map.data_ptr()
-        if u8:
-            a.kv_u8, a.k_meta, a.v_meta = 1, k_meta.data_ptr(), v_meta.data_ptr()
-        a.q_token = a.k_token = a.v_token = qkv.stride(0)
-        a.qo_token = q_out.stride(0)
-        a.q_head = a.k_head = a.v_head = a.qo_head = D
-        a.B, a.S, a.Hq, a.Hkv, a.block_size, a.slots = 1, T, Hq, Hkv, block_size, k_cache.shape[0] * block_size
-        if T:
-            _check(lib().ovb_qk_norm_rope(C.byref(a), C.c_void_p(_stream())), "ovb_qk_norm_rope")
+        if not (t.shape == (blocks, Hkv, block_size, D) and t.dtype == (torch.uint8 if u8 else dtype) and t.is_contiguous()):
+            raise ValueError("caches are contiguous [num_blocks, %d, %d, %d] of the type of qkv, or uint8" % (Hkv, block_size, D))
+    if u8:
+        for t in (k_meta, v_meta):
+            _need(t is not None and t.dtype == torch.float16 and t.shape == (blocks, Hkv, block_size, 2) and t.is_contiguous(),
+                  "a uint8 cache needs fp16 tables [num_blocks, %d, %d, 2]", Hkv, block_size)
+    rot = _rope_operands(dtype, D, inv_freq, q_norm, k_norm)
+    if q_out is None:
+        _need(T <= 1 or pitch >= width, "rows that are written in place must not overlap")
+        q_out = qkv
+    elif not (q_out.dim() == 2 and q_out.shape[0] == T and q_out.shape[1] >= Hq * D and q_out.stride(1) == 1 and q_out.dtype == dtype and (T <= 1 or q_out.stride(0) >= Hq * D)):
+        raise ValueError("q_out has to be [%d, %d] of the type of qkv" % (T, Hq * D))
+    d = _one_device(qkv, positions, slot_map, k_cache, v_cache, inv_freq, q_norm, k_norm, q_out, *((k_meta, v_meta) if u8 else ()))
+    if T:
+        at, head = qkv.data_ptr(), D * 2
+        _call(lib().ovb_qk_norm_rope, _QK_ROPE.pack(at, at + Hq * head, at + (Hq + Hkv) * head, q_out.data_ptr(), 0, k_cache.data_ptr(), v_cache.data_ptr(), k_meta.data_ptr() if u8 else 0,
+                                                    v_meta.data_ptr() if u8 else 0, positions.data_ptr(), slot_map.data_ptr(), inv_freq.data_ptr(),
+                                                    0 if q_norm is None else q_norm.data_ptr(), 0 if k_norm is None else k_norm.data_ptr(), 0, pitch, D, 0, pitch, D, 0, pitch, D,
+                                                    0, q_out.stride(0), D, 0, 0, 0, 0, blocks * block_size, 1, T, Hq, Hkv, D, rot, block_size, bool(interleaved),
+                                                    dtype == torch.float16, u8, eps, mult), d, "ovb_qk_norm_rope")
 
 
 def paged_attention(q, k_cache, v_cache, past_lens, subsequence_begins, block_indices, block_indices_begins, Hq, Hkv, D,
