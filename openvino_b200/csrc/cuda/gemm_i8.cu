@@ -7,71 +7,141 @@
 // the kernel that wrote the tokens has finished. The partial sums are integers: they go to shared memory as [token][channel], every CTA of the cluster
 // adds up its share of the tokens over all partials and finishes them, lanes along the channels.
 #include <mutex>
+#include <stdlib.h>
+#include <type_traits>
 
 #include "gemm_i8.cuh"
 
 namespace ovb {
 
-constexpr int kI8Threads = 128;
 constexpr int kI8MaxStages = 12;
+constexpr int kI8QuantWarps = 8;
+constexpr int kI8Hold = 8;                          // pieces of eight columns of a row that a quantising thread holds
+constexpr int kI8FusedTokens = 8;
+constexpr int i8_threads(bool fused) { return fused ? 64 + kI8QuantWarps * 32 : 256; }
+constexpr int kI8FusedBlock = 16 * kI8BlockK;       // a k-block of the codes
 
 struct I8TileParams : I8Params {
-    int bt, stages, splits;
+    int bt, stages, splits, early, prefetch;
+    int whole;                    // 16-bit results and residuals in groups of four aligned columns
+    // quantisation in the kernel
+    const void* raw;
+    const void* gamma;
+    const int* row_idx;
+    int64_t ld_raw;
+    int raw_rows;
+    float eps;
 };
 
+// Up to eight rows, quantised by eight warps into the swizzled operand of the MMA ([k-block][16 rows][128 bytes]; the last eight rows are not set, their
+// sums are not read). Every CTA needs the largest magnitude of whole rows, so it reads them whole, and keeps the codes of its k-blocks. All rows go at a
+// time, each to eight, four, two warps or one, which hold it in registers.
 template <class E>
-__device__ __forceinline__ void i8_store4(const I8Params& p, int t, int col, int cols, float (&v)[4]) {
-    // four adjacent columns of a token: one 8- or 16-byte access where all of them exist and the place is aligned
-    if (p.residual != nullptr) {
-        const E* r = static_cast<const E*>(p.residual) + (size_t)t * p.ldr + col;
-        if (col + 4 <= cols && (reinterpret_cast<uintptr_t>(r) & 7) == 0) {
-            const uint2 raw = __ldcg(reinterpret_cast<const uint2*>(r));
-            const E* e = reinterpret_cast<const E*>(&raw);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] += to_float(e[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (col + i < cols) v[i] += to_float(r[i]);
-        }
+__device__ __forceinline__ void i8_quantize_rows(const I8TileParams& p, uint8_t* codes, int kb0, int kb1, float* row_scale, int* row_sum, float* box_f, uint32_t* box_u, int* box_i) {
+    const int tid = threadIdx.x - 64, warp = tid >> 5, lane = tid & 31, pieces = p.K >> 3;
+    const int wpr = p.T == 1 ? 8 : p.T == 2 ? 4 : p.T <= 4 ? 2 : 1, span = wpr * 32;        // warps and threads of a row
+    const int t = warp / wpr, first_warp = t * wpr, at0 = tid - first_warp * 32;
+    auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(kI8QuantWarps * 32) : "memory"); };
+    const bool live = t < p.T;
+    uint4 x[kI8Hold], g[kI8Hold];
+    int row = t;
+    if (live && p.row_idx != nullptr) {
+        row = p.row_idx[t];
+        if (row < 0 || row >= p.raw_rows) row = 0;
     }
-    if (p.out_f32) {
-        float* o = static_cast<float*>(p.out) + (size_t)t * p.ldo + col;
-        if (col + 4 <= cols && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
-            *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
-        } else {
+    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const E*>(p.raw) + row * p.ld_raw);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (col + i < cols) o[i] = v[i];
-        }
-        return;
+    for (int h = 0; h < kI8Hold; ++h) {
+        const int at = at0 + h * span;
+        x[h] = live && at < pieces ? __ldcg(src + at) : make_uint4(0, 0, 0, 0);
+        if (p.gamma != nullptr && live && at < pieces) g[h] = __ldg(static_cast<const uint4*>(p.gamma) + at);
     }
-    E* o = static_cast<E*>(p.out) + (size_t)t * p.ldo + col;
-    E e[4] = {from_float<E>(v[0]), from_float<E>(v[1]), from_float<E>(v[2]), from_float<E>(v[3])};
-    if (col + 4 <= cols && (reinterpret_cast<uintptr_t>(o) & 7) == 0) {
-        *reinterpret_cast<uint2*>(o) = *reinterpret_cast<uint2*>(e);
-    } else {
+    float inv = 1.f;
+    if (p.gamma != nullptr) {
+        float ss = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (col + i < cols) o[i] = e[i];
+        for (int h = 0; h < kI8Hold; ++h) {
+            const E* e = reinterpret_cast<const E*>(&x[h]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) ss = fmaf(to_float(e[j]), to_float(e[j]), ss);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (lane == 0) box_f[warp] = ss;
+        meet();
+        ss = 0.f;
+        for (int w = 0; w < wpr; ++w) ss += box_f[first_warp + w];
+        inv = rsqrtf(ss / (float)p.K + p.eps);
+    }
+    auto value = [&](int h, int j) {
+        const float v = to_float(reinterpret_cast<const E*>(&x[h])[j]);
+        return p.gamma != nullptr ? v * inv * to_float(reinterpret_cast<const E*>(&g[h])[j]) : v;
+    };
+    uint32_t top = 0;
+#pragma unroll
+    for (int h = 0; h < kI8Hold; ++h)
+        if (live && at0 + h * span < pieces) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = max(top, magnitude(value(h, j)));
+        }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) box_u[warp] = top;
+    meet();
+    top = 0;
+    for (int w = 0; w < wpr; ++w) top = max(top, box_u[first_warp + w]);
+    const float f = row_factor(top);
+    int sum = 0;
+#pragma unroll
+    for (int h = 0; h < kI8Hold; ++h) {
+        const int at = at0 + h * span, kb = at >> 4;
+        const bool mine = kb >= kb0 && kb < kb1;
+        if (!live || at >= pieces || (!mine && p.w_zp == nullptr)) continue;
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int c = f != 0.f ? __float2int_rn(__fmul_rn(value(h, j), f)) : 0;
+            sum += c;
+            w[j >> 2] |= (uint32_t)(c & 0xFF) << (8 * (j & 3));
+        }
+        if (mine) *reinterpret_cast<uint2*>(codes + (kb - kb0) * kI8FusedBlock + t * 128 + ((((at & 15) >> 1) ^ t) << 4) + ((at & 1) << 3)) = make_uint2(w[0], w[1]);
+    }
+    if (p.w_zp != nullptr) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) box_i[warp] = sum;
+    }
+    fence_proxy_async_smem();                           // the codes are read by the tensor cores
+    meet();
+    if (live && at0 == 0) {
+        row_scale[t] = row_scale_of(top);
+        sum = 0;
+        if (p.w_zp != nullptr)
+            for (int w = 0; w < wpr; ++w) sum += box_i[first_warp + w];
+        row_sum[t] = sum;
     }
 }
 
-template <bool F16>
-__global__ void __launch_bounds__(kI8Threads) gemm_i8_tile_kernel(const __grid_constant__ CUtensorMap tmX, const I8TileParams p) {
+template <bool F16, bool FUSED, int FORM>
+__global__ void __launch_bounds__(i8_threads(FUSED)) gemm_i8_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ I8TileParams p) {
     using E = typename Elem<F16>::type;
+    constexpr int WARPS = i8_threads(FUSED) / 32;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    const int stage_bytes = kI8TileBytes + p.bt * kI8BlockK;
-    __shared__ uint64_t full[kI8MaxStages], empty[kI8MaxStages], done;
+    __shared__ uint64_t full[kI8MaxStages], empty[kI8MaxStages], done, rows_ready;
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
+    __shared__ float row_scale[FUSED ? kI8FusedTokens : 256];
+    __shared__ int row_sum[FUSED ? kI8FusedTokens : 256];
     volatile int* abort_flag = &abort_word;
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // the shuffle tells the compiler that a warp's index is the same in all lanes: the MMA loop below then runs on uniform registers
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int split = blockIdx.x % p.splits, tile = blockIdx.x / p.splits;      // a cluster is the splits of one tile
     const int n0 = tile * TILE_N, t0 = blockIdx.y * p.bt;
     const int kb0 = (int)((int64_t)p.KB * split / p.splits), kb1 = (int)((int64_t)p.KB * (split + 1) / p.splits);
+    const int stage_bytes = kI8TileBytes + (FUSED ? 0 : p.bt * kI8BlockK);
+    uint8_t* stages = FUSED ? smem + (kb1 - kb0) * kI8FusedBlock : smem;                // fused: the rows' codes come first
     const uint32_t tmem_cols = p.bt <= 32 ? 32u : p.bt <= 64 ? 64u : p.bt <= 128 ? 128u : 256u;
     if (threadIdx.x == 0) {
         for (int s = 0; s < p.stages; ++s) {
@@ -79,9 +149,10 @@ __global__ void __launch_bounds__(kI8Threads) gemm_i8_tile_kernel(const __grid_c
             mbar_init(&empty[s], 1);
         }
         mbar_init(&done, 1);
+        mbar_init(&rows_ready, 1);
         abort_word = 0;
         mbar_fence_init();
-        tma_prefetch_desc(&tmX);
+        if (!FUSED) tma_prefetch_desc(&tmX);
     }
     if (warp == 1) {
         tmem_alloc(&tmem_slot, tmem_cols);
@@ -91,6 +162,7 @@ __global__ void __launch_bounds__(kI8Threads) gemm_i8_tile_kernel(const __grid_c
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = tmem_slot;
+    if (p.early) pdl_trigger();
 
     if (warp == 0) {
         if (lane == 0) {
@@ -98,56 +170,84 @@ __global__ void __launch_bounds__(kI8Threads) gemm_i8_tile_kernel(const __grid_c
             const int n = kb1 - kb0, ahead = n < p.stages ? n : p.stages;
             for (int i = 0; i < ahead; ++i) {           // weights are constants: they come before the tokens may be read
                 mbar_arrive_expect_tx(&full[i], (uint32_t)stage_bytes);
-                bulk_load_1d(smem + i * stage_bytes, w + (size_t)i * kI8TileBytes, kI8TileBytes, &full[i]);
+                bulk_load_1d(stages + i * stage_bytes, w + (size_t)i * kI8TileBytes, kI8TileBytes, &full[i]);
             }
-            pdl_wait();
-            for (int i = 0; i < ahead; ++i) tma_load_2d(smem + i * stage_bytes + kI8TileBytes, &tmX, &full[i], (kb0 + i) * kI8BlockK, t0);
+            int fetched = min(n, ahead + p.prefetch);   // chunks that have been asked for, into shared memory or L2
+            for (int i = ahead; i < fetched; ++i) bulk_prefetch_l2(w + (size_t)i * kI8TileBytes, kI8TileBytes);
+            if (!FUSED) {
+                pdl_wait();
+                for (int i = 0; i < ahead; ++i) tma_load_2d(stages + i * stage_bytes + kI8TileBytes, &tmX, &full[i], (kb0 + i) * kI8BlockK, t0);
+            }
             int s = 0;
             uint32_t phase = 0;
             for (int i = ahead; i < n; ++i) {
                 if (!mbar_wait(&empty[s], phase, abort_flag, p.status)) break;
+                if (fetched < n) bulk_prefetch_l2(w + (size_t)fetched++ * kI8TileBytes, kI8TileBytes);
                 mbar_arrive_expect_tx(&full[s], (uint32_t)stage_bytes);
-                bulk_load_1d(smem + s * stage_bytes, w + (size_t)i * kI8TileBytes, kI8TileBytes, &full[s]);
-                tma_load_2d(smem + s * stage_bytes + kI8TileBytes, &tmX, &full[s], (kb0 + i) * kI8BlockK, t0);
+                bulk_load_1d(stages + s * stage_bytes, w + (size_t)i * kI8TileBytes, kI8TileBytes, &full[s]);
+                if (!FUSED) tma_load_2d(stages + s * stage_bytes + kI8TileBytes, &tmX, &full[s], (kb0 + i) * kI8BlockK, t0);
                 if (++s == p.stages) { s = 0; phase ^= 1; }
             }
-            if (OVB_PDL_GEMM) pdl_trigger();
+            if (FUSED) pdl_wait();
+            if (OVB_PDL_GEMM && !p.early) pdl_trigger();
         }
         __syncwarp();
     } else if (warp == 1) {
         const uint32_t idesc = umma_idesc_i8(TILE_N, p.bt);
         int s = 0;
         uint32_t phase = 0;
-        bool ok = true;
+        // no way out of the loop: once a wait has run out all later ones return at once, and what is computed then is not stored
+        if (FUSED) mbar_wait(&rows_ready, 0, abort_flag, p.status);
         for (int kb = kb0; kb < kb1; ++kb) {
-            ok = mbar_wait(&full[s], phase, abort_flag, p.status);
-            if (!ok) break;
+            mbar_wait(&full[s], phase, abort_flag, p.status);
             tc_fence_after_sync();
-            const uint32_t a = smem_u32(smem) + s * stage_bytes;
-            const uint64_t da = umma_desc_k_sw128(a, 1024), db = umma_desc_k_sw128(a + kI8TileBytes, 1024);
-#pragma unroll
-            for (int k = 0; k < kI8BlockK / 32; ++k) umma_i8_ss_elect(tmem, da + 2 * k, db + 2 * k, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
-            umma_commit_elect(&empty[s]);
+            const uint32_t a = smem_u32(stages) + s * stage_bytes;
+            const uint64_t da = umma_desc_k_sw128(a, 1024), db = umma_desc_k_sw128(FUSED ? smem_u32(smem) + (kb - kb0) * kI8FusedBlock : a + kI8TileBytes, 1024);
+            umma_i8_block_elect(tmem, da, db, idesc, kb > kb0 ? 1u : 0u, &empty[s]);
             if (++s == p.stages) { s = 0; phase ^= 1; }
         }
-        if (ok) umma_commit_elect(&done);
+        umma_commit_elect(&done);
         __syncwarp();
+    } else if (FUSED) {
+        __shared__ float box_f[8];
+        __shared__ uint32_t box_u[8];
+        __shared__ int box_i[8];
+        pdl_wait();
+        i8_quantize_rows<E>(p, smem, kb0, kb1, row_scale, row_sum, box_f, box_u, box_i);
+        if (threadIdx.x == 64) mbar_arrive(&rows_ready);
     }
-    // every thread reads what the kernel before this one wrote (the tokens' scales), or writes over what it read
+    // while the products run: the scales of this thread's four channels and of the tokens (which the kernel before this one may have written)
+    const int n = n0 + lane * 4;
+    float ws[4], b[4];
+    int zp[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const bool in = n + i < p.N;
+        ws[i] = in ? __ldg(p.w_scale + n + i) : 0.f;
+        zp[i] = in && p.w_zp != nullptr ? __ldg(p.w_zp + n + i) : 0;
+        b[i] = in && p.bias != nullptr ? to_float(static_cast<const E*>(p.bias)[n + i]) : 0.f;
+    }
     pdl_wait();
+    const int tokens = min(p.bt, p.T - t0);
+    if (!FUSED)
+        for (int t = threadIdx.x; t < tokens; t += WARPS * 32) {
+            row_scale[t] = __ldcg(p.x_scale + t0 + t);
+            row_sum[t] = __ldcg(p.x_sum + t0 + t);
+        }
     mbar_wait(&done, 0, abort_flag, p.status);
     __syncthreads();
     const bool fine = *abort_flag == 0;
     // every copy has landed and every MMA has read its operands: the stages hold the partial sums now
-    int* part = reinterpret_cast<int*>(smem);           // [bt][128]
-    if (fine) {
+    int* part = reinterpret_cast<int*>(stages);         // [bt][128]
+    if (fine && warp < 8) {
         tc_fence_after_sync();
-        for (int c = 0; c < p.bt; c += 16) {
+        const int q = warp & 3;
+        for (int c = (warp >> 2) * 16; c < p.bt; c += 32) {
             uint32_t r[16];
-            tmem_ld_x16(tmem + (uint32_t(warp * 32) << 16) + c, r);
+            tmem_ld_x16(tmem + (uint32_t(q * 32) << 16) + c, r);
             tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) part[(c + j) * TILE_N + warp * 32 + lane] = (int)r[j];
+            for (int j = 0; j < 16; ++j) part[(c + j) * TILE_N + q * 32 + lane] = (int)r[j];
         }
     }
     tc_fence_before_sync();
@@ -158,48 +258,84 @@ __global__ void __launch_bounds__(kI8Threads) gemm_i8_tile_kernel(const __grid_c
         __syncthreads();
     }
     if (fine) {
-        const int tokens = min(p.bt, p.T - t0), share0 = tokens * split / p.splits, share1 = tokens * (split + 1) / p.splits;
-        const bool gated = is_gated(p.act);
-        const int n = n0 + lane * 4;
-        float ws[4], b[4];
-        int zp[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const bool in = n + i < p.N;
-            ws[i] = in ? __ldg(p.w_scale + n + i) : 0.f;
-            zp[i] = in && p.w_zp != nullptr ? __ldg(p.w_zp + n + i) : 0;
-            b[i] = in && p.bias != nullptr ? to_float(static_cast<const E*>(p.bias)[n + i]) : 0.f;
-        }
+        const int share0 = tokens * split / p.splits, share1 = tokens * (split + 1) / p.splits;
         const uint32_t mine = smem_u32(part) + lane * 16;
-        for (int t = share0 + warp; t < share1; t += kI8Threads / 32) {
-            int4 a = make_int4(0, 0, 0, 0);
-            if (p.splits > 1) {
-                for (int r = 0; r < p.splits; ++r) {
-                    const float4 f = ld_dsmem_f4(dsmem_addr(mine + t * (TILE_N * 4), (uint32_t)r));
-                    a.x += __float_as_int(f.x); a.y += __float_as_int(f.y); a.z += __float_as_int(f.z); a.w += __float_as_int(f.w);
-                }
-            } else {
-                a = *reinterpret_cast<const int4*>(part + t * TILE_N + lane * 4);
-            }
-            const float xs = __ldcg(p.x_scale + t0 + t);
-            const int sum = p.w_zp != nullptr ? __ldcg(p.x_sum + t0 + t) : 0;
-            float v[4] = {i8_value(a.x, zp[0], sum, xs * ws[0]) + b[0], i8_value(a.y, zp[1], sum, xs * ws[1]) + b[1],
-                          i8_value(a.z, zp[2], sum, xs * ws[2]) + b[2], i8_value(a.w, zp[3], sum, xs * ws[3]) + b[3]};
-            if (gated) {
-                // rows 0 .. 63 of the tile are the gate, 64 .. 127 the up values of the same channels
-                float u[4];
+        constexpr bool GATED = i8_gated_form(FORM);
+        const int cols = GATED ? p.N >> 1 : p.N, col = GATED ? (n0 >> 1) + lane * 4 : n, left = GATED && lane >= 16 ? 0 : cols - col;
+        // S partials of as many tokens as give sixteen loads in flight. WHOLE: 16-bit results, four columns of a row in one aligned access.
+        auto finish = [&](auto count, auto kind) {
+            constexpr int S = decltype(count)::value, AT_ONCE = S == 1 ? 4 : 16 / S;
+            constexpr bool WHOLE = decltype(kind)::value;
+            uint32_t from[S];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) u[i] = __shfl_down_sync(0xffffffffu, v[i], 16);
-                if (lane < 16) {
+            for (int r = 0; r < S; ++r) from[r] = S == 1 ? mine : dsmem_addr(mine, (uint32_t)r);
+#pragma unroll 1
+            for (int first = share0 + warp; first < share1; first += WARPS * AT_ONCE) {
+                float4 f[AT_ONCE][S];
+                uint2 res[AT_ONCE];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) v[i] = p.act == OVB_ACT_SWIGLU ? v[i] / (1.0f + __expf(-v[i])) * u[i] : glu_limited(p, v[i], u[i]);
-                    i8_store4<E>(p, t0 + t, (n0 >> 1) + lane * 4, p.N >> 1, v);
+                for (int i = 0; i < AT_ONCE; ++i) {
+                    const int t = min(first + i * WARPS, share1 - 1);          // the last one again, where there are no more
+#pragma unroll
+                    for (int r = 0; r < S; ++r) f[i][r] = S == 1 ? *reinterpret_cast<const float4*>(part + t * TILE_N + lane * 4) : ld_dsmem_f4(from[r] + t * (TILE_N * 4));
+                    if (WHOLE && !GATED) {
+                        res[i] = make_uint2(0, 0);
+                        if (p.residual != nullptr && left > 0) res[i] = __ldcg(reinterpret_cast<const uint2*>(static_cast<const E*>(p.residual) + (size_t)(t0 + t) * p.ldr + col));
+                    }
                 }
-            } else {
-                apply_act_n(v, p);
-                i8_store4<E>(p, t0 + t, n, p.N, v);
+#pragma unroll
+                for (int i = 0; i < AT_ONCE; ++i) {
+                    const int t = min(first + i * WARPS, share1 - 1);
+                    int a[4] = {0, 0, 0, 0};
+#pragma unroll
+                    for (int r = 0; r < S; ++r) {
+                        a[0] += __float_as_int(f[i][r].x);
+                        a[1] += __float_as_int(f[i][r].y);
+                        a[2] += __float_as_int(f[i][r].z);
+                        a[3] += __float_as_int(f[i][r].w);
+                    }
+                    const float xs = row_scale[t];
+                    const int sum = row_sum[t];
+                    float v[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] = i8_value<FORM>(a[j], zp[j], sum, xs * ws[j], b[j]);
+                    if (GATED) {
+                        // rows 0 .. 63 of the tile are the gate, 64 .. 127 the up values of the same channels
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) v[j] = i8_gate(p, v[j], __shfl_down_sync(0xffffffffu, v[j], 16));
+                    }
+                    if (FORM == kI8Any && p.act != OVB_ACT_NONE) apply_act_n(v, p);
+                    const size_t at = (size_t)(t0 + t) * p.ldo + col;
+                    if (WHOLE) {
+                        if (!GATED && p.residual != nullptr) {
+                            const E* e = reinterpret_cast<const E*>(&res[i]);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) v[j] += to_float(e[j]);
+                        }
+                        if (left > 0 && first + i * WARPS < share1) *reinterpret_cast<uint2*>(static_cast<E*>(p.out) + at) = make_uint2(pack_pair<E>(v[0], v[1]), pack_pair<E>(v[2], v[3]));
+                    } else {
+                        if (first + i * WARPS >= share1) continue;              // a residual in place is added once
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (j < left) {
+                                if (p.residual != nullptr) v[j] += to_float(static_cast<const E*>(p.residual)[(size_t)(t0 + t) * p.ldr + col + j]);
+                                if (p.out_f32) static_cast<float*>(p.out)[at + j] = v[j];
+                                else static_cast<E*>(p.out)[at + j] = from_float<E>(v[j]);
+                            }
+                    }
+                }
             }
-        }
+        };
+        auto finish_as = [&](auto kind) {
+            switch (p.splits) {
+                case 1: finish(std::integral_constant<int, 1>(), kind); break;
+                case 2: finish(std::integral_constant<int, 2>(), kind); break;
+                case 4: finish(std::integral_constant<int, 4>(), kind); break;
+                default: finish(std::integral_constant<int, 8>(), kind); break;
+            }
+        };
+        if (p.whole) finish_as(std::true_type());
+        else finish_as(std::false_type());
     }
     if (p.splits > 1) {             // a CTA's partials stay until the others have read them
         cluster_arrive();
@@ -234,41 +370,76 @@ __global__ void __launch_bounds__(256) pack_i8_kernel(const uint8_t* __restrict_
     }
 }
 
-template <bool F16>
-static int set_up_i8_tile() {
+static int env_int(const char* n, int d) { const char* v = getenv(n); return v ? atoi(v) : d; }
+
+template <bool F16, bool FUSED, int FORM>
+static int launch_i8_tile(const cudaLaunchConfig_t& cfg, const CUtensorMap& tm, const I8TileParams& p) {
     static std::mutex mu;
     static bool known[64] = {false};
     int dev = 0;
     OVB_CHECK_CUDA(cudaGetDevice(&dev));
-    std::lock_guard<std::mutex> lk(mu);
-    if (!known[dev & 63]) {
-        OVB_CHECK_CUDA(cudaFuncSetAttribute(gemm_i8_tile_kernel<F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
+    {
+        std::lock_guard<std::mutex> lk(mu);
+        if (!known[dev & 63]) OVB_CHECK_CUDA(cudaFuncSetAttribute(gemm_i8_tile_kernel<F16, FUSED, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
         known[dev & 63] = true;
     }
+    OVB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, gemm_i8_tile_kernel<F16, FUSED, FORM>, tm, p));
     return 0;
 }
+template <bool F16, bool FUSED>
+static int launch_i8_tile(int form, const cudaLaunchConfig_t& cfg, const CUtensorMap& tm, const I8TileParams& p) {
+    switch (form) {
+        case kI8Plain: return launch_i8_tile<F16, FUSED, kI8Plain>(cfg, tm, p);
+        case kI8Gated: return launch_i8_tile<F16, FUSED, kI8Gated>(cfg, tm, p);
+        case kI8GatedZp: return launch_i8_tile<F16, FUSED, kI8GatedZp>(cfg, tm, p);
+        default: return launch_i8_tile<F16, FUSED, kI8Any>(cfg, tm, p);
+    }
+}
 
-static int run_i8_tile(const ovb_gemm_i8_args* a, const I8Params& base, cudaStream_t stream) {
+// Rows that the kernel quantises itself: whole aligned pieces of eight columns, as many as six warps hold.
+static bool i8_fuses(const ovb_gemm_i8_args* a) {
+    const auto bits = [](const void* x) { return reinterpret_cast<uintptr_t>(x); };
+    const int rows = a->T <= 2 ? a->T : a->T <= 4 ? 4 : 8;       // as the warps share them
+    return a->raw != nullptr && a->T <= kI8FusedTokens && a->K % 8 == 0 && rows * a->K <= kI8QuantWarps * 32 * kI8Hold * 8 && (a->T == 1 || a->ld_raw % 8 == 0) &&
+           ((bits(a->raw) | bits(a->gamma)) & 15) == 0 && env_int("OVB_I8_FUSE", 1);
+}
+
+static int run_i8_tile(const ovb_gemm_i8_args* a, const I8Params& base, bool fused, cudaStream_t stream) {
     I8TileParams p;
     static_cast<I8Params&>(p) = base;
-    p.bt = a->T <= 256 ? (a->T + 15) / 16 * 16 : 256;
+    const auto bits = [](const void* x) { return reinterpret_cast<uintptr_t>(x); };
+    p.whole = !a->out_f32 && a->N % 4 == 0 && a->ldo % 4 == 0 && (bits(a->out) & 7) == 0 && (a->residual == nullptr || (a->ldr % 4 == 0 && (bits(a->residual) & 7) == 0));
+    p.raw = a->raw;
+    p.gamma = a->gamma;
+    p.row_idx = a->row_idx;
+    p.ld_raw = a->ld_raw;
+    p.raw_rows = a->raw_rows;
+    p.eps = a->eps;
+    p.bt = fused ? 16 : a->T <= 256 ? (a->T + 15) / 16 * 16 : 256;
+    p.bt = fused ? p.bt : env_int("OVB_I8_BT", p.bt);
     const int tiles = ceil_div(a->N, TILE_N), rows = ceil_div(a->T, p.bt);
     p.splits = 1;
     while (p.splits < 8 && (int64_t)tiles * rows * p.splits * 2 <= 160 && p.KB >= p.splits * 2) p.splits *= 2;
-    const int stage = kI8TileBytes + p.bt * kI8BlockK;
+    p.splits = env_int("OVB_I8_S", p.splits);
+    if (p.splits > p.KB) p.splits = p.KB;
     const int per_split = ceil_div(p.KB, p.splits);
-    p.stages = (216 * 1024) / stage;
+    const int stage = kI8TileBytes + (fused ? 0 : p.bt * kI8BlockK), head = fused ? per_split * kI8FusedBlock : 0;
+    p.stages = (env_int("OVB_I8_KB", 216) * 1024 - head) / stage;
     if (p.stages > kI8MaxStages) p.stages = kI8MaxStages;
     if (p.stages > per_split) p.stages = per_split;
+    if (p.stages < 1) p.stages = 1;
     int bytes = p.stages * stage;
     if (bytes < p.bt * TILE_N * 4) bytes = p.bt * TILE_N * 4;
     CUtensorMap tm;
-    if (int rc = make_tmap_2d(&tm, a->x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a->T, a->K, a->ldx, p.bt, kI8BlockK, true)) return rc;
+    if (fused) memset(&tm, 0, sizeof(tm));
+    else if (int rc = make_tmap_2d(&tm, a->x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a->T, a->K, a->ldx, p.bt, kI8BlockK, true)) return rc;
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3(tiles * p.splits, rows);
-    cfg.blockDim = dim3(kI8Threads);
-    cfg.dynamicSmemBytes = bytes + 1024;
+    cfg.blockDim = dim3(i8_threads(fused));
+    p.early = env_int("OVB_I8_EARLY", 0);
+    p.prefetch = env_int("OVB_I8_PF", 16);
+    cfg.dynamicSmemBytes = head + bytes + 1024;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     int n = 0;
@@ -285,14 +456,9 @@ static int run_i8_tile(const ovb_gemm_i8_args* a, const I8Params& base, cudaStre
     }
     cfg.attrs = attr;
     cfg.numAttrs = n;
-    if (a->f16) {
-        if (int rc = set_up_i8_tile<true>()) return rc;
-        OVB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, gemm_i8_tile_kernel<true>, tm, p));
-    } else {
-        if (int rc = set_up_i8_tile<false>()) return rc;
-        OVB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, gemm_i8_tile_kernel<false>, tm, p));
-    }
-    return 0;
+    const int form = i8_form(a);
+    if (fused) return a->f16 ? launch_i8_tile<true, true>(form, cfg, tm, p) : launch_i8_tile<false, true>(form, cfg, tm, p);
+    return a->f16 ? launch_i8_tile<true, false>(form, cfg, tm, p) : launch_i8_tile<false, false>(form, cfg, tm, p);
 }
 
 }  // namespace ovb
@@ -332,7 +498,8 @@ int ovb_gemm_i8(const ovb_gemm_i8_args* a, ovb_stream_t stream_) {
     OVB_REQUIRE(a->residual == nullptr || !a->out_f32, "ovb_gemm_i8: a residual belongs to a 16-bit output");
     const int cols = gated ? a->N / 2 : a->N;
     OVB_REQUIRE(a->ldo >= cols && (a->residual == nullptr || a->ldr >= cols), "ovb_gemm_i8: row pitch of the output %d or residual %d below %d columns", a->ldo, a->ldr, cols);
-    if (a->raw != nullptr) {
+    const bool fused = i8_fuses(a);
+    if (a->raw != nullptr && !fused) {
         const ovb_quant_rows_args rows = {a->raw, a->gamma, a->row_idx, const_cast<void*>(a->x), const_cast<float*>(a->x_scale), const_cast<int*>(a->x_sum), a->ld_raw, a->T, a->K,
                                           a->raw_rows, a->ldx, a->f16, a->eps};
         if (int rc = ovb_quantize_rows(&rows, stream_)) return rc;
@@ -352,7 +519,7 @@ int ovb_gemm_i8(const ovb_gemm_i8_args* a, ovb_stream_t stream_) {
     p.ldo = a->ldo; p.ldr = a->ldr;
     p.act = a->act; p.out_f32 = a->out_f32;
     p.act_limit = a->act_limit; p.act_slope = a->act_slope; p.act_shift = a->act_shift;
-    return a->T > 256 ? gemm_i8_pair(a, p, stream) : run_i8_tile(a, p, stream);
+    return a->T > env_int("OVB_I8_PAIR", 256) ? gemm_i8_pair(a, p, stream) : run_i8_tile(a, p, fused, stream);
 }
 
 }  // extern "C"

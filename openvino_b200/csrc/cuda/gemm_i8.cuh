@@ -29,8 +29,56 @@ struct I8Params {
     float act_limit, act_slope, act_shift;
 };
 
-__device__ __forceinline__ float i8_value(int acc, int zp, int sum, float scale) { return float(acc - zp * sum) * scale; }
-__device__ __forceinline__ bool is_gated(int act) { return act == OVB_ACT_SWIGLU || act == OVB_ACT_GLU_LIMITED; }
+// Quantisation of a row y (x, or x * rsqrt(mean(x^2) + eps) * gamma):  a = max |y|;  q = round_half_even(y * (127 / a));  scale = a / 127;  sum = sum q.
+// Quotients and products are rounded to 32 bits once each. |y| * (127 / a) is at most 127 (1 + 2^-23), so no value has to be clamped. A row whose largest
+// magnitude is below 2^-119, where 127 / a would not be finite, counts as zero (scale 0); one with a value that is not finite gets the scale NaN and codes of
+// zero, so that every result of the row is NaN. The magnitudes are compared as integers, where NaN is the largest.
+constexpr uint32_t kNotFinite = 0x7F800000u;
+constexpr float kQuantFloor = 1.5046327690525280e-36f;      // 2^-119
+
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+__device__ __forceinline__ float row_scale_of(uint32_t top) {
+    const float a = __uint_as_float(top);
+    return top >= kNotFinite ? __int_as_float(0x7FFFFFFF) : a < kQuantFloor ? 0.f : __fdiv_rn(a, 127.f);
+}
+// 127 / a, or 0 where the row has no codes
+__device__ __forceinline__ float row_factor(uint32_t top) {
+    const float a = __uint_as_float(top);
+    return top >= kNotFinite || a < kQuantFloor ? 0.f : __fdiv_rn(127.f, a);
+}
+
+__host__ __device__ inline bool is_gated(int act) { return act == OVB_ACT_SWIGLU || act == OVB_ACT_GLU_LIMITED; }
+
+// Forms of the epilogues. The code of one form is short: the uniform branches of an epilogue for all activations, which jump over long unrolled pieces, cost
+// more than its arithmetic (512 x 4096 x 4096: 8100 of 31000 cycles with them).
+constexpr int kI8Plain = 0;       // neither activation nor bias nor zero points
+constexpr int kI8Gated = 1;       // gated, no zero points
+constexpr int kI8GatedZp = 2;
+constexpr int kI8Any = 3;         // not gated, all of them
+constexpr bool i8_gated_form(int form) { return form == kI8Gated || form == kI8GatedZp; }
+constexpr bool i8_zp_form(int form) { return form == kI8GatedZp || form == kI8Any; }
+inline int i8_form(const ovb_gemm_i8_args* a) {
+    if (is_gated(a->act)) return a->w_zp != nullptr ? kI8GatedZp : kI8Gated;
+    return a->act == OVB_ACT_NONE && a->bias == nullptr && a->w_zp == nullptr ? kI8Plain : kI8Any;
+}
+template <int FORM>
+__device__ __forceinline__ float i8_value(int acc, int zp, int sum, float scale, float bias) {
+    const float v = float(i8_zp_form(FORM) ? acc - zp * sum : acc);
+    return FORM == kI8Any ? fmaf(v, scale, bias) : v * scale;
+}
+template <class E>
+__device__ __forceinline__ uint32_t pack_pair(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float a, float b) { return pack_bf16x2(a, b); }
+template <>
+__device__ __forceinline__ uint32_t pack_pair<__half>(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <class P>
+__device__ __forceinline__ float i8_gate(const P& p, float g, float u) {
+    return p.act == OVB_ACT_SWIGLU ? __fdividef(g, 1.0f + __expf(-g)) * u : glu_limited(p, g, u);
+}
 
 // gemm_i8_pair.cu: many tokens, pairs of CTAs.
 int gemm_i8_pair(const ovb_gemm_i8_args* a, const I8Params& p, cudaStream_t stream);

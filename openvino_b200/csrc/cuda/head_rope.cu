@@ -8,8 +8,8 @@
 // 4e-3 off, more than a bf16 rounding of the result. The angles of a token are the same for all heads: a block computes them once, in shared
 // memory, while its first heads are on their way. Sums, norms and rotation are held in 32 bits, every result is rounded once.
 //
-// What bounds it: memory, each head read and written once. Eight elements of a head, two pieces of four, lie in one lane: the pair of a
-// dimension is in the same lane, and the lanes of a head (8, 16 or 32) need shuffles for the sum of squares only.
+// What bounds it: memory, each head read and written once. A lane holds two pieces of a head: the partner of a
+// dimension is in the same lane, and the lanes of a head need shuffles for the sum of squares only.
 #include "gemm_common.cuh"
 
 namespace ovb {
@@ -19,8 +19,8 @@ struct HeadRopeParams : ovb_qk_rope_args {
     int heads, per_block;         // all heads of a token; heads of a block
 };
 
-constexpr int kRopeThreads = 256;
-constexpr int kRopeBatch = 4;     // heads that a group of lanes has in flight
+constexpr int kRopeThreads = 128;
+constexpr int kRopeBatch = 2;     // heads that a group of lanes has in flight
 
 __device__ __forceinline__ float2 turn_of(int position, float inv_freq, float mult) {
     const double turns = (double)position * (double)inv_freq * 0.15915494309189533577;
@@ -29,159 +29,186 @@ __device__ __forceinline__ float2 turn_of(int position, float inv_freq, float mu
     return make_float2(c * mult, s * mult);
 }
 
-struct HeadAt {
-    const void* src;              // + element
-    void* dst;                    // NULL: not kept
-    __half2* meta;
-    int kind;                     // 0 query, 1 key, 2 value
+// Where a token's heads are: a base for each kind, steps between heads.
+template <class E>
+struct TokenRows {
+    const E* src[3];
+    uint8_t* dst[3];              // NULL: not kept
+    int64_t src_step[3], dst_step[3];      // elements, bytes
+    int64_t row;                  // of the first key (value) head in the cache
+    bool outside;                 // the slot is behind the cache
 };
 
 template <class E, bool U8>
-__device__ __forceinline__ HeadAt head_at(const HeadRopeParams& p, int b, int s, int h, int64_t slot) {
-    HeadAt r;
-    r.meta = nullptr;
-    if (h < p.Hq) {
-        r.kind = 0;
-        r.src = static_cast<const E*>(p.q) + b * p.q_batch + s * p.q_token + h * p.q_head;
-        r.dst = static_cast<E*>(p.q_out) + b * p.qo_batch + s * p.qo_token + h * p.qo_head;
+__device__ __forceinline__ TokenRows<E> token_rows(const HeadRopeParams& p, int t) {
+    TokenRows<E> r;
+    const int b = t / p.S, s = t - b * p.S;
+    r.src[0] = static_cast<const E*>(p.q) + b * p.q_batch + s * p.q_token;
+    r.src[1] = static_cast<const E*>(p.k) + b * p.k_batch + s * p.k_token;
+    r.src[2] = static_cast<const E*>(p.v) + b * p.v_batch + s * p.v_token;
+    r.src_step[0] = p.q_head;
+    r.src_step[1] = p.k_head;
+    r.src_step[2] = p.v_head;
+    r.dst[0] = reinterpret_cast<uint8_t*>(static_cast<E*>(p.q_out) + b * p.qo_batch + s * p.qo_token);
+    r.dst_step[0] = p.qo_head * (int)sizeof(E);
+    r.row = 0;
+    r.outside = false;
+    if (p.k_cache == nullptr) {
+        r.dst[1] = reinterpret_cast<uint8_t*>(static_cast<E*>(p.k_out) + b * p.ko_batch + s * p.ko_token);
+        r.dst_step[1] = p.ko_head * (int)sizeof(E);
+        r.dst[2] = nullptr;
+        r.dst_step[2] = 0;
         return r;
     }
-    const bool value = h >= p.Hq + p.Hkv;
-    const int g = value ? h - p.Hq - p.Hkv : h - p.Hq;
-    r.kind = value ? 2 : 1;
-    r.src = value ? static_cast<const E*>(p.v) + b * p.v_batch + s * p.v_token + g * p.v_head : static_cast<const E*>(p.k) + b * p.k_batch + s * p.k_token + g * p.k_head;
-    if (p.k_cache == nullptr) {
-        r.dst = static_cast<E*>(p.k_out) + b * p.ko_batch + s * p.ko_token + g * p.ko_head;
-    } else if (slot < 0) {
-        r.dst = nullptr;
-    } else {
-        const int64_t row = (slot / p.block_size * p.Hkv + g) * p.block_size + slot % p.block_size;
-        void* cache = value ? p.v_cache : p.k_cache;
-        r.dst = U8 ? static_cast<void*>(static_cast<uint8_t*>(cache) + row * p.D) : static_cast<void*>(static_cast<E*>(cache) + row * p.D);
-        if (U8) r.meta = static_cast<__half2*>(value ? p.v_meta : p.k_meta) + row;
-    }
+    const int slot = p.slot_map[t], size = U8 ? 1 : (int)sizeof(E);
+    const bool inside = slot < p.slots;
+    r.outside = !inside;
+    const int blk = slot / p.block_size, off = slot - blk * p.block_size;
+    r.row = (int64_t)blk * p.Hkv * p.block_size + off;
+    r.dst[1] = slot >= 0 && inside ? static_cast<uint8_t*>(p.k_cache) + r.row * p.D * size : nullptr;
+    r.dst[2] = slot >= 0 && inside ? static_cast<uint8_t*>(p.v_cache) + r.row * p.D * size : nullptr;
+    r.dst_step[1] = r.dst_step[2] = (int64_t)p.block_size * p.D * size;
     return r;
 }
 
-// The slot of a token, -1 where its rows are not kept.
-__device__ __forceinline__ int64_t slot_of(const HeadRopeParams& p, int t) {
-    if (p.k_cache == nullptr) return -1;
-    const int slot = p.slot_map[t];
-    if (slot >= p.slots) {
-        if (threadIdx.x == 0) report_status(p.status, STATUS_BAD_INDEX);
-        return -1;
+// CH elements side by side, 8 or 16 bytes.
+template <class E, int CH>
+struct Piece {
+    uint32_t w[CH / 2];
+    __device__ __forceinline__ void load(const E* src) {
+        if (CH == 8) {
+            const uint4 v = *reinterpret_cast<const uint4*>(src);
+            w[0] = v.x; w[1] = v.y; w[CH / 2 - 2] = v.z; w[CH / 2 - 1] = v.w;
+        } else {
+            const uint2 v = *reinterpret_cast<const uint2*>(src);
+            w[0] = v.x; w[1] = v.y;
+        }
     }
-    return slot;
-}
-
-template <class E>
-__device__ __forceinline__ void unpack4(uint2 raw, float (&v)[4]) {
-    const E* e = reinterpret_cast<const E*>(&raw);
+    __device__ __forceinline__ void store(void* dst) const {
+        if (CH == 8) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[CH / 2 - 2], w[CH / 2 - 1]);
+        else *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+    }
+    __device__ __forceinline__ void unpack(float (&v)[CH]) const {
+        const E* e = reinterpret_cast<const E*>(w);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = to_float(e[i]);
-}
-template <class E>
-__device__ __forceinline__ uint2 pack4(const float (&v)[4]) {
-    E e[4] = {from_float<E>(v[0]), from_float<E>(v[1]), from_float<E>(v[2]), from_float<E>(v[3])};
-    return *reinterpret_cast<uint2*>(e);
-}
+        for (int i = 0; i < CH; ++i) v[i] = to_float(e[i]);
+    }
+    __device__ __forceinline__ void pack(const float (&v)[CH]) {
+#pragma unroll
+        for (int i = 0; i < CH; i += 2) {
+            E e[2] = {from_float<E>(v[i]), from_float<E>(v[i + 1])};
+            w[i / 2] = *reinterpret_cast<const uint32_t*>(e);
+        }
+    }
+};
 
-// Head sizes that are multiples of 8 up to 256, rotations that are multiples of 8, aligned heads. LANES lanes share a head.
-template <class E, bool INTER, int LANES, bool U8>
-__global__ void __launch_bounds__(kRopeThreads) head_rope_kernel(const __grid_constant__ HeadRopeParams p) {
+// Heads and rotations of whole pieces, aligned heads. LANES lanes share a head, each with two pieces of CH elements: the partners of its CH pairs, or 2 CH
+// neighbours.
+template <class E, bool INTER, int CH, int LANES, bool U8>
+__global__ void __launch_bounds__(kRopeThreads, 8) head_rope_kernel(const __grid_constant__ HeadRopeParams p) {
     __shared__ float2 turn[128];
     constexpr int GROUPS = kRopeThreads / LANES;
-    const int t = blockIdx.x, b = t / p.S, s = t - b * p.S;
+    const int t = blockIdx.x;
     const int group = threadIdx.x / LANES, l = threadIdx.x % LANES;
     const int h_begin = blockIdx.y * p.per_block, h_end = min(p.heads, h_begin + p.per_block);
-    const bool own = l * 8 < p.D;                       // this lane has elements
-    const int pair0 = l * 4, half = p.rot >> 1;
+    const bool own = l * 2 * CH < p.D;                  // this lane has elements
+    const int pair0 = l * CH, half = p.rot >> 1;
     const bool turns = own && pair0 < half;
-    // the two pieces of four elements; behind the rotated dimensions, and in the interleaved form, they are neighbours
-    const int o0 = turns && !INTER ? pair0 : pair0 * 2, o1 = turns && !INTER ? half + pair0 : pair0 * 2 + 4;
+    // behind the rotated dimensions, and in the interleaved form, the two pieces are neighbours
+    const int o0 = turns && !INTER ? pair0 : pair0 * 2, o1 = turns && !INTER ? half + pair0 : pair0 * 2 + CH;
     pdl_enter();
-    float wq[8], wk[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) wq[j] = wk[j] = 1.f;
-    if (own && p.q_norm != nullptr) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) wq[j] = to_float(static_cast<const E*>(p.q_norm)[(j < 4 ? o0 : o1 - 4) + j]);
-    }
-    if (own && p.k_norm != nullptr) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) wk[j] = to_float(static_cast<const E*>(p.k_norm)[(j < 4 ? o0 : o1 - 4) + j]);
-    }
-    const int64_t slot = slot_of(p, t);
-    const int position = p.positions[b * p.pos_batch + s];
+    const TokenRows<E> rows = token_rows<E, U8>(p, t);
+    auto kind_of = [&](int h) { return h < p.Hq ? 0 : h < p.Hq + p.Hkv ? 1 : 2; };
+    auto index_of = [&](int h, int kind) { return kind == 0 ? h : kind == 1 ? h - p.Hq : h - p.Hq - p.Hkv; };
+    auto pick = [&](const auto& of, int kind) { return kind == 0 ? of[0] : kind == 1 ? of[1] : of[2]; };
+    float cs[CH], sn[CH];
     bool have_turns = false;
     for (int base = h_begin; base < h_end; base += GROUPS * kRopeBatch) {
-        uint2 r0[kRopeBatch], r1[kRopeBatch];
+        Piece<E, CH> r0[kRopeBatch], r1[kRopeBatch];
 #pragma unroll
         for (int i = 0; i < kRopeBatch; ++i) {
             const int h = base + i * GROUPS + group;
-            r0[i] = r1[i] = make_uint2(0, 0);
             if (h < h_end && own) {
-                const E* src = static_cast<const E*>(head_at<E, U8>(p, b, s, h, slot).src);
-                r0[i] = *reinterpret_cast<const uint2*>(src + o0);
-                r1[i] = *reinterpret_cast<const uint2*>(src + o1);
+                const int kind = kind_of(h);
+                const E* src = pick(rows.src, kind) + index_of(h, kind) * pick(rows.src_step, kind);
+                r0[i].load(src + o0);
+                r1[i].load(src + o1);
+            } else {
+#pragma unroll
+                for (int j = 0; j < CH / 2; ++j) r0[i].w[j] = r1[i].w[j] = 0;
             }
         }
         if (!have_turns) {
-            if ((int)threadIdx.x < half) turn[threadIdx.x] = turn_of(position, p.inv_freq[threadIdx.x], p.mult);
+            const int b = t / p.S, s = t - b * p.S;
+            if ((int)threadIdx.x < half) turn[threadIdx.x] = turn_of(p.positions[b * p.pos_batch + s], p.inv_freq[threadIdx.x], p.mult);
             __syncthreads();
             have_turns = true;
+            if (rows.outside && threadIdx.x == 0) report_status(p.status, STATUS_BAD_INDEX);
+#pragma unroll
+            for (int j = 0; j < CH; ++j) {
+                const float2 u = turns ? turn[pair0 + j] : make_float2(1.f, 0.f);
+                cs[j] = u.x;
+                sn[j] = u.y;
+            }
         }
 #pragma unroll
         for (int i = 0; i < kRopeBatch; ++i) {
             const int h = base + i * GROUPS + group;
             if (base + i * GROUPS >= h_end) break;      // the same for all threads of the block
             const bool live = h < h_end && own;
-            const HeadAt at = head_at<E, U8>(p, b, s, h < h_end ? h : h_begin, slot);
-            float a[4], c[4];
-            unpack4<E>(r0[i], a);
-            unpack4<E>(r1[i], c);
-            const bool norm = at.kind == 0 ? p.q_norm != nullptr : at.kind == 1 && p.k_norm != nullptr;
+            const int kind = kind_of(h);
+            float a[CH], c[CH];
+            r0[i].unpack(a);
+            r1[i].unpack(c);
+            const E* weight = static_cast<const E*>(kind == 0 ? p.q_norm : kind == 1 ? p.k_norm : nullptr);
             if (p.q_norm != nullptr || p.k_norm != nullptr) {
                 float ss = 0.f;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) ss = fmaf(a[j], a[j], fmaf(c[j], c[j], ss));
+                for (int j = 0; j < CH; ++j) ss = fmaf(a[j], a[j], fmaf(c[j], c[j], ss));
 #pragma unroll
                 for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                if (norm) {
+                if (weight != nullptr && own) {
                     const float inv = rsqrtf(ss / (float)p.D + p.eps);
+                    Piece<E, CH> w0, w1;                // the same lines for all heads: they stay in L1
+                    float wa[CH], wc[CH];
+                    w0.load(weight + o0);
+                    w1.load(weight + o1);
+                    w0.unpack(wa);
+                    w1.unpack(wc);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        a[j] = a[j] * inv * (at.kind == 0 ? wq[j] : wk[j]);
-                        c[j] = c[j] * inv * (at.kind == 0 ? wq[4 + j] : wk[4 + j]);
+                    for (int j = 0; j < CH; ++j) {
+                        a[j] = a[j] * inv * wa[j];
+                        c[j] = c[j] * inv * wc[j];
                     }
                 }
             }
-            if (turns && at.kind != 2) {
+            if (turns && kind != 2) {
                 if (INTER) {
 #pragma unroll
-                    for (int j = 0; j < 4; j += 2) {
-                        const float2 u = turn[pair0 + (j >> 1)], w = turn[pair0 + 2 + (j >> 1)];
+                    for (int j = 0; j < CH; j += 2) {
                         const float a0 = a[j], c0 = c[j];
-                        a[j] = a0 * u.x - a[j + 1] * u.y;
-                        a[j + 1] = a[j + 1] * u.x + a0 * u.y;
-                        c[j] = c0 * w.x - c[j + 1] * w.y;
-                        c[j + 1] = c[j + 1] * w.x + c0 * w.y;
+                        a[j] = a0 * cs[j / 2] - a[j + 1] * sn[j / 2];
+                        a[j + 1] = a[j + 1] * cs[j / 2] + a0 * sn[j / 2];
+                        c[j] = c0 * cs[(CH + j) / 2] - c[j + 1] * sn[(CH + j) / 2];
+                        c[j + 1] = c[j + 1] * cs[(CH + j) / 2] + c0 * sn[(CH + j) / 2];
                     }
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float2 u = turn[pair0 + j];
+                    for (int j = 0; j < CH; ++j) {
                         const float a0 = a[j];
-                        a[j] = a0 * u.x - c[j] * u.y;
-                        c[j] = c[j] * u.x + a0 * u.y;
+                        a[j] = a0 * cs[j] - c[j] * sn[j];
+                        c[j] = c[j] * cs[j] + a0 * sn[j];
                     }
                 }
             }
-            if (!U8 || at.kind == 0) {
-                if (live && at.dst != nullptr) {
-                    E* dst = static_cast<E*>(at.dst);
-                    *reinterpret_cast<uint2*>(dst + o0) = pack4<E>(a);
-                    *reinterpret_cast<uint2*>(dst + o1) = pack4<E>(c);
+            uint8_t* dst = live ? pick(rows.dst, kind) : nullptr;
+            if (dst != nullptr) dst += index_of(h, kind) * pick(rows.dst_step, kind);
+            if (!U8 || kind == 0) {
+                if (dst != nullptr) {
+                    r0[i].pack(a);
+                    r1[i].pack(c);
+                    r0[i].store(reinterpret_cast<E*>(dst) + o0);
+                    r1[i].store(reinterpret_cast<E*>(dst) + o1);
                 }
             }
             if (U8) {
@@ -189,7 +216,7 @@ __global__ void __launch_bounds__(kRopeThreads) head_rope_kernel(const __grid_co
                 float mn = INFINITY, mx = -INFINITY;
                 if (own) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
+                    for (int j = 0; j < CH; ++j) {
                         mn = fminf(mn, fminf(a[j], c[j]));
                         mx = fmaxf(mx, fmaxf(a[j], c[j]));
                     }
@@ -199,20 +226,23 @@ __global__ void __launch_bounds__(kRopeThreads) head_rope_kernel(const __grid_co
                     mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
                 }
-                if (live && at.kind != 0 && at.dst != nullptr) {
+                if (dst != nullptr && kind != 0) {
                     float scale = __half2float(__float2half_rn((mx - mn) * (1.0f / 255.0f)));
                     if (!(scale > 0.f)) scale = 1.0f;
                     const float zp = __half2float(__float2half_rn(-mn / scale));
-                    uint32_t w0 = 0, w1 = 0;
+                    uint32_t w0[CH / 4], w1[CH / 4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        w0 |= (uint32_t)fminf(fmaxf(rintf(a[j] / scale + zp), 0.f), 255.f) << (8 * j);
-                        w1 |= (uint32_t)fminf(fmaxf(rintf(c[j] / scale + zp), 0.f), 255.f) << (8 * j);
+                    for (int j = 0; j < CH; ++j) {
+                        const uint32_t b0 = (uint32_t)fminf(fmaxf(rintf(a[j] / scale + zp), 0.f), 255.f), b1 = (uint32_t)fminf(fmaxf(rintf(c[j] / scale + zp), 0.f), 255.f);
+                        w0[j / 4] = j % 4 == 0 ? b0 : w0[j / 4] | b0 << (8 * (j % 4));
+                        w1[j / 4] = j % 4 == 0 ? b1 : w1[j / 4] | b1 << (8 * (j % 4));
                     }
-                    uint8_t* dst = static_cast<uint8_t*>(at.dst);
-                    *reinterpret_cast<uint32_t*>(dst + o0) = w0;
-                    *reinterpret_cast<uint32_t*>(dst + o1) = w1;
-                    if (l == 0) *at.meta = __floats2half2_rn(scale, zp);
+#pragma unroll
+                    for (int j = 0; j < CH / 4; ++j) {
+                        reinterpret_cast<uint32_t*>(dst + o0)[j] = w0[j];
+                        reinterpret_cast<uint32_t*>(dst + o1)[j] = w1[j];
+                    }
+                    if (l == 0) static_cast<__half2*>(kind == 2 ? p.v_meta : p.k_meta)[rows.row + (int64_t)index_of(h, kind) * p.block_size] = __floats2half2_rn(scale, zp);
                 }
             }
         }
@@ -228,16 +258,17 @@ __global__ void __launch_bounds__(kRopeThreads) head_rope_any_kernel(const __gri
     const int h_begin = blockIdx.y * p.per_block, h_end = min(p.heads, h_begin + p.per_block);
     const int half = p.rot >> 1;
     pdl_enter();
-    const int64_t slot = slot_of(p, t);
+    const TokenRows<E> rows = token_rows<E, false>(p, t);
+    if (rows.outside && threadIdx.x == 0) report_status(p.status, STATUS_BAD_INDEX);
     const int position = p.positions[b * p.pos_batch + s];
     for (int i = threadIdx.x; i < half; i += kRopeThreads) turn_any[i] = turn_of(position, p.inv_freq[i], p.mult);
     __syncthreads();
     for (int h = h_begin + warp; h < h_end; h += kRopeThreads / 32) {
-        const HeadAt at = head_at<E, false>(p, b, s, h, slot);
-        if (at.dst == nullptr) continue;
-        const E* src = static_cast<const E*>(at.src);
-        E* dst = static_cast<E*>(at.dst);
-        const E* w = static_cast<const E*>(at.kind == 0 ? p.q_norm : at.kind == 1 ? p.k_norm : nullptr);
+        const int kind = h < p.Hq ? 0 : h < p.Hq + p.Hkv ? 1 : 2, g = kind == 0 ? h : kind == 1 ? h - p.Hq : h - p.Hq - p.Hkv;
+        if (rows.dst[kind] == nullptr) continue;
+        const E* src = rows.src[kind] + g * rows.src_step[kind];
+        E* dst = reinterpret_cast<E*>(rows.dst[kind] + g * rows.dst_step[kind]);
+        const E* w = static_cast<const E*>(kind == 0 ? p.q_norm : kind == 1 ? p.k_norm : nullptr);
         float inv = 1.f;
         if (w != nullptr) {
             float ss = 0.f;
@@ -247,7 +278,7 @@ __global__ void __launch_bounds__(kRopeThreads) head_rope_any_kernel(const __gri
             inv = rsqrtf(ss / (float)p.D + p.eps);
         }
         auto value = [&](int d) { return w != nullptr ? to_float(src[d]) * inv * to_float(w[d]) : to_float(src[d]); };
-        const int turned = at.kind == 2 ? 0 : half;
+        const int turned = kind == 2 ? 0 : half;
         for (int i = lane; i < turned; i += 32) {
             const int d0 = p.interleaved ? 2 * i : i, d1 = p.interleaved ? 2 * i + 1 : half + i;
             const float a = value(d0), c = value(d1);
@@ -259,16 +290,20 @@ __global__ void __launch_bounds__(kRopeThreads) head_rope_any_kernel(const __gri
     }
 }
 
-template <class E, bool INTER, bool U8>
-static cudaError_t run_head_rope(const HeadRopeParams& p, dim3 grid, cudaStream_t stream) {
-    if (p.D <= 64) return launch_pdl(head_rope_kernel<E, INTER, 8, U8>, grid, dim3(kRopeThreads), 0, stream, p);
-    if (p.D <= 128) return launch_pdl(head_rope_kernel<E, INTER, 16, U8>, grid, dim3(kRopeThreads), 0, stream, p);
-    return launch_pdl(head_rope_kernel<E, INTER, 32, U8>, grid, dim3(kRopeThreads), 0, stream, p);
+template <class E, bool INTER, int CH, bool U8>
+static cudaError_t run_head_rope(const HeadRopeParams& p, dim3 grid, int lanes, cudaStream_t stream) {
+    constexpr int FEW = 32 / CH;
+    auto kern = lanes == FEW ? head_rope_kernel<E, INTER, CH, FEW, U8> : lanes == 2 * FEW ? head_rope_kernel<E, INTER, CH, 2 * FEW, U8> : head_rope_kernel<E, INTER, CH, 4 * FEW, U8>;
+    return launch_pdl(kern, grid, dim3(kRopeThreads), 0, stream, p);
+}
+template <class E, bool INTER>
+static cudaError_t run_head_rope(const HeadRopeParams& p, dim3 grid, int ch, int lanes, cudaStream_t stream) {
+    if (ch == 8) return p.kv_u8 ? run_head_rope<E, INTER, 8, true>(p, grid, lanes, stream) : run_head_rope<E, INTER, 8, false>(p, grid, lanes, stream);
+    return p.kv_u8 ? run_head_rope<E, INTER, 4, true>(p, grid, lanes, stream) : run_head_rope<E, INTER, 4, false>(p, grid, lanes, stream);
 }
 template <class E>
-static cudaError_t run_head_rope(const HeadRopeParams& p, dim3 grid, cudaStream_t stream) {
-    if (p.kv_u8) return p.interleaved ? run_head_rope<E, true, true>(p, grid, stream) : run_head_rope<E, false, true>(p, grid, stream);
-    return p.interleaved ? run_head_rope<E, true, false>(p, grid, stream) : run_head_rope<E, false, false>(p, grid, stream);
+static cudaError_t run_head_rope(const HeadRopeParams& p, dim3 grid, int ch, int lanes, cudaStream_t stream) {
+    return p.interleaved ? run_head_rope<E, true>(p, grid, ch, lanes, stream) : run_head_rope<E, false>(p, grid, ch, lanes, stream);
 }
 
 }  // namespace ovb
@@ -289,9 +324,11 @@ extern "C" int ovb_qk_norm_rope(const ovb_qk_rope_args* a, ovb_stream_t stream_)
     p.heads = a->Hq + a->Hkv * (cache ? 2 : 1);
     const int tokens = a->B * a->S;
     const auto bits = [](const void* x) { return reinterpret_cast<uintptr_t>(x); };
-    uintptr_t at = bits(a->q) | bits(a->q_out) | bits(a->k) | bits(a->k_out) | bits(a->v) | (a->kv_u8 ? 0 : bits(a->k_cache) | bits(a->v_cache));
+    uintptr_t at = bits(a->q_norm) | bits(a->k_norm) | bits(a->q) | bits(a->q_out) | bits(a->k) | bits(a->k_out) | bits(a->v) | (a->kv_u8 ? 0 : bits(a->k_cache) | bits(a->v_cache));
     int64_t pitch = a->q_batch | a->q_token | a->q_head | a->k_batch | a->k_token | a->k_head | a->qo_batch | a->qo_token | a->qo_head;
     pitch |= cache ? a->v_batch | a->v_token | a->v_head : a->ko_batch | a->ko_token | a->ko_head;
+    // elements of a lane's two pieces: eight where heads, rotation and alignment allow it, else four
+    const int ch = a->D % 16 == 0 && a->rot % 16 == 0 && (at & 15) == 0 && (pitch & 7) == 0 ? 8 : 4;
     const bool pieces = a->D % 8 == 0 && a->D <= 256 && a->rot % 8 == 0 && (at & 7) == 0 && (pitch & 3) == 0;
     if (a->kv_u8) {
         OVB_REQUIRE(a->k_meta && a->v_meta, "ovb_qk_norm_rope: a u8 cache needs its (scale, zero point) tables");
@@ -299,11 +336,11 @@ extern "C" int ovb_qk_norm_rope(const ovb_qk_rope_args* a, ovb_stream_t stream_)
                     "ovb_qk_norm_rope: the u8 cache is served for head sizes and rotations that are multiples of 8 up to 256, in heads that are 8-byte aligned");
     }
     // heads of a block: all from 512 tokens on (a block per token then fills every SM three times); with fewer, as many as its lanes take at a time
-    const int lanes = a->D <= 64 ? 8 : a->D <= 128 ? 16 : 32, at_a_time = pieces ? kRopeThreads / lanes : kRopeThreads / 32;
+    const int lanes = (a->D <= 64 ? 32 : a->D <= 128 ? 64 : 128) / ch, at_a_time = pieces ? kRopeThreads / lanes : kRopeThreads / 32;
     p.per_block = tokens >= 512 ? p.heads : at_a_time;
     const dim3 grid(tokens, ceil_div(p.heads, p.per_block));
     OVB_REQUIRE(grid.y <= 65535, "ovb_qk_norm_rope: %d heads", p.heads);
-    if (pieces) OVB_CHECK_CUDA(a->f16 ? run_head_rope<__half>(p, grid, stream) : run_head_rope<__nv_bfloat16>(p, grid, stream));
+    if (pieces) OVB_CHECK_CUDA(a->f16 ? run_head_rope<__half>(p, grid, ch, lanes, stream) : run_head_rope<__nv_bfloat16>(p, grid, ch, lanes, stream));
     else OVB_CHECK_CUDA(launch_pdl(a->f16 ? head_rope_any_kernel<__half> : head_rope_any_kernel<__nv_bfloat16>, grid, dim3(kRopeThreads), (size_t)(a->rot >> 1) * sizeof(float2), stream, p));
     return 0;
 }

@@ -1,15 +1,10 @@
 // Rows of 16-bit values -> signed bytes with one scale per row, the RMS norm of the row on the way where there is one.
 //
-//   y = x, or x * rsqrt(mean(x^2) + eps) * gamma;  a = max |y|;  q = round_half_even(y * (127 / a));  scale = a / 127;  sum = sum q
-//
-// Quotients and products are rounded to 32 bits once each, the norm's sums are held in 32 bits. |y| * (127 / a) is at most 127 (1 + 2^-23), so no value
-// has to be clamped. A row whose largest magnitude is below 2^-119, where 127 / a would not be finite, counts as zero (scale 0); one with a value that
-// is not finite gets the scale NaN and codes of zero, so that every result of the row is NaN. The magnitudes are compared as integers, where NaN is the
-// largest.
+// The arithmetic is in gemm_i8.cuh; the norm's sums are held in 32 bits.
 //
 // What bounds it: memory, three bytes per value (two of them usually from L2). A row stays in registers between the passes: every thread holds HOLD
 // pieces of eight columns.
-#include "gemm_common.cuh"
+#include "gemm_i8.cuh"
 
 namespace ovb {
 
@@ -25,11 +20,6 @@ struct QuantParams {
     int ldq;
     float eps;
 };
-
-constexpr uint32_t kNotFinite = 0x7F800000u;
-constexpr float kQuantFloor = 1.5046327690525280e-36f;      // 2^-119
-
-__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
 // The sum (largest) over the warps that share a row; every thread gets it.
 template <int WPR, class T, class F>
@@ -47,14 +37,8 @@ __device__ __forceinline__ T over_row(T v, T* box, F&& f) {
 }
 
 __device__ __forceinline__ void row_result(const QuantParams& p, int row, uint32_t top, int sum) {
-    const float a = __uint_as_float(top);
-    p.scale[row] = top >= kNotFinite ? __int_as_float(0x7FFFFFFF) : a < kQuantFloor ? 0.f : __fdiv_rn(a, 127.f);
+    p.scale[row] = row_scale_of(top);
     p.sum[row] = sum;
-}
-// 127 / a, or 0 where the row has no codes
-__device__ __forceinline__ float row_factor(uint32_t top) {
-    const float a = __uint_as_float(top);
-    return top >= kNotFinite || a < kQuantFloor ? 0.f : __fdiv_rn(127.f, a);
 }
 
 __device__ __forceinline__ int source_row(const QuantParams& p, int row) {

@@ -233,6 +233,11 @@ __device__ __forceinline__ void bulk_load_1d(void* dst, const void* src, uint32_
                  : "memory");
 }
 
+// Ask for global memory to be brought into L2 (16-byte aligned, a multiple of 16 bytes).
+__device__ __forceinline__ void bulk_prefetch_l2(const void* src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
+}
+
 // ---------------------------------------------------------------- tcgen05 / TMEM
 // Allocation and release are warp-collective (.sync.aligned): call with a full, converged warp.
 __device__ __forceinline__ void tmem_alloc(uint32_t* smem_result, uint32_t ncols) {
@@ -324,13 +329,23 @@ __device__ __forceinline__ void umma_f16_ts_elect(uint32_t tmem_d, uint32_t tmem
         ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-__device__ __forceinline__ void umma_i8_ss_elect(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+// The four products of a 128-byte k-block of signed bytes and the commit of its stage, one elect.sync for all of them: with few tokens the issue of these
+// instructions is what a k-block costs (cycles per k-block, 16 tokens: 377 with an elect each and a loop whose counters are not uniform, 320 with uniform
+// counters, 262 like this).
+__device__ __forceinline__ void umma_i8_block_elect(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate, uint64_t* bar) {
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
+        "{\n\t.reg .pred p, q, t;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.eq.b32 t, 0, 0;\n\t"
+        "add.s64 a1, %1, 2;\n\tadd.s64 a2, %1, 4;\n\tadd.s64 a3, %1, 6;\n\t"
+        "add.s64 b1, %2, 2;\n\tadd.s64 b2, %2, 4;\n\tadd.s64 b3, %2, 6;\n\t"
         "elect.sync _|q, 0xffffffff;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        "@q tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::i8 [%0], a1, b1, %3, t;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::i8 [%0], a2, b2, %3, t;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::i8 [%0], a3, b3, %3, t;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%5];\n\t}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(smem_u32(bar))
         : "memory");
 }
 __device__ __forceinline__ void umma_commit_elect(uint64_t* bar) {
