@@ -30,6 +30,17 @@ __device__ __forceinline__ __half from_float<__half>(float v) {
     return __float2half_rn(v);
 }
 
+// Two values rounded to a 16-bit pair, one instruction.
+template <class E>
+__device__ __forceinline__ uint32_t pack_pair(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float a, float b) { return pack_bf16x2(a, b); }
+template <>
+__device__ __forceinline__ uint32_t pack_pair<__half>(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
 // cap * tanh(v / cap); the error is of the order of an ulp of cap.
 __device__ __forceinline__ float soft_cap(float v, float cap) { return cap - __fdividef(2.0f * cap, 1.0f + __expf(__fdividef(2.0f * v, cap))); }
 

@@ -22,7 +22,7 @@ constexpr int i8_threads(bool fused) { return fused ? 64 + kI8QuantWarps * 32 : 
 constexpr int kI8FusedBlock = 16 * kI8BlockK;       // a k-block of the codes
 
 struct I8TileParams : I8Params {
-    int bt, stages, splits, early, prefetch;
+    int bt, stages, splits;
     int whole;                    // 16-bit results and residuals in groups of four aligned columns
     // quantisation in the kernel
     const void* raw;
@@ -162,7 +162,6 @@ __global__ void __launch_bounds__(i8_threads(FUSED)) gemm_i8_tile_kernel(const _
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = tmem_slot;
-    if (p.early) pdl_trigger();
 
     if (warp == 0) {
         if (lane == 0) {
@@ -172,8 +171,6 @@ __global__ void __launch_bounds__(i8_threads(FUSED)) gemm_i8_tile_kernel(const _
                 mbar_arrive_expect_tx(&full[i], (uint32_t)stage_bytes);
                 bulk_load_1d(stages + i * stage_bytes, w + (size_t)i * kI8TileBytes, kI8TileBytes, &full[i]);
             }
-            int fetched = min(n, ahead + p.prefetch);   // chunks that have been asked for, into shared memory or L2
-            for (int i = ahead; i < fetched; ++i) bulk_prefetch_l2(w + (size_t)i * kI8TileBytes, kI8TileBytes);
             if (!FUSED) {
                 pdl_wait();
                 for (int i = 0; i < ahead; ++i) tma_load_2d(stages + i * stage_bytes + kI8TileBytes, &tmX, &full[i], (kb0 + i) * kI8BlockK, t0);
@@ -182,14 +179,13 @@ __global__ void __launch_bounds__(i8_threads(FUSED)) gemm_i8_tile_kernel(const _
             uint32_t phase = 0;
             for (int i = ahead; i < n; ++i) {
                 if (!mbar_wait(&empty[s], phase, abort_flag, p.status)) break;
-                if (fetched < n) bulk_prefetch_l2(w + (size_t)fetched++ * kI8TileBytes, kI8TileBytes);
                 mbar_arrive_expect_tx(&full[s], (uint32_t)stage_bytes);
                 bulk_load_1d(stages + s * stage_bytes, w + (size_t)i * kI8TileBytes, kI8TileBytes, &full[s]);
                 if (!FUSED) tma_load_2d(stages + s * stage_bytes + kI8TileBytes, &tmX, &full[s], (kb0 + i) * kI8BlockK, t0);
                 if (++s == p.stages) { s = 0; phase ^= 1; }
             }
             if (FUSED) pdl_wait();
-            if (OVB_PDL_GEMM && !p.early) pdl_trigger();
+            if (OVB_PDL_GEMM) pdl_trigger();
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -264,7 +260,7 @@ __global__ void __launch_bounds__(i8_threads(FUSED)) gemm_i8_tile_kernel(const _
         const int cols = GATED ? p.N >> 1 : p.N, col = GATED ? (n0 >> 1) + lane * 4 : n, left = GATED && lane >= 16 ? 0 : cols - col;
         // S partials of as many tokens as give sixteen loads in flight. WHOLE: 16-bit results, four columns of a row in one aligned access.
         auto finish = [&](auto count, auto kind) {
-            constexpr int S = decltype(count)::value, AT_ONCE = S == 1 ? 4 : 16 / S;
+            constexpr int S = decltype(count)::value, AT_ONCE = FUSED ? 1 : S == 1 ? 4 : 16 / S;      // (eight rows at most go to ten warps)
             constexpr bool WHOLE = decltype(kind)::value;
             uint32_t from[S];
 #pragma unroll
@@ -437,8 +433,6 @@ static int run_i8_tile(const ovb_gemm_i8_args* a, const I8Params& base, bool fus
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3(tiles * p.splits, rows);
     cfg.blockDim = dim3(i8_threads(fused));
-    p.early = env_int("OVB_I8_EARLY", 0);
-    p.prefetch = env_int("OVB_I8_PF", 16);
     cfg.dynamicSmemBytes = head + bytes + 1024;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -519,7 +513,7 @@ int ovb_gemm_i8(const ovb_gemm_i8_args* a, ovb_stream_t stream_) {
     p.ldo = a->ldo; p.ldr = a->ldr;
     p.act = a->act; p.out_f32 = a->out_f32;
     p.act_limit = a->act_limit; p.act_slope = a->act_slope; p.act_shift = a->act_shift;
-    return a->T > env_int("OVB_I8_PAIR", 256) ? gemm_i8_pair(a, p, stream) : run_i8_tile(a, p, fused, stream);
+    return a->T > env_int("OVB_I8_PAIR", 256) ? gemm_i8_pair(a, p, env_int("OVB_I8_BN", 256), stream) : run_i8_tile(a, p, fused, stream);
 }
 
 }  // extern "C"

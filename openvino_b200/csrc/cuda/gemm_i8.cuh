@@ -66,21 +66,12 @@ __device__ __forceinline__ float i8_value(int acc, int zp, int sum, float scale,
     const float v = float(i8_zp_form(FORM) ? acc - zp * sum : acc);
     return FORM == kI8Any ? fmaf(v, scale, bias) : v * scale;
 }
-template <class E>
-__device__ __forceinline__ uint32_t pack_pair(float a, float b);
-template <>
-__device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float a, float b) { return pack_bf16x2(a, b); }
-template <>
-__device__ __forceinline__ uint32_t pack_pair<__half>(float a, float b) {
-    const __half2 v = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
 template <class P>
 __device__ __forceinline__ float i8_gate(const P& p, float g, float u) {
     return p.act == OVB_ACT_SWIGLU ? __fdividef(g, 1.0f + __expf(-g)) * u : glu_limited(p, g, u);
 }
 
 // gemm_i8_pair.cu: many tokens, pairs of CTAs.
-int gemm_i8_pair(const ovb_gemm_i8_args* a, const I8Params& p, cudaStream_t stream);
+int gemm_i8_pair(const ovb_gemm_i8_args* a, const I8Params& p, int bn, cudaStream_t stream);
 
 }  // namespace ovb

@@ -7,29 +7,24 @@
 //  * warps 4 .. 11: epilogue. Tokens are the lanes, so a thread holds one row: adjacent channels lie in its registers, a gate and its up value too, and
 //    results leave in whole 32-byte sectors. Scales, zero points and biases of the channels come from shared memory, the same for all lanes.
 #include <mutex>
-#include <stdlib.h>
 #include <type_traits>
 
 #include "gemm_i8.cuh"
 
 namespace ovb {
 
-constexpr int kI8PairMaxStages = 6;
+constexpr int kI8PairStages = 6;
 constexpr int kI8PairThreads = 384;
 constexpr int kI8PairStageBytes = 2 * kI8TileBytes;                      // 128 tokens and up to 128 weight rows
 constexpr int kI8PairChannels = 256;                                     // channels of a tile at most
-constexpr int kI8PairUnit = 64;                                          // channels that the epilogue takes at a time
+constexpr int kI8PairBox = 2048;                                         // 32 rows x 64 bytes of an epilogue warp, on their way from rows to lines
 constexpr int kI8PairBand = 8;                                           // token tiles per rasterisation band
-constexpr int i8_pair_smem(int stages, int recv_bytes) { return stages * kI8PairStageBytes + recv_bytes + 2 * kI8PairChannels * 12 + 1024 + 1024; }
+constexpr int kI8PairSmem = kI8PairStages * kI8PairStageBytes + 8 * kI8PairBox + 2 * kI8PairChannels * 12 + 1024 + 1024;
 
 struct I8PairParams : I8Params {
     int bn;                       // channels of a tile: 256 or 128
     int tiles_n, tiles_t;
-    int stages;
-    int splits;                   // pairs that share the k-blocks of a tile (SPLIT)
-    int recv_bytes;
-    int whole;                    // 16-bit results and residuals in whole aligned sectors
-    int prefetch;                 // k-blocks that weights are asked into L2 ahead
+    int whole;                    // 16-bit results and residuals in aligned pieces of eight columns
 };
 
 // Tiles in bands of eight token tiles: a band's tokens stay in L2 while its weights pass once.
@@ -43,7 +38,7 @@ __device__ __forceinline__ bool i8_pair_tile(const I8PairParams& p, int idx, int
 }
 
 // The four products of a k-block and the commit of its stage in both CTAs (see umma_i8_block_elect).
-__device__ __forceinline__ void pair_i8_block_elect(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate, uint64_t* bar, uint16_t ctas) {
+__device__ __forceinline__ void pair_i8_block_elect(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate, uint64_t* bar) {
     asm volatile(
         "{\n\t.reg .pred p, q, t;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
@@ -56,54 +51,32 @@ __device__ __forceinline__ void pair_i8_block_elect(uint32_t tmem_d, uint64_t de
         "@q tcgen05.mma.cta_group::2.kind::i8 [%0], a2, b2, %3, t;\n\t"
         "@q tcgen05.mma.cta_group::2.kind::i8 [%0], a3, b3, %3, t;\n\t"
         "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%5], %6;\n\t}"
-        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(smem_u32(bar)), "h"(ctas)
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(smem_u32(bar)), "h"((uint16_t)3)
         : "memory");
 }
-__device__ __forceinline__ void pair_commit_to_elect(uint64_t* bar, uint16_t ctas) {
-    asm volatile(
-        "{\n\t.reg .pred q;\n\t"
-        "elect.sync _|q, 0xffffffff;\n\t"
-        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}"
-        ::"r"(smem_u32(bar)), "h"(ctas)
-        : "memory");
-}
-
-// 32 bytes at a time: one whole sector of the row that a lane owns
-__device__ __forceinline__ void st_global_32(void* p, const uint32_t* v) {
-    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
-}
-__device__ __forceinline__ void ld_global_32(const void* p, uint32_t* v) {
-    asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "l"(p) : "memory");
-}
-// SPLIT: a cluster of `splits` pairs shares the k-blocks of one tile. The columns of the tile are shared out among the pairs: every CTA sends the partial
-// sums of the others' columns from its registers into the shared memory of the CTA that finishes them for the same tokens.
-template <bool F16, bool SPLIT, int FORM>
-__global__ void __launch_bounds__(kI8PairThreads, 1)
+template <bool F16, int FORM>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8PairThreads, 1)
 gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const __grid_constant__ I8PairParams p) {
     using E = typename Elem<F16>::type;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* recv = smem + p.stages * kI8PairStageBytes;
-    float* chan_scale = reinterpret_cast<float*>(recv + p.recv_bytes);                          // [2][256] each
+    uint8_t* boxes = smem + kI8PairStages * kI8PairStageBytes;
+    float* chan_scale = reinterpret_cast<float*>(boxes + 8 * kI8PairBox);                          // [2][256] each
     float* chan_bias = chan_scale + 2 * kI8PairChannels;
     int* chan_zp = reinterpret_cast<int*>(chan_bias + 2 * kI8PairChannels);
     uint64_t* bars = reinterpret_cast<uint64_t*>(chan_zp + 2 * kI8PairChannels);
     uint64_t* full = bars;                              // [stages] even CTA: both CTAs' tiles have landed
-    uint64_t* empty = bars + kI8PairMaxStages;          // [stages] both CTAs: the stage has been read
-    uint64_t* acc_full = bars + 2 * kI8PairMaxStages;   // [2] both CTAs: accumulator complete
+    uint64_t* empty = bars + kI8PairStages;          // [stages] both CTAs: the stage has been read
+    uint64_t* acc_full = bars + 2 * kI8PairStages;   // [2] both CTAs: accumulator complete
     uint64_t* acc_empty = acc_full + 2;                 // [2] even CTA: accumulator drained by the 16 epilogue warps of the pair
-    uint64_t* received = acc_empty + 2;                 // the other pairs' sums of this CTA's columns have arrived
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(received + 1);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* went_well = abort_flag + 1;           // [2]
 
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
-    const uint32_t cluster_rank = cluster_ctarank(), rank = cluster_rank & 1u, even = cluster_rank & ~1u;
-    const int part = SPLIT ? (int)(cluster_rank >> 1) : 0;
-    const uint16_t both = (uint16_t)(3u << even);
+    const uint32_t rank = cluster_ctarank();
     if (threadIdx.x == 0) {
-        for (int s = 0; s < p.stages; ++s) {
+        for (int s = 0; s < kI8PairStages; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
@@ -111,10 +84,8 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
             mbar_init(&acc_full[b], 1);
             mbar_init(&acc_empty[b], 16);
         }
-        mbar_init(received, 1);
         *abort_flag = 0;
         mbar_fence_init();
-        if (SPLIT) mbar_arrive_expect_tx(received, (uint32_t)p.recv_bytes);
         tma_prefetch_desc(&tmW);
         tma_prefetch_desc(&tmX);
     }
@@ -128,23 +99,8 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
     cluster_wait();
     tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot;
-    const int ctas = SPLIT ? 2 * p.splits : 2;
-    const int step = (int)gridDim.x / ctas, first = (int)blockIdx.x / ctas;
-    const int kb0 = SPLIT ? (int)((int64_t)p.KB * part / p.splits) : 0, kb1 = SPLIT ? (int)((int64_t)p.KB * (part + 1) / p.splits) : p.KB;
+    const int pairs = (int)gridDim.x >> 1, first = (int)blockIdx.x >> 1;
     const int half_n = p.bn >> 1;                       // weight rows that a CTA loads
-    // the rows of k-block kb of a tile's weights that this CTA loads, as they are packed: 128 of a chunk, chunk after chunk along K. Channels behind the last
-    // chunk are not there: the box then reads the last chunk's again, and nothing of them is stored
-    const int last_chunk = (p.N - 1) / TILE_N;
-    auto weight_row = [&](int n0, int kb) {
-        const int row = n0 + (int)rank * half_n;
-        return (min(row / TILE_N, last_chunk) * p.KB + kb) * TILE_N + row % TILE_N;
-    };
-    auto prefetch = [&](int row) { bulk_prefetch_l2(p.w + (size_t)row * kI8BlockK, (uint32_t)(half_n * kI8BlockK)); };
-    if (warp == 0 && lane == 0) {                       // weights are constants: they start for L2 before the tokens are there
-        int t0, n0;
-        if (i8_pair_tile(p, first, t0, n0))
-            for (int kb = kb0; kb < min(kb1, kb0 + p.prefetch); ++kb) prefetch(weight_row(n0, kb));
-    }
     pdl_wait();
 
     if (warp == 0) {
@@ -153,19 +109,21 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
             uint32_t phase = 1;
             bool ok = true;
             const uint32_t tx = 2u * (kI8TileBytes + half_n * kI8BlockK);
-            for (int idx = first; ok && i8_pair_tile(p, idx, t0, n0); idx += step) {
-                int w_row = weight_row(n0, kb0);
+            for (int idx = first; ok && i8_pair_tile(p, idx, t0, n0); idx += pairs) {
+                // the weight's rows as they are packed: 128 of a chunk, chunk after chunk along K. Channels behind the last chunk are not there: the
+                // box then reads the last chunk's again, and nothing of them is stored
+                const int row = n0 + (int)rank * half_n;
+                int w_row = min(row / TILE_N, (p.N - 1) / TILE_N) * p.KB * TILE_N + row % TILE_N;
                 const int x_row = t0 + (int)rank * 128;
-                for (int kb = kb0; kb < kb1; ++kb) {
+                for (int kb = 0; kb < p.KB; ++kb) {
                     ok = mbar_wait(&empty[s], phase, abort_flag, p.status);
                     if (!ok) break;
                     const uint32_t st = smem_u32(smem) + s * kI8PairStageBytes, bar = smem_u32(&full[s]);
                     if (rank == 0) mbar_arrive_expect_tx(&full[s], tx);
-                    if (kb + p.prefetch < kb1) prefetch(w_row + p.prefetch * TILE_N);
                     pair_load_2d(st, &tmX, bar, kb * kI8BlockK, x_row);
                     pair_load_2d(st + kI8TileBytes, &tmW, bar, 0, w_row);
                     w_row += TILE_N;
-                    if (++s == p.stages) { s = 0; phase ^= 1; }
+                    if (++s == kI8PairStages) { s = 0; phase ^= 1; }
                 }
             }
             if (OVB_PDL_GEMM) pdl_trigger();
@@ -178,18 +136,18 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
             int s = 0, buf = 0, t0, n0;
             uint32_t phase = 0, acc_phase = 1;
             // no way out of the loops: once a wait has run out all later ones return at once, and what is computed then is not stored
-            for (int idx = first; i8_pair_tile(p, idx, t0, n0); idx += step) {
+            for (int idx = first; i8_pair_tile(p, idx, t0, n0); idx += pairs) {
                 mbar_wait(&acc_empty[buf], acc_phase, abort_flag, p.status);
                 tc_fence_after_sync();
                 const uint32_t d = tmem_base + uint32_t(buf * 256);
-                for (int kb = kb0; kb < kb1; ++kb) {
+                for (int kb = 0; kb < p.KB; ++kb) {
                     mbar_wait(&full[s], phase, abort_flag, p.status);
                     tc_fence_after_sync();
                     const uint64_t da = desc0 + (uint64_t)((s * kI8PairStageBytes) >> 4), db = da + (uint64_t)(kI8TileBytes >> 4);
-                    pair_i8_block_elect(d, da, db, idesc, kb > kb0 ? 1u : 0u, &empty[s], both);
-                    if (++s == p.stages) { s = 0; phase ^= 1; }
+                    pair_i8_block_elect(d, da, db, idesc, kb > 0 ? 1u : 0u, &empty[s]);
+                    if (++s == kI8PairStages) { s = 0; phase ^= 1; }
                 }
-                pair_commit_to_elect(&acc_full[buf], both);
+                pair_commit_elect(&acc_full[buf]);
                 if (++buf == 2) { buf = 0; acc_phase ^= 1; }
             }
         }
@@ -197,17 +155,19 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
     } else if (warp >= 4) {
         const int q = warp & 3, half = (warp - 4) >> 2, tid = threadIdx.x - 128;
         constexpr bool GATED = i8_gated_form(FORM);
-        const uint32_t drained0 = dsmem_addr(smem_u32(&acc_empty[0]), even);
-        const int units = p.bn / kI8PairUnit, own = SPLIT ? units / p.splits : units, unit0 = part * own;      // this CTA finishes `own` units from unit0 on
+        const uint32_t drained0 = dsmem_addr(smem_u32(&acc_empty[0]), 0);
+        // A job is 32 columns of the result: 32 of the tile's, or the gate and the up values of the same channels (64 rows of a weight tile are the gate, then
+        // 64 the up values), in two steps of 16. The two warps of a token quarter take jobs in turn.
+        constexpr int RUNS = GATED ? 2 : 1;
+        const int jobs = p.bn / (32 * RUNS);
         const int out_cols = GATED ? p.N >> 1 : p.N;
-        // A unit is 64 columns of the tile, two runs of 32: neighbours, or the gate and the up values of the same channels (rows 0 .. 63 of a weight tile are
-        // the gate). A warp takes 16 columns of each run.
-        auto run_at = [&](int u, int run) { return (GATED ? (u >> 1) * 128 + (u & 1) * 32 + run * 64 : u * 64 + run * 32) + half * 16; };
-        // where the 16 bytes of four columns (from column 4 quad of run `run` of a CTA's unit u) of this thread's token arrive
-        auto box = [&](int slot, int u, int run, int quad) { return ((((slot * own + u) * 2 + run) * 2 + half) * 4 + quad) * 2048 + (q * 32 + lane) * 16; };
+        auto column = [&](int job, int run, int step) { return (GATED ? (job >> 1) * 128 + (job & 1) * 32 + run * 64 : job * 32) + step * 16; };
+        // this warp's box: 64 bytes of each of its 32 rows, pieces of 16 bytes placed so that rows and lines are both free of bank conflicts
+        uint8_t* box = boxes + (warp - 4) * kI8PairBox;
+        auto in_box = [&](int r, int piece) { return reinterpret_cast<uint4*>(box + r * 64 + ((piece ^ ((r >> 1) & 3)) << 4)); };
         int buf = 0, t0, n0;
         uint32_t acc_phase = 0;
-        for (int idx = first; i8_pair_tile(p, idx, t0, n0); idx += step) {
+        for (int idx = first; i8_pair_tile(p, idx, t0, n0); idx += pairs) {
             const int t = t0 + (int)rank * 128 + q * 32 + lane;
             const bool row = t < p.T;
             const float xs = row ? __ldcg(p.x_scale + t) : 0.f;
@@ -227,60 +187,7 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
             if (!went_well[buf]) break;
             tc_fence_after_sync();
             const uint32_t src = tmem_base + (uint32_t(q * 32) << 16) + uint32_t(buf * 256);
-            auto drained = [&]() {                      // the accumulator has been read by this warp
-                tc_fence_before_sync();
-                __syncwarp();
-                if (lane == 0) arrive_cluster(drained0 + buf * 8);
-            };
-            if (SPLIT) {
-                for (int o = 1; o < p.splits; ++o) {
-                    const int to = (part + o) % p.splits, slot = part < to ? part : part - 1;      // the receiver's slots leave itself out
-                    const uint32_t there = dsmem_addr(smem_u32(recv), (uint32_t)(2 * to) + rank), bar = dsmem_addr(smem_u32(received), (uint32_t)(2 * to) + rank);
-                    for (int u = 0; u < own; ++u) {
-                        uint32_t r[32];
-                        tmem_ld_x16(src + run_at(to * own + u, 0), r);
-                        tmem_ld_x16(src + run_at(to * own + u, 1), r + 16);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) st_async_v4(there + box(slot, u, i >> 2, i & 3), r + 4 * i, bar);
-                    }
-                }
-                if (tid == 0) went_well[1] = mbar_wait(received, 0, abort_flag, p.status) ? 1 : 0;
-                asm volatile("bar.sync 1, 256;" ::: "memory");
-                if (!went_well[1]) break;
-            }
-            uint8_t* out_row = static_cast<uint8_t*>(p.out) + (size_t)t * p.ldo * (p.out_f32 ? 4 : 2);
-            const E* res_row = static_cast<const E*>(p.residual) + (size_t)t * p.ldr;
-            // 16 finished values of this row from column `col` on; WHOLE: 16-bit results in whole aligned sectors
-            auto put = [&](auto kind, const float* v, int col) {
-                constexpr bool WHOLE = decltype(kind)::value;
-                const bool there = row && col < out_cols;
-                const E* r = res_row + col;
-                if (WHOLE) {
-                    uint32_t raw[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-                    if (!GATED && p.residual != nullptr) {
-                        if (there) ld_global_32(r, raw);
-                        const E* e = reinterpret_cast<const E*>(raw);
-                        float w[16];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) w[i] = v[i] + to_float(e[i]);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) raw[i] = pack_pair<E>(w[2 * i], w[2 * i + 1]);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) raw[i] = pack_pair<E>(v[2 * i], v[2 * i + 1]);
-                    }
-                    if (there) st_global_32(reinterpret_cast<E*>(out_row) + col, raw);
-                } else if (there) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (col + i < out_cols) {
-                            const float w = p.residual != nullptr ? v[i] + to_float(r[i]) : v[i];
-                            if (p.out_f32) reinterpret_cast<float*>(out_row)[col + i] = w;
-                            else reinterpret_cast<E*>(out_row)[col + i] = from_float<E>(w);
-                        }
-                }
-            };
+            const int first_row = t - lane, rows = min(32, p.T - first_row);           // of this warp; rows may be negative
             auto values = [&](const uint32_t* r, int c, float* v) {
 #pragma unroll
                 for (int i = 0; i < 16; i += 4) {
@@ -295,38 +202,99 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
                     v[i + 3] = i8_value<FORM>((int)r[i + 3], z4.w, sum, xs * s4.w, b4.w);
                 }
             };
-            auto finish = [&](auto kind) {
-#pragma unroll 1
-                for (int u = unit0; u < unit0 + own; ++u) {
-                    uint32_t r[32];
-                    tmem_ld_x16(src + run_at(u, 0), r);
-                    tmem_ld_x16(src + run_at(u, 1), r + 16);
-                    tmem_ld_wait();
-                    if (u + 1 == unit0 + own) drained();
-                    if (SPLIT) {
-                        for (int slot = 0; slot + 1 < p.splits; ++slot)
+            // 16 columns of a job as finished values, the residual not yet added
+            auto compute = [&](int job, int step, float (&v)[16]) {
+                uint32_t r[16 * RUNS];
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                const uint4 w = *reinterpret_cast<const uint4*>(recv + box(slot, u - unit0, i >> 2, i & 3));
-                                r[4 * i] += w.x; r[4 * i + 1] += w.y; r[4 * i + 2] += w.z; r[4 * i + 3] += w.w;
-                            }
-                    }
-                    float v[32];
-                    values(r, run_at(u, 0), v);
-                    values(r + 16, run_at(u, 1), v + 16);
-                    if (GATED) {
+                for (int run = 0; run < RUNS; ++run) tmem_ld_x16(src + column(job, run, step), r + 16 * run);
+                tmem_ld_wait();
+                values(r, column(job, 0, step), v);
+                if (GATED) {
+                    float u[16];
+                    values(r + 16, column(job, RUNS - 1, step), u);
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) v[i] = i8_gate(p, v[i], v[16 + i]);
-                        put(kind, v, (n0 >> 1) + u * 32 + half * 16);
-                    } else {
-                        if (FORM == kI8Any && p.act != OVB_ACT_NONE) apply_act_n(v, p);
-                        put(kind, v, n0 + run_at(u, 0));
-                        put(kind, v + 16, n0 + run_at(u, 1));
-                    }
+                    for (int i = 0; i < 16; ++i) v[i] = i8_gate(p, v[i], u[i]);
+                } else if (FORM == kI8Any && p.act != OVB_ACT_NONE) {
+                    apply_act_n(v, p);
                 }
             };
-            if (p.whole) finish(std::true_type());
-            else finish(std::false_type());
+            // 16-bit results: the box holds the 32 columns of the job, first of the residual, then of the result. WHOLE: aligned pieces of eight columns
+            auto finish16 = [&](auto kind) {
+                constexpr bool WHOLE = decltype(kind)::value;
+#pragma unroll 1
+                for (int job = half; job < jobs; job += 2) {
+                    const int col = (GATED ? n0 >> 1 : n0) + job * 32;
+                    const bool res = !GATED && p.residual != nullptr;
+                    if (res) {
+                        const E* from = static_cast<const E*>(p.residual) + (size_t)first_row * p.ldr + col;
+                        if (WHOLE) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const int r = i * 8 + (lane >> 2), c = (lane & 3) * 8;
+                                if (r < rows && col + c < out_cols) *in_box(r, lane & 3) = __ldcg(reinterpret_cast<const uint4*>(from + (size_t)r * p.ldr + c));
+                            }
+                        } else {
+                            for (int r = 0; r < rows; ++r)
+                                if (col + lane < out_cols) reinterpret_cast<E*>(in_box(r, lane >> 3))[lane & 7] = from[(size_t)r * p.ldr + lane];
+                        }
+                        __syncwarp();
+                    }
+#pragma unroll
+                    for (int step = 0; step < 2; ++step) {
+                        float v[16];
+                        compute(job, step, v);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            uint4* place = in_box(lane, step * 2 + h);
+                            if (res) {
+                                const uint4 raw = *place;
+                                const E* e = reinterpret_cast<const E*>(&raw);
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) v[h * 8 + i] += to_float(e[i]);
+                            }
+                            *place = make_uint4(pack_pair<E>(v[h * 8], v[h * 8 + 1]), pack_pair<E>(v[h * 8 + 2], v[h * 8 + 3]), pack_pair<E>(v[h * 8 + 4], v[h * 8 + 5]),
+                                                pack_pair<E>(v[h * 8 + 6], v[h * 8 + 7]));
+                        }
+                    }
+                    __syncwarp();
+                    E* to = static_cast<E*>(p.out) + (size_t)first_row * p.ldo + col;
+                    if (WHOLE) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int r = i * 8 + (lane >> 2), c = (lane & 3) * 8;
+                            if (r < rows && col + c < out_cols) *reinterpret_cast<uint4*>(to + (size_t)r * p.ldo + c) = *in_box(r, lane & 3);
+                        }
+                    } else {
+                        for (int r = 0; r < rows; ++r)
+                            if (col + lane < out_cols) to[(size_t)r * p.ldo + lane] = reinterpret_cast<const E*>(in_box(r, lane >> 3))[lane & 7];
+                    }
+                    __syncwarp();
+                }
+            };
+            // fp32 results: 16 columns at a time, two rows of them to a store
+            auto finish32 = [&]() {
+                for (int job = half; job < jobs; job += 2)
+                    for (int step = 0; step < 2; ++step) {
+                        float v[16];
+                        compute(job, step, v);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            *in_box(lane, i) = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]));
+                        __syncwarp();
+                        const int c = lane & 15, col = n0 + job * 32 + step * 16 + c;
+                        float* to = static_cast<float*>(p.out) + (size_t)first_row * p.ldo + col;
+                        for (int r = lane >> 4; r < rows; r += 2)
+                            if (col < out_cols) to[(size_t)r * p.ldo] = reinterpret_cast<const float*>(in_box(r, c >> 2))[c & 3];
+                        __syncwarp();
+                    }
+            };
+            if (!GATED && p.out_f32) finish32();
+            else if (p.whole) finish16(std::true_type());
+            else finish16(std::false_type());
+            // the accumulator has been read by this warp
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) arrive_cluster(drained0 + buf * 8);
             if (++buf == 2) { buf = 0; acc_phase ^= 1; }
         }
     }
@@ -346,25 +314,8 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
     }
 }
 
-static cudaLaunchConfig_t i8_pair_config(unsigned grid, int ctas, int smem, cudaStream_t stream, cudaLaunchAttribute (&attr)[2]) {
-    cudaLaunchConfig_t cfg;
-    memset(&cfg, 0, sizeof(cfg));
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(kI8PairThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = ctas;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = pdl_enabled() ? 2 : 1;
-    return cfg;
-}
-
 // Pairs of CTAs that are resident at a time, asked once per device.
-template <bool F16, bool SPLIT, int FORM>
+template <bool F16, int FORM>
 static int resident_i8_pairs(int* pairs) {
     static std::mutex mu;
     static int known[64] = {0};
@@ -372,60 +323,52 @@ static int resident_i8_pairs(int* pairs) {
     OVB_CHECK_CUDA(cudaGetDevice(&dev));
     std::lock_guard<std::mutex> lk(mu);
     if (known[dev & 63] == 0) {
-        const int smem = i8_pair_smem(kI8PairMaxStages, 0);
-        OVB_CHECK_CUDA(cudaFuncSetAttribute(gemm_i8_pair_kernel<F16, SPLIT, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        cudaLaunchAttribute attr[2];
-        cudaLaunchConfig_t cfg = i8_pair_config(148, 2, smem, nullptr, attr);
-        cfg.numAttrs = 1;
+        OVB_CHECK_CUDA(cudaFuncSetAttribute(gemm_i8_pair_kernel<F16, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, kI8PairSmem));
+        cudaLaunchConfig_t cfg;
+        memset(&cfg, 0, sizeof(cfg));
+        cfg.gridDim = dim3(148);
+        cfg.blockDim = dim3(kI8PairThreads);
+        cfg.dynamicSmemBytes = kI8PairSmem;
         int n = 0;
-        OVB_CHECK_CUDA(cudaOccupancyMaxActiveClusters(&n, gemm_i8_pair_kernel<F16, SPLIT, FORM>, &cfg));
+        OVB_CHECK_CUDA(cudaOccupancyMaxActiveClusters(&n, gemm_i8_pair_kernel<F16, FORM>, &cfg));
         known[dev & 63] = n < 1 ? 1 : n;
     }
     *pairs = known[dev & 63];
     return 0;
 }
 
-template <bool F16, bool SPLIT, int FORM>
+template <bool F16, int FORM>
 static int launch_i8_pair(const CUtensorMap& tmW, const CUtensorMap& tmX, const I8PairParams& p, cudaStream_t stream) {
     int pairs = 0;
-    if (int rc = resident_i8_pairs<F16, SPLIT, FORM>(&pairs)) return rc;
+    if (int rc = resident_i8_pairs<F16, FORM>(&pairs)) return rc;
     const int64_t tiles = (int64_t)p.tiles_n * p.tiles_t;
-    const unsigned grid = SPLIT ? 2 * p.splits * (unsigned)tiles : 2 * (unsigned)(tiles < pairs ? tiles : pairs);
-    cudaLaunchAttribute attr[2];
-    const cudaLaunchConfig_t cfg = i8_pair_config(grid, 2 * p.splits, i8_pair_smem(p.stages, p.recv_bytes), stream, attr);
-    OVB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, gemm_i8_pair_kernel<F16, SPLIT, FORM>, tmW, tmX, p));
+    OVB_CHECK_CUDA(launch_pdl(gemm_i8_pair_kernel<F16, FORM>, dim3(2 * (unsigned)(tiles < pairs ? tiles : pairs)), dim3(kI8PairThreads), kI8PairSmem, stream, tmW, tmX, p));
     return 0;
 }
-template <bool F16, bool SPLIT>
+template <bool F16>
 static int launch_i8_pair(int form, const CUtensorMap& tmW, const CUtensorMap& tmX, const I8PairParams& p, cudaStream_t stream) {
     switch (form) {
-        case kI8Plain: return launch_i8_pair<F16, SPLIT, kI8Plain>(tmW, tmX, p, stream);
-        case kI8Gated: return launch_i8_pair<F16, SPLIT, kI8Gated>(tmW, tmX, p, stream);
-        case kI8GatedZp: return launch_i8_pair<F16, SPLIT, kI8GatedZp>(tmW, tmX, p, stream);
-        default: return launch_i8_pair<F16, SPLIT, kI8Any>(tmW, tmX, p, stream);
+        case kI8Plain: return launch_i8_pair<F16, kI8Plain>(tmW, tmX, p, stream);
+        case kI8Gated: return launch_i8_pair<F16, kI8Gated>(tmW, tmX, p, stream);
+        case kI8GatedZp: return launch_i8_pair<F16, kI8GatedZp>(tmW, tmX, p, stream);
+        default: return launch_i8_pair<F16, kI8Any>(tmW, tmX, p, stream);
     }
 }
 
-int gemm_i8_pair(const ovb_gemm_i8_args* a, const I8Params& base, cudaStream_t stream) {
+int gemm_i8_pair(const ovb_gemm_i8_args* a, const I8Params& base, int bn, cudaStream_t stream) {
     I8PairParams p;
     static_cast<I8Params&>(p) = base;
     const auto bits = [](const void* x) { return reinterpret_cast<uintptr_t>(x); };
     const int out_cols = is_gated(a->act) ? a->N / 2 : a->N;
-    p.whole = !a->out_f32 && out_cols % 16 == 0 && a->ldo % 16 == 0 && (bits(a->out) & 31) == 0 && (a->residual == nullptr || (a->ldr % 16 == 0 && (bits(a->residual) & 31) == 0));
+    p.whole = out_cols % 8 == 0 && a->ldo % 8 == 0 && (bits(a->out) & 15) == 0 && (a->residual == nullptr || (a->ldr % 8 == 0 && (bits(a->residual) & 15) == 0));
+    p.bn = bn;
     p.tiles_t = ceil_div(a->T, 256);
-    p.bn = getenv("OVB_I8_BN") ? atoi(getenv("OVB_I8_BN")) : 256;
-    p.splits = getenv("OVB_I8_PS") ? atoi(getenv("OVB_I8_PS")) : 1;
-    p.prefetch = getenv("OVB_I8_PF") ? atoi(getenv("OVB_I8_PF")) : 0;
-    p.tiles_n = ceil_div(a->N, p.bn);
-    p.recv_bytes = (p.splits - 1) * (p.bn / p.splits) * 128 * 4;
-    p.stages = kI8PairMaxStages - (p.recv_bytes + kI8PairStageBytes - 1) / kI8PairStageBytes;
+    p.tiles_n = ceil_div(a->N, bn);
     CUtensorMap tmW, tmX;
     if (int rc = make_tmap_2d(&tmX, a->x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a->T, a->K, a->ldx, 128, kI8BlockK, true)) return rc;
     // the chunks are already in the swizzled order of the MMA: plain boxes of rows of 128 bytes
-    if (int rc = make_tmap_2d(&tmW, a->w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)ceil_div(a->N, TILE_N) * p.KB * TILE_N, kI8BlockK, kI8BlockK, p.bn / 2, kI8BlockK, false)) return rc;
-    const int form = i8_form(a);
-    if (p.splits > 1) return a->f16 ? launch_i8_pair<true, true>(form, tmW, tmX, p, stream) : launch_i8_pair<false, true>(form, tmW, tmX, p, stream);
-    return a->f16 ? launch_i8_pair<true, false>(form, tmW, tmX, p, stream) : launch_i8_pair<false, false>(form, tmW, tmX, p, stream);
+    if (int rc = make_tmap_2d(&tmW, a->w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)ceil_div(a->N, TILE_N) * p.KB * TILE_N, kI8BlockK, kI8BlockK, bn / 2, kI8BlockK, false)) return rc;
+    return a->f16 ? launch_i8_pair<true>(i8_form(a), tmW, tmX, p, stream) : launch_i8_pair<false>(i8_form(a), tmW, tmX, p, stream);
 }
 
 }  // namespace ovb

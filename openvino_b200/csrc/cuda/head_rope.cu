@@ -16,11 +16,15 @@ namespace ovb {
 
 struct HeadRopeParams : ovb_qk_rope_args {
     int* status;
-    int heads, per_block;         // all heads of a token; heads of a block
+    int src_step[3], dst_step[3]; // from head to head, queries, keys, values: elements, bytes
+    int heads;                    // of a token, all kinds
+    int parts, per_warp;          // warps of a token and their heads
+    float inv_d;
 };
 
 constexpr int kRopeThreads = 128;
-constexpr int kRopeBatch = 2;     // heads that a group of lanes has in flight
+constexpr int kRopeBlocks = 5;    // resident on an SM
+constexpr int kRopeAhead = 2;     // rounds of heads that a warp has in flight
 
 __device__ __forceinline__ float2 turn_of(int position, float inv_freq, float mult) {
     const double turns = (double)position * (double)inv_freq * 0.15915494309189533577;
@@ -29,12 +33,11 @@ __device__ __forceinline__ float2 turn_of(int position, float inv_freq, float mu
     return make_float2(c * mult, s * mult);
 }
 
-// Where a token's heads are: a base for each kind, steps between heads.
+// Where a token's heads are: a base for each kind.
 template <class E>
 struct TokenRows {
     const E* src[3];
     uint8_t* dst[3];              // NULL: not kept
-    int64_t src_step[3], dst_step[3];      // elements, bytes
     int64_t row;                  // of the first key (value) head in the cache
     bool outside;                 // the slot is behind the cache
 };
@@ -46,18 +49,12 @@ __device__ __forceinline__ TokenRows<E> token_rows(const HeadRopeParams& p, int 
     r.src[0] = static_cast<const E*>(p.q) + b * p.q_batch + s * p.q_token;
     r.src[1] = static_cast<const E*>(p.k) + b * p.k_batch + s * p.k_token;
     r.src[2] = static_cast<const E*>(p.v) + b * p.v_batch + s * p.v_token;
-    r.src_step[0] = p.q_head;
-    r.src_step[1] = p.k_head;
-    r.src_step[2] = p.v_head;
     r.dst[0] = reinterpret_cast<uint8_t*>(static_cast<E*>(p.q_out) + b * p.qo_batch + s * p.qo_token);
-    r.dst_step[0] = p.qo_head * (int)sizeof(E);
     r.row = 0;
     r.outside = false;
     if (p.k_cache == nullptr) {
         r.dst[1] = reinterpret_cast<uint8_t*>(static_cast<E*>(p.k_out) + b * p.ko_batch + s * p.ko_token);
-        r.dst_step[1] = p.ko_head * (int)sizeof(E);
         r.dst[2] = nullptr;
-        r.dst_step[2] = 0;
         return r;
     }
     const int slot = p.slot_map[t], size = U8 ? 1 : (int)sizeof(E);
@@ -67,7 +64,6 @@ __device__ __forceinline__ TokenRows<E> token_rows(const HeadRopeParams& p, int 
     r.row = (int64_t)blk * p.Hkv * p.block_size + off;
     r.dst[1] = slot >= 0 && inside ? static_cast<uint8_t*>(p.k_cache) + r.row * p.D * size : nullptr;
     r.dst[2] = slot >= 0 && inside ? static_cast<uint8_t*>(p.v_cache) + r.row * p.D * size : nullptr;
-    r.dst_step[1] = r.dst_step[2] = (int64_t)p.block_size * p.D * size;
     return r;
 }
 
@@ -95,90 +91,90 @@ struct Piece {
     }
     __device__ __forceinline__ void pack(const float (&v)[CH]) {
 #pragma unroll
-        for (int i = 0; i < CH; i += 2) {
-            E e[2] = {from_float<E>(v[i]), from_float<E>(v[i + 1])};
-            w[i / 2] = *reinterpret_cast<const uint32_t*>(e);
-        }
+        for (int i = 0; i < CH; i += 2) w[i / 2] = pack_pair<E>(v[i], v[i + 1]);
     }
 };
 
 // Heads and rotations of whole pieces, aligned heads. LANES lanes share a head, each with two pieces of CH elements: the partners of its CH pairs, or 2 CH
-// neighbours.
+// neighbours. A warp works alone, on a token's heads or a part of them, with the heads of kRopeAhead rounds on their way.
 template <class E, bool INTER, int CH, int LANES, bool U8>
-__global__ void __launch_bounds__(kRopeThreads, 8) head_rope_kernel(const __grid_constant__ HeadRopeParams p) {
-    __shared__ float2 turn[128];
-    constexpr int GROUPS = kRopeThreads / LANES;
-    const int t = blockIdx.x;
-    const int group = threadIdx.x / LANES, l = threadIdx.x % LANES;
-    const int h_begin = blockIdx.y * p.per_block, h_end = min(p.heads, h_begin + p.per_block);
+__global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) head_rope_kernel(const __grid_constant__ HeadRopeParams p) {
+    __shared__ float2 turn_of_warp[kRopeThreads / 32][128];
+    constexpr int GROUPS = 32 / LANES;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int id = blockIdx.x * (kRopeThreads / 32) + warp, t = id / p.parts;
+    const int group = lane / LANES, l = lane % LANES;
+    const int h_begin = (id - t * p.parts) * p.per_warp, h_end = min(p.heads, h_begin + p.per_warp);
     const bool own = l * 2 * CH < p.D;                  // this lane has elements
     const int pair0 = l * CH, half = p.rot >> 1;
     const bool turns = own && pair0 < half;
     // behind the rotated dimensions, and in the interleaved form, the two pieces are neighbours
     const int o0 = turns && !INTER ? pair0 : pair0 * 2, o1 = turns && !INTER ? half + pair0 : pair0 * 2 + CH;
     pdl_enter();
+    if (t >= p.B * p.S) return;                         // whole warps, which share nothing
     const TokenRows<E> rows = token_rows<E, U8>(p, t);
     auto kind_of = [&](int h) { return h < p.Hq ? 0 : h < p.Hq + p.Hkv ? 1 : 2; };
     auto index_of = [&](int h, int kind) { return kind == 0 ? h : kind == 1 ? h - p.Hq : h - p.Hq - p.Hkv; };
     auto pick = [&](const auto& of, int kind) { return kind == 0 ? of[0] : kind == 1 ? of[1] : of[2]; };
+    Piece<E, CH> r0[kRopeAhead], r1[kRopeAhead];
+    auto fetch = [&](int h, Piece<E, CH>& a, Piece<E, CH>& c) {
+        if (h < h_end && own) {
+            const int kind = kind_of(h);
+            const E* src = pick(rows.src, kind) + (int64_t)index_of(h, kind) * pick(p.src_step, kind);
+            a.load(src + o0);
+            c.load(src + o1);
+        } else {
+#pragma unroll
+            for (int j = 0; j < CH / 2; ++j) a.w[j] = c.w[j] = 0;
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < kRopeAhead; ++i) fetch(h_begin + i * GROUPS + group, r0[i], r1[i]);
+    float2* turn = turn_of_warp[warp];
+    const int position = p.positions[(t / p.S) * p.pos_batch + t % p.S];
+    for (int i = lane; i < half; i += 32) turn[i] = turn_of(position, p.inv_freq[i], p.mult);
+    __syncwarp();
+    if (rows.outside && lane == 0) report_status(p.status, STATUS_BAD_INDEX);
     float cs[CH], sn[CH];
-    bool have_turns = false;
-    for (int base = h_begin; base < h_end; base += GROUPS * kRopeBatch) {
-        Piece<E, CH> r0[kRopeBatch], r1[kRopeBatch];
 #pragma unroll
-        for (int i = 0; i < kRopeBatch; ++i) {
+    for (int j = 0; j < CH; ++j) {
+        const float2 u = turns ? turn[pair0 + j] : make_float2(1.f, 0.f);
+        cs[j] = u.x;
+        sn[j] = u.y;
+    }
+    for (int base = h_begin; base < h_end; base += GROUPS * kRopeAhead) {
+#pragma unroll
+        for (int i = 0; i < kRopeAhead; ++i) {
             const int h = base + i * GROUPS + group;
-            if (h < h_end && own) {
-                const int kind = kind_of(h);
-                const E* src = pick(rows.src, kind) + index_of(h, kind) * pick(rows.src_step, kind);
-                r0[i].load(src + o0);
-                r1[i].load(src + o1);
-            } else {
-#pragma unroll
-                for (int j = 0; j < CH / 2; ++j) r0[i].w[j] = r1[i].w[j] = 0;
-            }
-        }
-        if (!have_turns) {
-            const int b = t / p.S, s = t - b * p.S;
-            if ((int)threadIdx.x < half) turn[threadIdx.x] = turn_of(p.positions[b * p.pos_batch + s], p.inv_freq[threadIdx.x], p.mult);
-            __syncthreads();
-            have_turns = true;
-            if (rows.outside && threadIdx.x == 0) report_status(p.status, STATUS_BAD_INDEX);
-#pragma unroll
-            for (int j = 0; j < CH; ++j) {
-                const float2 u = turns ? turn[pair0 + j] : make_float2(1.f, 0.f);
-                cs[j] = u.x;
-                sn[j] = u.y;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < kRopeBatch; ++i) {
-            const int h = base + i * GROUPS + group;
-            if (base + i * GROUPS >= h_end) break;      // the same for all threads of the block
+            if (base + i * GROUPS >= h_end) break;      // the same for the whole warp
             const bool live = h < h_end && own;
             const int kind = kind_of(h);
             float a[CH], c[CH];
             r0[i].unpack(a);
             r1[i].unpack(c);
-            const E* weight = static_cast<const E*>(kind == 0 ? p.q_norm : kind == 1 ? p.k_norm : nullptr);
+            fetch(h + kRopeAhead * GROUPS, r0[i], r1[i]);
             if (p.q_norm != nullptr || p.k_norm != nullptr) {
-                float ss = 0.f;
+                uint64_t ss2 = pair_of(0.f);
 #pragma unroll
-                for (int j = 0; j < CH; ++j) ss = fmaf(a[j], a[j], fmaf(c[j], c[j], ss));
+                for (int j = 0; j < CH; j += 2) ss2 = fma2(pair_of(a[j], a[j + 1]), pair_of(a[j], a[j + 1]), fma2(pair_of(c[j], c[j + 1]), pair_of(c[j], c[j + 1]), ss2));
+                float ss, ss1;
+                unpair(ss2, ss, ss1);
+                ss += ss1;
 #pragma unroll
                 for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                const E* weight = static_cast<const E*>(kind == 0 ? p.q_norm : kind == 1 ? p.k_norm : nullptr);
                 if (weight != nullptr && own) {
-                    const float inv = rsqrtf(ss / (float)p.D + p.eps);
-                    Piece<E, CH> w0, w1;                // the same lines for all heads: they stay in L1
+                    const float inv = rsqrtf(fmaf(ss, p.inv_d, p.eps));
+                    Piece<E, CH> w0, w1;                // the same lines for all heads: they stay in L1 (held in registers they are spilled)
                     float wa[CH], wc[CH];
                     w0.load(weight + o0);
                     w1.load(weight + o1);
                     w0.unpack(wa);
                     w1.unpack(wc);
 #pragma unroll
-                    for (int j = 0; j < CH; ++j) {
-                        a[j] = a[j] * inv * wa[j];
-                        c[j] = c[j] * inv * wc[j];
+                    for (int j = 0; j < CH; j += 2) {
+                        unpair(mul2(mul2(pair_of(a[j], a[j + 1]), pair_of(inv)), pair_of(wa[j], wa[j + 1])), a[j], a[j + 1]);
+                        unpair(mul2(mul2(pair_of(c[j], c[j + 1]), pair_of(inv)), pair_of(wc[j], wc[j + 1])), c[j], c[j + 1]);
                     }
                 }
             }
@@ -194,21 +190,22 @@ __global__ void __launch_bounds__(kRopeThreads, 8) head_rope_kernel(const __grid
                     }
                 } else {
 #pragma unroll
-                    for (int j = 0; j < CH; ++j) {
-                        const float a0 = a[j];
-                        a[j] = a0 * cs[j] - c[j] * sn[j];
-                        c[j] = c[j] * cs[j] + a0 * sn[j];
+                    for (int j = 0; j < CH; j += 2) {
+                        const uint64_t a2 = pair_of(a[j], a[j + 1]), c2 = pair_of(c[j], c[j + 1]), co = pair_of(cs[j], cs[j + 1]), si = pair_of(sn[j], sn[j + 1]);
+                        unpair(fma2(c2, pair_of(-sn[j], -sn[j + 1]), mul2(a2, co)), a[j], a[j + 1]);
+                        unpair(fma2(a2, si, mul2(c2, co)), c[j], c[j + 1]);
                     }
                 }
             }
             uint8_t* dst = live ? pick(rows.dst, kind) : nullptr;
-            if (dst != nullptr) dst += index_of(h, kind) * pick(rows.dst_step, kind);
+            if (dst != nullptr) dst += (int64_t)index_of(h, kind) * pick(p.dst_step, kind);
             if (!U8 || kind == 0) {
                 if (dst != nullptr) {
-                    r0[i].pack(a);
-                    r1[i].pack(c);
-                    r0[i].store(reinterpret_cast<E*>(dst) + o0);
-                    r1[i].store(reinterpret_cast<E*>(dst) + o1);
+                    Piece<E, CH> w0, w1;
+                    w0.pack(a);
+                    w1.pack(c);
+                    w0.store(reinterpret_cast<E*>(dst) + o0);
+                    w1.store(reinterpret_cast<E*>(dst) + o1);
                 }
             }
             if (U8) {
@@ -255,7 +252,6 @@ __global__ void __launch_bounds__(kRopeThreads) head_rope_any_kernel(const __gri
     extern __shared__ float2 turn_any[];
     const int t = blockIdx.x, b = t / p.S, s = t - b * p.S;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int h_begin = blockIdx.y * p.per_block, h_end = min(p.heads, h_begin + p.per_block);
     const int half = p.rot >> 1;
     pdl_enter();
     const TokenRows<E> rows = token_rows<E, false>(p, t);
@@ -263,11 +259,11 @@ __global__ void __launch_bounds__(kRopeThreads) head_rope_any_kernel(const __gri
     const int position = p.positions[b * p.pos_batch + s];
     for (int i = threadIdx.x; i < half; i += kRopeThreads) turn_any[i] = turn_of(position, p.inv_freq[i], p.mult);
     __syncthreads();
-    for (int h = h_begin + warp; h < h_end; h += kRopeThreads / 32) {
+    for (int h = warp; h < p.heads; h += kRopeThreads / 32) {
         const int kind = h < p.Hq ? 0 : h < p.Hq + p.Hkv ? 1 : 2, g = kind == 0 ? h : kind == 1 ? h - p.Hq : h - p.Hq - p.Hkv;
         if (rows.dst[kind] == nullptr) continue;
-        const E* src = rows.src[kind] + g * rows.src_step[kind];
-        E* dst = reinterpret_cast<E*>(rows.dst[kind] + g * rows.dst_step[kind]);
+        const E* src = rows.src[kind] + (int64_t)g * p.src_step[kind];
+        E* dst = reinterpret_cast<E*>(rows.dst[kind] + (int64_t)g * p.dst_step[kind]);
         const E* w = static_cast<const E*>(kind == 0 ? p.q_norm : kind == 1 ? p.k_norm : nullptr);
         float inv = 1.f;
         if (w != nullptr) {
@@ -275,7 +271,7 @@ __global__ void __launch_bounds__(kRopeThreads) head_rope_any_kernel(const __gri
             for (int d = lane; d < p.D; d += 32) ss = fmaf(to_float(src[d]), to_float(src[d]), ss);
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            inv = rsqrtf(ss / (float)p.D + p.eps);
+            inv = rsqrtf(fmaf(ss, p.inv_d, p.eps));
         }
         auto value = [&](int d) { return w != nullptr ? to_float(src[d]) * inv * to_float(w[d]) : to_float(src[d]); };
         const int turned = kind == 2 ? 0 : half;
@@ -322,6 +318,12 @@ extern "C" int ovb_qk_norm_rope(const ovb_qk_rope_args* a, ovb_stream_t stream_)
     static_cast<ovb_qk_rope_args&>(p) = *a;
     p.status = status_word();
     p.heads = a->Hq + a->Hkv * (cache ? 2 : 1);
+    p.inv_d = 1.f / (float)a->D;
+    const int64_t to_cache = (int64_t)a->block_size * a->D * (a->kv_u8 ? 1 : 2), steps[6] = {a->q_head, a->k_head, cache ? a->v_head : 0, a->qo_head * 2, cache ? to_cache : a->ko_head * 2, to_cache};
+    for (int i = 0; i < 6; ++i) {
+        OVB_REQUIRE(steps[i] >= 0 && steps[i] <= INT32_MAX, "ovb_qk_norm_rope: heads %lld apart", (long long)steps[i]);
+        (i < 3 ? p.src_step : p.dst_step)[i % 3] = (int)steps[i];
+    }
     const int tokens = a->B * a->S;
     const auto bits = [](const void* x) { return reinterpret_cast<uintptr_t>(x); };
     uintptr_t at = bits(a->q_norm) | bits(a->k_norm) | bits(a->q) | bits(a->q_out) | bits(a->k) | bits(a->k_out) | bits(a->v) | (a->kv_u8 ? 0 : bits(a->k_cache) | bits(a->v_cache));
@@ -335,12 +337,20 @@ extern "C" int ovb_qk_norm_rope(const ovb_qk_rope_args* a, ovb_stream_t stream_)
         OVB_REQUIRE(pieces && ((bits(a->k_cache) | bits(a->v_cache) | bits(a->k_meta) | bits(a->v_meta)) & 3) == 0,
                     "ovb_qk_norm_rope: the u8 cache is served for head sizes and rotations that are multiples of 8 up to 256, in heads that are 8-byte aligned");
     }
-    // heads of a block: all from 512 tokens on (a block per token then fills every SM three times); with fewer, as many as its lanes take at a time
-    const int lanes = (a->D <= 64 ? 32 : a->D <= 128 ? 64 : 128) / ch, at_a_time = pieces ? kRopeThreads / lanes : kRopeThreads / 32;
-    p.per_block = tokens >= 512 ? p.heads : at_a_time;
-    const dim3 grid(tokens, ceil_div(p.heads, p.per_block));
-    OVB_REQUIRE(grid.y <= 65535, "ovb_qk_norm_rope: %d heads", p.heads);
-    if (pieces) OVB_CHECK_CUDA(a->f16 ? run_head_rope<__half>(p, grid, ch, lanes, stream) : run_head_rope<__nv_bfloat16>(p, grid, ch, lanes, stream));
-    else OVB_CHECK_CUDA(launch_pdl(a->f16 ? head_rope_any_kernel<__half> : head_rope_any_kernel<__nv_bfloat16>, grid, dim3(kRopeThreads), (size_t)(a->rot >> 1) * sizeof(float2), stream, p));
+    if (!pieces) {
+        OVB_CHECK_CUDA(launch_pdl(a->f16 ? head_rope_any_kernel<__half> : head_rope_any_kernel<__nv_bfloat16>, dim3(tokens), dim3(kRopeThreads), (size_t)(a->rot >> 1) * sizeof(float2),
+                                  stream, p));
+        return 0;
+    }
+    // parts of a token's heads: as many as rounds while all warps are resident at a time, fewer with more tokens
+    const int lanes = (a->D <= 64 ? 32 : a->D <= 128 ? 64 : 128) / ch, groups = 32 / lanes, rounds = ceil_div(p.heads, groups);
+    const int64_t room = 148ll * kRopeBlocks * (kRopeThreads / 32);
+    int parts = (int)(room / tokens);
+    parts = parts < 1 ? 1 : parts > rounds ? rounds : parts;
+    p.per_warp = ceil_div(rounds, parts) * groups;
+    p.parts = ceil_div(p.heads, p.per_warp);
+    const int64_t blocks = ((int64_t)tokens * p.parts + kRopeThreads / 32 - 1) / (kRopeThreads / 32);
+    OVB_REQUIRE(blocks <= INT32_MAX, "ovb_qk_norm_rope: %d tokens", tokens);
+    OVB_CHECK_CUDA(a->f16 ? run_head_rope<__half>(p, dim3((unsigned)blocks), ch, lanes, stream) : run_head_rope<__nv_bfloat16>(p, dim3((unsigned)blocks), ch, lanes, stream));
     return 0;
 }

@@ -233,11 +233,6 @@ __device__ __forceinline__ void bulk_load_1d(void* dst, const void* src, uint32_
                  : "memory");
 }
 
-// Ask for global memory to be brought into L2 (16-byte aligned, a multiple of 16 bytes).
-__device__ __forceinline__ void bulk_prefetch_l2(const void* src, uint32_t bytes) {
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
-}
-
 // ---------------------------------------------------------------- tcgen05 / TMEM
 // Allocation and release are warp-collective (.sync.aligned): call with a full, converged warp.
 __device__ __forceinline__ void tmem_alloc(uint32_t* smem_result, uint32_t ncols) {
