@@ -7,7 +7,6 @@
 // the kernel that wrote the tokens has finished. The partial sums are integers: they go to shared memory as [token][channel], every CTA of the cluster
 // adds up its share of the tokens over all partials and finishes them, lanes along the channels.
 #include <mutex>
-#include <stdlib.h>
 #include <type_traits>
 
 #include "gemm_i8.cuh"
@@ -16,8 +15,7 @@ namespace ovb {
 
 constexpr int kI8MaxStages = 12;
 constexpr int kI8QuantWarps = 8;
-constexpr int kI8Hold = 8;                          // pieces of eight columns of a row that a quantising thread holds
-constexpr int kI8FusedTokens = 8;
+constexpr int kI8Hold = 8;                          // pieces of eight columns of the row that a quantising thread holds
 constexpr int i8_threads(bool fused) { return fused ? 64 + kI8QuantWarps * 32 : 256; }
 constexpr int kI8FusedBlock = 16 * kI8BlockK;       // a k-block of the codes
 
@@ -33,78 +31,75 @@ struct I8TileParams : I8Params {
     float eps;
 };
 
-// Up to eight rows, quantised by eight warps into the swizzled operand of the MMA ([k-block][16 rows][128 bytes]; the last eight rows are not set, their
-// sums are not read). Every CTA needs the largest magnitude of whole rows, so it reads them whole, and keeps the codes of its k-blocks. All rows go at a
-// time, each to eight, four, two warps or one, which hold it in registers.
+// The row of a single token, quantised by eight warps into the swizzled operand of the MMA ([k-block][16 rows][128 bytes]; the other rows are not set,
+// their sums are not read). Every CTA needs the largest magnitude of the whole row, so it reads it whole, and keeps the codes of its k-blocks.
 template <class E>
-__device__ __forceinline__ void i8_quantize_rows(const I8TileParams& p, uint8_t* codes, int kb0, int kb1, float* row_scale, int* row_sum, float* box_f, uint32_t* box_u, int* box_i) {
+__device__ __forceinline__ void i8_quantize_row(const I8TileParams& p, uint8_t* codes, int kb0, int kb1, float* row_scale, int* row_sum, float* box_f, uint32_t* box_u, int* box_i) {
+    constexpr int SPAN = kI8QuantWarps * 32;
     const int tid = threadIdx.x - 64, warp = tid >> 5, lane = tid & 31, pieces = p.K >> 3;
-    const int wpr = p.T == 1 ? 8 : p.T == 2 ? 4 : p.T <= 4 ? 2 : 1, span = wpr * 32;        // warps and threads of a row
-    const int t = warp / wpr, first_warp = t * wpr, at0 = tid - first_warp * 32;
-    auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(kI8QuantWarps * 32) : "memory"); };
-    const bool live = t < p.T;
+    auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(SPAN) : "memory"); };
     uint4 x[kI8Hold], g[kI8Hold];
-    int row = t;
-    if (live && p.row_idx != nullptr) {
-        row = p.row_idx[t];
+    int row = 0;
+    if (p.row_idx != nullptr) {
+        row = p.row_idx[0];
         if (row < 0 || row >= p.raw_rows) row = 0;
     }
     const uint4* src = reinterpret_cast<const uint4*>(static_cast<const E*>(p.raw) + row * p.ld_raw);
 #pragma unroll
     for (int h = 0; h < kI8Hold; ++h) {
-        const int at = at0 + h * span;
-        x[h] = live && at < pieces ? __ldcg(src + at) : make_uint4(0, 0, 0, 0);
-        if (p.gamma != nullptr && live && at < pieces) g[h] = __ldg(static_cast<const uint4*>(p.gamma) + at);
+        const int at = tid + h * SPAN;
+        x[h] = at < pieces ? __ldcg(src + at) : make_uint4(0, 0, 0, 0);
+        if (p.gamma != nullptr && at < pieces) g[h] = __ldg(static_cast<const uint4*>(p.gamma) + at);
     }
     float inv = 1.f;
     if (p.gamma != nullptr) {
-        float ss = 0.f;
+        // in the order of ovb_quantize_rows for few rows of up to 4096 columns
+        uint64_t ss2 = pair_of(0.f);
 #pragma unroll
         for (int h = 0; h < kI8Hold; ++h) {
-            const E* e = reinterpret_cast<const E*>(&x[h]);
+            float v[8];
+            row_values<E, false>(x[h], x[h], 1.f, v);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) ss = fmaf(to_float(e[j]), to_float(e[j]), ss);
+            for (int j = 0; j < 8; j += 2) ss2 = fma2(pair_of(v[j], v[j + 1]), pair_of(v[j], v[j + 1]), ss2);
         }
+        float ss, ss1;
+        unpair(ss2, ss, ss1);
+        ss += ss1;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         if (lane == 0) box_f[warp] = ss;
         meet();
-        ss = 0.f;
-        for (int w = 0; w < wpr; ++w) ss += box_f[first_warp + w];
+        ss = box_f[lane % kI8QuantWarps];
+#pragma unroll
+        for (int o = kI8QuantWarps / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         inv = rsqrtf(ss / (float)p.K + p.eps);
     }
-    auto value = [&](int h, int j) {
-        const float v = to_float(reinterpret_cast<const E*>(&x[h])[j]);
-        return p.gamma != nullptr ? v * inv * to_float(reinterpret_cast<const E*>(&g[h])[j]) : v;
-    };
+    const bool norm = p.gamma != nullptr;
     uint32_t top = 0;
 #pragma unroll
     for (int h = 0; h < kI8Hold; ++h)
-        if (live && at0 + h * span < pieces) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) top = max(top, magnitude(value(h, j)));
-        }
+        if (tid + h * SPAN < pieces) top = norm ? top_of8<E, true>(x[h], g[h], inv, top) : top_of8<E, false>(x[h], x[h], 1.f, top);
+    top = norm ? top : row_top<E, false>(top);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (lane == 0) box_u[warp] = top;
     meet();
     top = 0;
-    for (int w = 0; w < wpr; ++w) top = max(top, box_u[first_warp + w]);
+#pragma unroll
+    for (int w = 0; w < kI8QuantWarps; ++w) top = max(top, box_u[w]);
     const float f = row_factor(top);
     int sum = 0;
 #pragma unroll
     for (int h = 0; h < kI8Hold; ++h) {
-        const int at = at0 + h * span, kb = at >> 4;
+        const int at = tid + h * SPAN, kb = at >> 4;
         const bool mine = kb >= kb0 && kb < kb1;
-        if (!live || at >= pieces || (!mine && p.w_zp == nullptr)) continue;
-        uint32_t w[2] = {0, 0};
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int c = f != 0.f ? __float2int_rn(__fmul_rn(value(h, j), f)) : 0;
-            sum += c;
-            w[j >> 2] |= (uint32_t)(c & 0xFF) << (8 * (j & 3));
-        }
-        if (mine) *reinterpret_cast<uint2*>(codes + (kb - kb0) * kI8FusedBlock + t * 128 + ((((at & 15) >> 1) ^ t) << 4) + ((at & 1) << 3)) = make_uint2(w[0], w[1]);
+        if (at >= pieces || (!mine && p.w_zp == nullptr)) continue;
+        float v[8];
+        if (norm) row_values<E, true>(x[h], g[h], inv, v);
+        else row_values<E, false>(x[h], x[h], 1.f, v);
+        const uint2 w = f != 0.f ? codes_of8(v, f) : make_uint2(0, 0);
+        sum = sum_of8(w, sum);
+        if (mine) *reinterpret_cast<uint2*>(codes + (kb - kb0) * kI8FusedBlock + ((at & 15) << 3)) = w;      // row 0 of the swizzle: in order
     }
     if (p.w_zp != nullptr) {
 #pragma unroll
@@ -113,12 +108,12 @@ __device__ __forceinline__ void i8_quantize_rows(const I8TileParams& p, uint8_t*
     }
     fence_proxy_async_smem();                           // the codes are read by the tensor cores
     meet();
-    if (live && at0 == 0) {
-        row_scale[t] = row_scale_of(top);
+    if (tid == 0) {
+        *row_scale = row_scale_of(top);
         sum = 0;
         if (p.w_zp != nullptr)
-            for (int w = 0; w < wpr; ++w) sum += box_i[first_warp + w];
-        row_sum[t] = sum;
+            for (int w = 0; w < kI8QuantWarps; ++w) sum += box_i[w];
+        *row_sum = sum;
     }
 }
 
@@ -131,8 +126,8 @@ __global__ void __launch_bounds__(i8_threads(FUSED)) gemm_i8_tile_kernel(const _
     __shared__ uint64_t full[kI8MaxStages], empty[kI8MaxStages], done, rows_ready;
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
-    __shared__ float row_scale[FUSED ? kI8FusedTokens : 256];
-    __shared__ int row_sum[FUSED ? kI8FusedTokens : 256];
+    __shared__ float row_scale[FUSED ? 1 : 256];
+    __shared__ int row_sum[FUSED ? 1 : 256];
     volatile int* abort_flag = &abort_word;
 
     // the shuffle tells the compiler that a warp's index is the same in all lanes: the MMA loop below then runs on uniform registers
@@ -209,7 +204,7 @@ __global__ void __launch_bounds__(i8_threads(FUSED)) gemm_i8_tile_kernel(const _
         __shared__ uint32_t box_u[8];
         __shared__ int box_i[8];
         pdl_wait();
-        i8_quantize_rows<E>(p, smem, kb0, kb1, row_scale, row_sum, box_f, box_u, box_i);
+        i8_quantize_row<E>(p, smem, kb0, kb1, row_scale, row_sum, box_f, box_u, box_i);
         if (threadIdx.x == 64) mbar_arrive(&rows_ready);
     }
     // while the products run: the scales of this thread's four channels and of the tokens (which the kernel before this one may have written)
@@ -260,7 +255,7 @@ __global__ void __launch_bounds__(i8_threads(FUSED)) gemm_i8_tile_kernel(const _
         const int cols = GATED ? p.N >> 1 : p.N, col = GATED ? (n0 >> 1) + lane * 4 : n, left = GATED && lane >= 16 ? 0 : cols - col;
         // S partials of as many tokens as give sixteen loads in flight. WHOLE: 16-bit results, four columns of a row in one aligned access.
         auto finish = [&](auto count, auto kind) {
-            constexpr int S = decltype(count)::value, AT_ONCE = FUSED ? 1 : S == 1 ? 4 : 16 / S;      // (eight rows at most go to ten warps)
+            constexpr int S = decltype(count)::value, AT_ONCE = FUSED ? 1 : S == 1 ? 4 : 16 / S;
             constexpr bool WHOLE = decltype(kind)::value;
             uint32_t from[S];
 #pragma unroll
@@ -306,7 +301,7 @@ __global__ void __launch_bounds__(i8_threads(FUSED)) gemm_i8_tile_kernel(const _
                         if (!GATED && p.residual != nullptr) {
                             const E* e = reinterpret_cast<const E*>(&res[i]);
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) v[j] += to_float(e[j]);
+                            for (int j = 0; j < 4; ++j) v[j] = __fadd_rn(v[j], to_float(e[j]));
                         }
                         if (left > 0 && first + i * WARPS < share1) *reinterpret_cast<uint2*>(static_cast<E*>(p.out) + at) = make_uint2(pack_pair<E>(v[0], v[1]), pack_pair<E>(v[2], v[3]));
                     } else {
@@ -314,7 +309,7 @@ __global__ void __launch_bounds__(i8_threads(FUSED)) gemm_i8_tile_kernel(const _
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
                             if (j < left) {
-                                if (p.residual != nullptr) v[j] += to_float(static_cast<const E*>(p.residual)[(size_t)(t0 + t) * p.ldr + col + j]);
+                                if (p.residual != nullptr) v[j] = __fadd_rn(v[j], to_float(static_cast<const E*>(p.residual)[(size_t)(t0 + t) * p.ldr + col + j]));
                                 if (p.out_f32) static_cast<float*>(p.out)[at + j] = v[j];
                                 else static_cast<E*>(p.out)[at + j] = from_float<E>(v[j]);
                             }
@@ -366,8 +361,6 @@ __global__ void __launch_bounds__(256) pack_i8_kernel(const uint8_t* __restrict_
     }
 }
 
-static int env_int(const char* n, int d) { const char* v = getenv(n); return v ? atoi(v) : d; }
-
 template <bool F16, bool FUSED, int FORM>
 static int launch_i8_tile(const cudaLaunchConfig_t& cfg, const CUtensorMap& tm, const I8TileParams& p) {
     static std::mutex mu;
@@ -392,15 +385,68 @@ static int launch_i8_tile(int form, const cudaLaunchConfig_t& cfg, const CUtenso
     }
 }
 
-// Rows that the kernel quantises itself: whole aligned pieces of eight columns, as many as six warps hold.
+// A single token's row is quantised by the product's kernel: whole aligned pieces of eight columns, as many as eight warps hold. (us with a norm, one launch / two:
+// 1 x 6144 x 4096 9.6 / 9.8, where the second launch also costs the host 2.5. With four rows the kernel's own way costs more than it saves: 4 x 4096 x 4096
+// 10.2 / 8.3.)
 static bool i8_fuses(const ovb_gemm_i8_args* a) {
     const auto bits = [](const void* x) { return reinterpret_cast<uintptr_t>(x); };
-    const int rows = a->T <= 2 ? a->T : a->T <= 4 ? 4 : 8;       // as the warps share them
-    return a->raw != nullptr && a->T <= kI8FusedTokens && a->K % 8 == 0 && rows * a->K <= kI8QuantWarps * 32 * kI8Hold * 8 && (a->T == 1 || a->ld_raw % 8 == 0) &&
-           ((bits(a->raw) | bits(a->gamma)) & 15) == 0 && env_int("OVB_I8_FUSE", 1);
+    return a->raw != nullptr && a->T == 1 && a->K % 8 == 0 && a->K <= kI8QuantWarps * 32 * kI8Hold * 8 && (a->row_idx == nullptr || a->ld_raw % 8 == 0) &&
+           ((bits(a->raw) | bits(a->gamma)) & 15) == 0;
 }
 
-static int run_i8_tile(const ovb_gemm_i8_args* a, const I8Params& base, bool fused, cudaStream_t stream) {
+// How a product is run: pairs of CTAs, or tiles of `bt` tokens whose K is shared by `splits` CTAs, with `room` KB of shared memory each (108: two to an SM).
+struct I8Plan {
+    bool pair;
+    int bt, splits, room;
+};
+
+// The fastest of the candidates by an estimate in us, fitted to 607 products (1 to 4096 tokens, 256 to 28672 channels, K 256 to 14336, cold weights): the
+// geometric mean of what the choice loses against the best candidate is 1.3 %, one in twenty loses more than 8 %, the worst 29 %.
+//  * tiles: waves of CTAs, of clusters where K is shared (as many as the device holds), each with its start and epilogue, its k-blocks at the issue rate of the
+//    products, the bytes that an SM takes (both shared by the CTAs of an SM) or the latency that its stages hide, whichever is longest; the exchange of
+//    partial sums; never less than the weights take from memory
+//  * pairs: waves of 256 x 256 tiles
+// us, 1 x 6144 x 4096 7.1; 64 x 28672 x 4096 21.6 (pairs 26.7); 256 x 28672 x 4096 39.5, pairs 30.2; 512 x 4096 x 4096 13.3, pairs 15.0; 999 x 8192 x 8192
+// 62.9, pairs 47.8.
+static bool i8_plan(int T, int N, int KB, bool fused, I8Plan* plan) {
+    const int tiles_n = ceil_div(N, TILE_N), t16 = T > 256 ? 256 : (T + 15) / 16 * 16;
+    *plan = {true, 256, 1, 216};
+    const double pair_waves = (double)(((int64_t)ceil_div(T, 256) * ceil_div(N, 256) + 73) / 74);
+    double best_us = fused ? 1e30 : 7.044 + pair_waves * KB * 0.3226 + (pair_waves - 1) * 5.848;
+    const double bytes_us = 1.314 + (double)N * KB * 128 / 6.4e6;
+    static constexpr int heights[6] = {16, 32, 64, 128, 256, 0};
+    for (int i = 0; i < 6; ++i) {
+        const int bt = heights[i] ? heights[i] : t16;
+        if (bt > t16 || (heights[i] == t16 && i < 5)) continue;          // (the last one is t16 itself)
+        if (fused && bt != 16) continue;
+        const int64_t tiles = (int64_t)tiles_n * ceil_div(T, bt);
+        if (ceil_div(T, bt) > 65535) continue;
+        for (int room = 108; room <= 216; room += 108) {
+            const int per_sm = 216 / room, stages = room * 8 / (128 + bt) < kI8MaxStages ? room * 8 / (128 + bt) : kI8MaxStages;
+            if (stages < 3) continue;
+            for (int S = 1; S <= 8 && S <= KB; S *= 2) {
+                if (S > 1 && tiles * S > 444) break;
+                if (fused && ceil_div(KB, S) * kI8FusedBlock + 3 * kI8TileBytes > room * 1024) continue;      // the row's codes stay in shared memory
+                const int64_t slots = (int64_t)(S == 1 ? 148 : cluster_capacity(S)) * per_sm;
+                const double waves = (double)((tiles + slots - 1) / slots);
+                const double share = tiles * S <= 148 ? 1 : per_sm;
+                const double issue = 0.1886 * share, bytes = 0.005616 * (16 + bt / 8.0) * share, latency = 1.649 / stages;
+                double block = issue > bytes ? issue : bytes;
+                if (latency > block) block = latency;
+                double us = waves * (5.365 + ceil_div(KB, S) * block + 0.007415 * bt / S * share);
+                if (S > 1) us += 2.164 + 0.01968 * bt * (S - 1) / S;
+                if (us < bytes_us) us = bytes_us;
+                if (us < best_us) {
+                    best_us = us;
+                    *plan = {false, bt, S, room};
+                }
+            }
+        }
+    }
+    return best_us < 1e30;
+}
+
+static int run_i8_tile(const ovb_gemm_i8_args* a, const I8Params& base, const I8Plan& plan, bool fused, cudaStream_t stream) {
     I8TileParams p;
     static_cast<I8Params&>(p) = base;
     const auto bits = [](const void* x) { return reinterpret_cast<uintptr_t>(x); };
@@ -411,19 +457,14 @@ static int run_i8_tile(const ovb_gemm_i8_args* a, const I8Params& base, bool fus
     p.ld_raw = a->ld_raw;
     p.raw_rows = a->raw_rows;
     p.eps = a->eps;
-    p.bt = fused ? 16 : a->T <= 256 ? (a->T + 15) / 16 * 16 : 256;
-    p.bt = fused ? p.bt : env_int("OVB_I8_BT", p.bt);
+    p.bt = plan.bt;
+    p.splits = plan.splits;
     const int tiles = ceil_div(a->N, TILE_N), rows = ceil_div(a->T, p.bt);
-    p.splits = 1;
-    while (p.splits < 8 && (int64_t)tiles * rows * p.splits * 2 <= 160 && p.KB >= p.splits * 2) p.splits *= 2;
-    p.splits = env_int("OVB_I8_S", p.splits);
-    if (p.splits > p.KB) p.splits = p.KB;
     const int per_split = ceil_div(p.KB, p.splits);
     const int stage = kI8TileBytes + (fused ? 0 : p.bt * kI8BlockK), head = fused ? per_split * kI8FusedBlock : 0;
-    p.stages = (env_int("OVB_I8_KB", 216) * 1024 - head) / stage;
+    p.stages = (plan.room * 1024 - head) / stage;
     if (p.stages > kI8MaxStages) p.stages = kI8MaxStages;
     if (p.stages > per_split) p.stages = per_split;
-    if (p.stages < 1) p.stages = 1;
     int bytes = p.stages * stage;
     if (bytes < p.bt * TILE_N * 4) bytes = p.bt * TILE_N * 4;
     CUtensorMap tm;
@@ -492,7 +533,10 @@ int ovb_gemm_i8(const ovb_gemm_i8_args* a, ovb_stream_t stream_) {
     OVB_REQUIRE(a->residual == nullptr || !a->out_f32, "ovb_gemm_i8: a residual belongs to a 16-bit output");
     const int cols = gated ? a->N / 2 : a->N;
     OVB_REQUIRE(a->ldo >= cols && (a->residual == nullptr || a->ldr >= cols), "ovb_gemm_i8: row pitch of the output %d or residual %d below %d columns", a->ldo, a->ldr, cols);
-    const bool fused = i8_fuses(a);
+    I8Plan plan;
+    const int KB = ceil_div(a->K, kI8BlockK);
+    const bool fused = i8_fuses(a) && i8_plan(a->T, a->N, KB, true, &plan);
+    if (!fused) i8_plan(a->T, a->N, KB, false, &plan);
     if (a->raw != nullptr && !fused) {
         const ovb_quant_rows_args rows = {a->raw, a->gamma, a->row_idx, const_cast<void*>(a->x), const_cast<float*>(a->x_scale), const_cast<int*>(a->x_sum), a->ld_raw, a->T, a->K,
                                           a->raw_rows, a->ldx, a->f16, a->eps};
@@ -509,11 +553,11 @@ int ovb_gemm_i8(const ovb_gemm_i8_args* a, ovb_stream_t stream_) {
     p.out = a->out;
     p.status = status_word();
     p.T = a->T; p.N = a->N; p.K = a->K;
-    p.KB = ceil_div(a->K, kI8BlockK);
+    p.KB = KB;
     p.ldo = a->ldo; p.ldr = a->ldr;
     p.act = a->act; p.out_f32 = a->out_f32;
     p.act_limit = a->act_limit; p.act_slope = a->act_slope; p.act_shift = a->act_shift;
-    return a->T > env_int("OVB_I8_PAIR", 256) ? gemm_i8_pair(a, p, env_int("OVB_I8_BN", 256), stream) : run_i8_tile(a, p, fused, stream);
+    return plan.pair ? gemm_i8_pair(a, p, stream) : run_i8_tile(a, p, plan, fused, stream);
 }
 
 }  // extern "C"

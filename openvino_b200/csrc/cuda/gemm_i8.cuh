@@ -61,10 +61,56 @@ inline int i8_form(const ovb_gemm_i8_args* a) {
     if (is_gated(a->act)) return a->w_zp != nullptr ? kI8GatedZp : kI8Gated;
     return a->act == OVB_ACT_NONE && a->bias == nullptr && a->w_zp == nullptr ? kI8Plain : kI8Any;
 }
+// Codes of eight values, in order. 1.5 * 2^23 added to a value within +-2^22 rounds it to a whole number, halves to even, whose low byte is the sum's: the same
+// as rint, without a conversion (of which an SM does 16 at a time).
+__device__ __forceinline__ uint2 codes_of8(const float (&y)[8], float f) {
+    uint32_t b[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b[j] = __float_as_uint(__fadd_rn(__fmul_rn(y[j], f), 12582912.f));      // (as pairs, mul.rn and add.rn come out fused)
+    return make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
+                      __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
+}
+__device__ __forceinline__ int sum_of8(uint2 codes, int sum) { return __dp4a((int)codes.y, 0x01010101, __dp4a((int)codes.x, 0x01010101, sum)); }
+
+// Eight values of a row: x, or x * inv * gamma.
+template <class E, bool NORM>
+__device__ __forceinline__ void row_values(const uint4& x, const uint4& g, float inv, float (&v)[8]) {
+    const E* e = reinterpret_cast<const E*>(&x);
+    const E* w = reinterpret_cast<const E*>(&g);
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        uint64_t y = pair_of(to_float(e[j]), to_float(e[j + 1]));
+        if (NORM) y = mul2(mul2(y, pair_of(inv)), pair_of(to_float(w[j]), to_float(w[j + 1])));
+        unpair(y, v[j], v[j + 1]);
+    }
+}
+// The largest magnitude of eight values, as the bits of fp32. Without a norm the 16-bit values are compared as pairs of integers.
+template <class E, bool NORM>
+__device__ __forceinline__ uint32_t top_of8(const uint4& x, const uint4& g, float inv, uint32_t top) {
+    if (NORM) {
+        float v[8];
+        row_values<E, true>(x, g, inv, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = max(top, magnitude(v[j]));
+        return top;
+    }
+    constexpr uint32_t M = 0x7FFF7FFFu;                 // (here `top` is a pair of 16-bit magnitudes: see row_top)
+    return __vmaxu2(top, __vmaxu2(__vmaxu2(x.x & M, x.y & M), __vmaxu2(x.z & M, x.w & M)));
+}
+template <class E, bool NORM>
+__device__ __forceinline__ uint32_t row_top(uint32_t top) {
+    if (NORM) return top;
+    const uint32_t half = max(top & 0xFFFFu, top >> 16);
+    const uint16_t bits = (uint16_t)half;
+    return magnitude(to_float(*reinterpret_cast<const E*>(&bits)));
+}
+
+// The roundings are written out, the residual's addition is __fadd_rn: left to the compiler, products and sums are fused in some kernels and paths and not in
+// others, and a call's bits would go by its sizes and alignment.
 template <int FORM>
 __device__ __forceinline__ float i8_value(int acc, int zp, int sum, float scale, float bias) {
     const float v = float(i8_zp_form(FORM) ? acc - zp * sum : acc);
-    return FORM == kI8Any ? fmaf(v, scale, bias) : v * scale;
+    return FORM == kI8Any ? fmaf(v, scale, bias) : __fmul_rn(v, scale);
 }
 template <class P>
 __device__ __forceinline__ float i8_gate(const P& p, float g, float u) {
@@ -72,6 +118,6 @@ __device__ __forceinline__ float i8_gate(const P& p, float g, float u) {
 }
 
 // gemm_i8_pair.cu: many tokens, pairs of CTAs.
-int gemm_i8_pair(const ovb_gemm_i8_args* a, const I8Params& p, int bn, cudaStream_t stream);
+int gemm_i8_pair(const ovb_gemm_i8_args* a, const I8Params& p, cudaStream_t stream);
 
 }  // namespace ovb

@@ -16,13 +16,12 @@ namespace ovb {
 constexpr int kI8PairStages = 6;
 constexpr int kI8PairThreads = 384;
 constexpr int kI8PairStageBytes = 2 * kI8TileBytes;                      // 128 tokens and up to 128 weight rows
-constexpr int kI8PairChannels = 256;                                     // channels of a tile at most
+constexpr int kI8PairChannels = 256;                                     // channels of a tile, half of which each CTA loads
 constexpr int kI8PairBox = 2048;                                         // 32 rows x 64 bytes of an epilogue warp, on their way from rows to lines
 constexpr int kI8PairBand = 8;                                           // token tiles per rasterisation band
 constexpr int kI8PairSmem = kI8PairStages * kI8PairStageBytes + 8 * kI8PairBox + 2 * kI8PairChannels * 12 + 1024 + 1024;
 
 struct I8PairParams : I8Params {
-    int bn;                       // channels of a tile: 256 or 128
     int tiles_n, tiles_t;
     int whole;                    // 16-bit results and residuals in aligned pieces of eight columns
 };
@@ -33,7 +32,7 @@ __device__ __forceinline__ bool i8_pair_tile(const I8PairParams& p, int idx, int
     const int band_sz = kI8PairBand * p.tiles_n, band = idx / band_sz, r = idx - band * band_sz;
     const int in_band = min(kI8PairBand, p.tiles_t - band * kI8PairBand), n = r / in_band;
     t0 = (band * kI8PairBand + (r - n * in_band)) * 256;
-    n0 = n * p.bn;
+    n0 = n * kI8PairChannels;
     return true;
 }
 
@@ -100,7 +99,6 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
     tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot;
     const int pairs = (int)gridDim.x >> 1, first = (int)blockIdx.x >> 1;
-    const int half_n = p.bn >> 1;                       // weight rows that a CTA loads
     pdl_wait();
 
     if (warp == 0) {
@@ -108,12 +106,10 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
             int s = 0, t0, n0;
             uint32_t phase = 1;
             bool ok = true;
-            const uint32_t tx = 2u * (kI8TileBytes + half_n * kI8BlockK);
+            const uint32_t tx = 2u * kI8PairStageBytes;
             for (int idx = first; ok && i8_pair_tile(p, idx, t0, n0); idx += pairs) {
-                // the weight's rows as they are packed: 128 of a chunk, chunk after chunk along K. Channels behind the last chunk are not there: the
-                // box then reads the last chunk's again, and nothing of them is stored
-                const int row = n0 + (int)rank * half_n;
-                int w_row = min(row / TILE_N, (p.N - 1) / TILE_N) * p.KB * TILE_N + row % TILE_N;
+                // one packed chunk of 128 rows for every k-block. An odd last chunk is read by both CTAs; what the second one makes of it is not stored
+                int w_row = min(n0 / TILE_N + (int)rank, (p.N - 1) / TILE_N) * p.KB * TILE_N;
                 const int x_row = t0 + (int)rank * 128;
                 for (int kb = 0; kb < p.KB; ++kb) {
                     ok = mbar_wait(&empty[s], phase, abort_flag, p.status);
@@ -132,7 +128,7 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
     } else if (warp == 1) {
         if (rank == 0) {
             const uint64_t desc0 = umma_desc_k_sw128(smem_u32(smem), 1024);
-            const uint32_t idesc = umma_idesc_i8(256, p.bn);
+            const uint32_t idesc = umma_idesc_i8(256, kI8PairChannels);
             int s = 0, buf = 0, t0, n0;
             uint32_t phase = 0, acc_phase = 1;
             // no way out of the loops: once a wait has run out all later ones return at once, and what is computed then is not stored
@@ -159,7 +155,7 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
         // A job is 32 columns of the result: 32 of the tile's, or the gate and the up values of the same channels (64 rows of a weight tile are the gate, then
         // 64 the up values), in two steps of 16. The two warps of a token quarter take jobs in turn.
         constexpr int RUNS = GATED ? 2 : 1;
-        const int jobs = p.bn / (32 * RUNS);
+        constexpr int JOBS = kI8PairChannels / (32 * RUNS);
         const int out_cols = GATED ? p.N >> 1 : p.N;
         auto column = [&](int job, int run, int step) { return (GATED ? (job >> 1) * 128 + (job & 1) * 32 + run * 64 : job * 32) + step * 16; };
         // this warp's box: 64 bytes of each of its 32 rows, pieces of 16 bytes placed so that rows and lines are both free of bank conflicts
@@ -175,12 +171,10 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
             float* cs = chan_scale + buf * kI8PairChannels;
             float* cb = chan_bias + buf * kI8PairChannels;
             int* cz = chan_zp + buf * kI8PairChannels;
-            if (tid < p.bn) {
-                const int n = n0 + tid;
-                cs[tid] = n < p.N ? __ldg(p.w_scale + n) : 0.f;
-                cb[tid] = n < p.N && p.bias != nullptr ? to_float(static_cast<const E*>(p.bias)[n]) : 0.f;
-                cz[tid] = n < p.N && p.w_zp != nullptr ? __ldg(p.w_zp + n) : 0;
-            }
+            const int n = n0 + tid;                     // a channel for each of the 256 threads
+            cs[tid] = n < p.N ? __ldg(p.w_scale + n) : 0.f;
+            cb[tid] = n < p.N && p.bias != nullptr ? to_float(static_cast<const E*>(p.bias)[n]) : 0.f;
+            cz[tid] = n < p.N && p.w_zp != nullptr ? __ldg(p.w_zp + n) : 0;
             // one thread polls and says how it ended; the others wait at the barrier, so that all eight warps go on or leave together
             if (tid == 0) went_well[buf] = mbar_wait(&acc_full[buf], acc_phase, abort_flag, p.status) ? 1 : 0;
             asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -222,7 +216,7 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
             auto finish16 = [&](auto kind) {
                 constexpr bool WHOLE = decltype(kind)::value;
 #pragma unroll 1
-                for (int job = half; job < jobs; job += 2) {
+                for (int job = half; job < JOBS; job += 2) {
                     const int col = (GATED ? n0 >> 1 : n0) + job * 32;
                     const bool res = !GATED && p.residual != nullptr;
                     if (res) {
@@ -250,7 +244,7 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
                                 const uint4 raw = *place;
                                 const E* e = reinterpret_cast<const E*>(&raw);
 #pragma unroll
-                                for (int i = 0; i < 8; ++i) v[h * 8 + i] += to_float(e[i]);
+                                for (int i = 0; i < 8; ++i) v[h * 8 + i] = __fadd_rn(v[h * 8 + i], to_float(e[i]));
                             }
                             *place = make_uint4(pack_pair<E>(v[h * 8], v[h * 8 + 1]), pack_pair<E>(v[h * 8 + 2], v[h * 8 + 3]), pack_pair<E>(v[h * 8 + 4], v[h * 8 + 5]),
                                                 pack_pair<E>(v[h * 8 + 6], v[h * 8 + 7]));
@@ -273,7 +267,7 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
             };
             // fp32 results: 16 columns at a time, two rows of them to a store
             auto finish32 = [&]() {
-                for (int job = half; job < jobs; job += 2)
+                for (int job = half; job < JOBS; job += 2)
                     for (int step = 0; step < 2; ++step) {
                         float v[16];
                         compute(job, step, v);
@@ -355,19 +349,18 @@ static int launch_i8_pair(int form, const CUtensorMap& tmW, const CUtensorMap& t
     }
 }
 
-int gemm_i8_pair(const ovb_gemm_i8_args* a, const I8Params& base, int bn, cudaStream_t stream) {
+int gemm_i8_pair(const ovb_gemm_i8_args* a, const I8Params& base, cudaStream_t stream) {
     I8PairParams p;
     static_cast<I8Params&>(p) = base;
     const auto bits = [](const void* x) { return reinterpret_cast<uintptr_t>(x); };
     const int out_cols = is_gated(a->act) ? a->N / 2 : a->N;
     p.whole = out_cols % 8 == 0 && a->ldo % 8 == 0 && (bits(a->out) & 15) == 0 && (a->residual == nullptr || (a->ldr % 8 == 0 && (bits(a->residual) & 15) == 0));
-    p.bn = bn;
     p.tiles_t = ceil_div(a->T, 256);
-    p.tiles_n = ceil_div(a->N, bn);
+    p.tiles_n = ceil_div(a->N, kI8PairChannels);
     CUtensorMap tmW, tmX;
     if (int rc = make_tmap_2d(&tmX, a->x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a->T, a->K, a->ldx, 128, kI8BlockK, true)) return rc;
     // the chunks are already in the swizzled order of the MMA: plain boxes of rows of 128 bytes
-    if (int rc = make_tmap_2d(&tmW, a->w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)ceil_div(a->N, TILE_N) * p.KB * TILE_N, kI8BlockK, kI8BlockK, bn / 2, kI8BlockK, false)) return rc;
+    if (int rc = make_tmap_2d(&tmW, a->w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)ceil_div(a->N, TILE_N) * p.KB * TILE_N, kI8BlockK, kI8BlockK, TILE_N, kI8BlockK, false)) return rc;
     return a->f16 ? launch_i8_pair<true>(i8_form(a), tmW, tmX, p, stream) : launch_i8_pair<false>(i8_form(a), tmW, tmX, p, stream);
 }
 

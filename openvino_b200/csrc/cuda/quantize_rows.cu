@@ -21,6 +21,8 @@ struct QuantParams {
     float eps;
 };
 
+constexpr int kManyRows = 1024;
+
 // The sum (largest) over the warps that share a row; every thread gets it.
 template <int WPR, class T, class F>
 __device__ __forceinline__ T over_row(T v, T* box, F&& f) {
@@ -48,7 +50,7 @@ __device__ __forceinline__ int source_row(const QuantParams& p, int row) {
 }
 
 // Rows of whole, aligned pieces of eight columns. WPR warps share a row; blocks of max(4, WPR) warps.
-template <class E, int WPR, int HOLD>
+template <class E, bool NORM, int WPR, int HOLD>
 __global__ void __launch_bounds__(WPR < 4 ? 128 : WPR * 32) quantize_rows_kernel(const QuantParams p) {
     constexpr int RPB = WPR < 4 ? 4 / WPR : 1, SPAN = WPR * 32;
     __shared__ float box_f[16];
@@ -56,65 +58,57 @@ __global__ void __launch_bounds__(WPR < 4 ? 128 : WPR * 32) quantize_rows_kernel
     __shared__ int box_i[16];
     const int row = blockIdx.x * RPB + (RPB > 1 ? (int)threadIdx.x / SPAN : 0), at = threadIdx.x % SPAN;
     const int pieces = p.cols >> 3;
-    constexpr bool HELD = HOLD <= 4;            // with more pieces the weights do not fit the registers beside the row: they are read again
-    uint4 g[HELD ? HOLD : 1];
     pdl_enter();
     if (row >= p.rows) return;              // whole warps, and only where rows do not share a block's barriers
-    if (HELD && p.gamma != nullptr) {
-#pragma unroll
-        for (int h = 0; h < HOLD; ++h)
-            if (at + h * SPAN < pieces) g[h] = __ldg(static_cast<const uint4*>(p.gamma) + at + h * SPAN);
-    }
     const uint4* src = reinterpret_cast<const uint4*>(static_cast<const E*>(p.x) + (size_t)source_row(p, row) * p.ldx);
-    uint4 x[HOLD];
+    const uint4* gamma = static_cast<const uint4*>(p.gamma);
+    constexpr bool HELD = NORM && HOLD <= 4;            // with more pieces the weights do not fit the registers beside the row: they are read again
+    uint4 x[HOLD], g[HELD ? HOLD : 1];
 #pragma unroll
     for (int h = 0; h < HOLD; ++h) x[h] = at + h * SPAN < pieces ? __ldcg(src + at + h * SPAN) : make_uint4(0, 0, 0, 0);
+    if (HELD) {
+#pragma unroll
+        for (int h = 0; h < HOLD; ++h)
+            if (at + h * SPAN < pieces) g[h] = __ldg(gamma + at + h * SPAN);
+    }
     float inv = 1.f;
-    if (p.gamma != nullptr) {
-        float ss = 0.f;
+    if (NORM) {
+        uint64_t ss2 = pair_of(0.f);
 #pragma unroll
         for (int h = 0; h < HOLD; ++h) {
-            const E* e = reinterpret_cast<const E*>(&x[h]);
+            float v[8];
+            row_values<E, false>(x[h], x[h], 1.f, v);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) ss = fmaf(to_float(e[j]), to_float(e[j]), ss);
+            for (int j = 0; j < 8; j += 2) ss2 = fma2(pair_of(v[j], v[j + 1]), pair_of(v[j], v[j + 1]), ss2);
         }
-        ss = over_row<WPR>(ss, box_f, [](float a, float b) { return a + b; });
+        float ss, ss1;
+        unpair(ss2, ss, ss1);
+        ss = over_row<WPR>(ss + ss1, box_f, [](float a, float b) { return a + b; });
         inv = rsqrtf(ss / (float)p.cols + p.eps);
     }
-    auto value = [&](int h, int j) {
-        const float v = to_float(reinterpret_cast<const E*>(&x[h])[j]);
-        return p.gamma != nullptr ? v * inv * to_float(reinterpret_cast<const E*>(&g[HELD ? h : 0])[j]) : v;
-    };
     auto weights = [&](int h) {
-        if (!HELD && p.gamma != nullptr) g[0] = __ldg(static_cast<const uint4*>(p.gamma) + at + h * SPAN);
+        if (NORM && !HELD) g[0] = __ldg(gamma + at + h * SPAN);
     };
     uint32_t top = 0;
 #pragma unroll
     for (int h = 0; h < HOLD; ++h)
         if (at + h * SPAN < pieces) {
             weights(h);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) top = max(top, magnitude(value(h, j)));
+            top = top_of8<E, NORM>(x[h], g[HELD ? h : 0], inv, top);
         }
-    top = over_row<WPR>(top, box_u, [](uint32_t a, uint32_t b) { return max(a, b); });
+    top = over_row<WPR>(row_top<E, NORM>(top), box_u, [](uint32_t a, uint32_t b) { return max(a, b); });
     const float f = row_factor(top);
-    const bool codes = f != 0.f;
     uint2* dst = reinterpret_cast<uint2*>(p.q + (size_t)row * p.ldq);
     int sum = 0;
 #pragma unroll
     for (int h = 0; h < HOLD; ++h)
         if (at + h * SPAN < pieces) {
-            uint32_t w[2] = {0, 0};
-            if (codes) {
-                weights(h);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int c = __float2int_rn(__fmul_rn(value(h, j), f));
-                    sum += c;
-                    w[j >> 2] |= (uint32_t)(c & 0xFF) << (8 * (j & 3));
-                }
-            }
-            dst[at + h * SPAN] = make_uint2(w[0], w[1]);
+            float v[8];
+            weights(h);
+            row_values<E, NORM>(x[h], g[HELD ? h : 0], inv, v);
+            const uint2 w = f != 0.f ? codes_of8(v, f) : make_uint2(0, 0);
+            sum = sum_of8(w, sum);
+            dst[at + h * SPAN] = w;
         }
     sum = over_row<WPR>(sum, box_i, [](int a, int b) { return a + b; });
     if (at == 0) row_result(p, row, top, sum);
@@ -152,18 +146,21 @@ __global__ void __launch_bounds__(256) quantize_rows_any_kernel(const QuantParam
     if (threadIdx.x == 0) row_result(p, row, top, sum);
 }
 
-template <class E>
+template <class E, bool NORM>
 static cudaError_t run_quantize(const QuantParams& p, cudaStream_t stream) {
     const bool whole = p.cols % 8 == 0 && p.ldx % 8 == 0 && p.ldq % 8 == 0 &&
                        ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.gamma)) & 15) == 0 && (reinterpret_cast<uintptr_t>(p.q) & 7) == 0;
     if (!whole || p.cols > 32768) return launch_pdl(quantize_rows_any_kernel<E>, dim3(p.rows), dim3(256), 0, stream, p);
     auto go = [&](auto kern, int wpr) { return launch_pdl(kern, dim3(wpr < 4 ? (p.rows + 4 / wpr - 1) / (4 / wpr) : p.rows), dim3(wpr < 4 ? 128 : wpr * 32), 0, stream, p); };
-    if (p.cols <= 512) return go(quantize_rows_kernel<E, 1, 2>, 1);
-    if (p.cols <= 1024) return go(quantize_rows_kernel<E, 1, 4>, 1);
-    if (p.cols <= 4096) return go(quantize_rows_kernel<E, 8, 2>, 8);
-    if (p.cols <= 8192) return go(quantize_rows_kernel<E, 16, 2>, 16);
-    if (p.cols <= 16384) return go(quantize_rows_kernel<E, 16, 4>, 16);
-    return go(quantize_rows_kernel<E, 16, 8>, 16);
+    // Many rows: few warps to a row, with more of it each (from so many on that they fill the machine); few rows: many warps, for the time of one row.
+    const bool many = p.rows >= kManyRows;
+    if (p.cols <= 512) return go(quantize_rows_kernel<E, NORM, 1, 2>, 1);
+    if (p.cols <= 1024) return go(quantize_rows_kernel<E, NORM, 1, 4>, 1);
+    if (p.cols <= 2048) return many ? go(quantize_rows_kernel<E, NORM, 1, 8>, 1) : go(quantize_rows_kernel<E, NORM, 8, 1>, 8);
+    if (p.cols <= 4096) return many ? go(quantize_rows_kernel<E, NORM, 4, 4>, 4) : go(quantize_rows_kernel<E, NORM, 8, 2>, 8);
+    if (p.cols <= 8192) return many ? go(quantize_rows_kernel<E, NORM, 4, 8>, 4) : go(quantize_rows_kernel<E, NORM, 16, 2>, 16);
+    if (p.cols <= 16384) return many ? go(quantize_rows_kernel<E, NORM, 8, 8>, 8) : go(quantize_rows_kernel<E, NORM, 16, 4>, 16);
+    return go(quantize_rows_kernel<E, NORM, 16, 8>, 16);
 }
 
 }  // namespace ovb
@@ -188,6 +185,8 @@ extern "C" int ovb_quantize_rows(const ovb_quant_rows_args* a, ovb_stream_t stre
     p.ldx = a->ldx;
     p.ldq = a->ldq;
     p.eps = a->eps;
-    OVB_CHECK_CUDA(a->f16 ? run_quantize<__half>(p, stream) : run_quantize<__nv_bfloat16>(p, stream));
+    const cudaError_t e = a->gamma != nullptr ? (a->f16 ? run_quantize<__half, true>(p, stream) : run_quantize<__nv_bfloat16, true>(p, stream))
+                                              : (a->f16 ? run_quantize<__half, false>(p, stream) : run_quantize<__nv_bfloat16, false>(p, stream));
+    OVB_CHECK_CUDA(e);
     return 0;
 }

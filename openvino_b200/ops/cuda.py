@@ -409,7 +409,8 @@ def _one_device(first: torch.Tensor, *others) -> int:
     for t in others:
         if t is not None and t.get_device() != d:
             d = -1
-    _need(d >= 0, "the operands have to be on one CUDA device")
+    if d < 0:
+        raise ValueError("the operands have to be on one CUDA device")
     return d
 
 
@@ -443,14 +444,17 @@ class QuantizedRows:
 
 def _raw_rows(x: torch.Tensor, norm):
     """(rows, weights of the norm, eps, row indices) of rows that are to be quantised."""
-    if x.dim() != 2 or x.dtype not in _HALVES:
-        raise ValueError("bf16 or fp16 rows [T, K] are expected, not %s %s" % (x.dtype, tuple(x.shape)))
+    dtype = x.dtype
+    if x.dim() != 2 or (dtype != torch.bfloat16 and dtype != torch.float16):
+        raise ValueError("bf16 or fp16 rows [T, K] are expected, not %s %s" % (dtype, tuple(x.shape)))
     T, cols = x.shape
-    _need(cols > 0 and (x.stride(1) == 1 or cols == 1), "the values of a row have to lie side by side")
+    if cols == 0 or (x.stride(1) != 1 and cols != 1):
+        raise ValueError("the values of a row have to lie side by side")
     if norm is None:
         return T, None, 0.0, None
     gamma, eps, idx = norm[0], norm[1], norm[2] if len(norm) > 2 else None
-    _need(gamma.numel() == cols and gamma.dtype == x.dtype and gamma.is_contiguous(), "the norm's weights are %d values of the rows' type", cols)
+    if gamma.numel() != cols or gamma.dtype != dtype or not gamma.is_contiguous():
+        raise ValueError("the norm's weights are %d values of the rows' type" % cols)
     if idx is not None:
         _need(idx.dtype == torch.int32 and idx.is_contiguous() and T > 0, "row indices are int32, and x has rows")
         T = idx.numel()
@@ -465,8 +469,8 @@ def quantize_rows(x: torch.Tensor, norm=None) -> QuantizedRows:
     T, gamma, eps, idx = _raw_rows(x, norm)
     d = _one_device(x, gamma, idx)
     cols = x.shape[1]
-    q = torch.empty((T, (cols + 15) // 16 * 16), dtype=torch.int8, device=x.device)[:, :cols]
-    scales, sums = torch.empty(T, dtype=torch.float32, device=x.device), torch.empty(T, dtype=torch.int32, device=x.device)
+    q = x.new_empty((T, (cols + 15) // 16 * 16), dtype=torch.int8)[:, :cols]
+    scales, sums = x.new_empty(T, dtype=torch.float32), x.new_empty(T, dtype=torch.int32)
     if T:
         _call(lib().ovb_quantize_rows, _QUANT_ROWS.pack(x.data_ptr(), _ptr(gamma) or 0, _ptr(idx) or 0, q.data_ptr(), scales.data_ptr(), sums.data_ptr(), x.stride(0), T, cols,
                                                         x.shape[0], q.stride(0), x.dtype == torch.float16, eps), d, "ovb_quantize_rows")
@@ -474,47 +478,62 @@ def quantize_rows(x: torch.Tensor, norm=None) -> QuantizedRows:
 
 
 def _gemm_i8(x, w: "PackedWeight", out, residual, act, out_f32, glu, cap, norm) -> torch.Tensor:
+    N, Kd, wt, bias, zps = w.N, w.K, w.w, w.bias, w.zps
     gamma = idx = None
     eps = 0.0
     quantized = isinstance(x, QuantizedRows)
     if quantized:
         _need(norm is None, "rows are normed before they are quantised: give quantize_rows the norm")
-        T, like = x.shape[0], x.q
+        like = x.q
+        T, cols_in = like.shape
     else:
-        T, gamma, eps, idx = _raw_rows(x, norm)
         like = x
-    N, Kd, dtype, bias, zps = w.N, w.K, x.dtype, w.bias, w.zps
-    if x.shape[1] != Kd:
-        raise ValueError("rows of %d values for weights of K = %d" % (x.shape[1], Kd))
-    cols = N // 2 if act in (ACT_SWIGLU, ACT_GLU_LIMITED) else N
-    kind = torch.float32 if out_f32 else dtype
+        T, gamma, eps, idx = _raw_rows(x, norm)
+        cols_in = x.shape[1]
+    dtype = x.dtype
+    if cols_in != Kd:
+        raise ValueError("rows of %d values for weights of K = %d" % (cols_in, Kd))
     if bias is not None and bias.dtype != dtype:
         raise ValueError("the bias is %s, the rows are %s" % (bias.dtype, dtype))
-    _need(act != ACT_GLU_LIMITED or (glu is not None and len(glu) == 3), "ACT_GLU_LIMITED needs its limit, slope and shift")
-    for name, t, of in (("out", out, kind), ("residual", residual, dtype)):
-        if t is not None and not (t.shape == (T, cols) and t.dtype == of and (cols == 1 or t.stride(1) == 1) and (T == 1 or t.stride(0) >= cols)):
-            raise ValueError("%s has to be %s [%d, %d] with the values of a row side by side" % (name, of, T, cols))
-    d = _one_device(like, w.w, gamma, idx, out, residual)
+    gated = act == ACT_SWIGLU or act == ACT_GLU_LIMITED
+    if act == ACT_GLU_LIMITED:
+        _need(glu is not None and len(glu) == 3, "ACT_GLU_LIMITED needs its limit, slope and shift")
+        limit, slope, shift = glu
+    else:
+        limit, slope, shift = cap, 0.0, 0.0
+    cols = N // 2 if gated else N
+    kind = torch.float32 if out_f32 else dtype
+    d = _one_device(like, wt, gamma, idx, out, residual)
     if out is None:
-        out = torch.empty((T, cols), dtype=kind, device=like.device)
+        out = like.new_empty((T, cols), dtype=kind)
+        ldo = cols
+    else:
+        ldo = _result_pitch("out", out, kind, T, cols)
+    ldr = 0 if residual is None else _result_pitch("residual", residual, dtype, T, cols)
     if T == 0:
         return out
     if quantized:
-        pitch, q, scales, sums, raw, ld_raw = x.q.stride(0), x.q.data_ptr(), x.scales.data_ptr(), x.sums.data_ptr(), 0, 0
+        pitch, q, scales, sums, raw, ld_raw = like.stride(0), like.data_ptr(), x.scales.data_ptr(), x.sums.data_ptr(), 0, 0
     else:
         # the quantised rows, their scales and sums: memory of the caching allocator, which belongs to the stream
         pitch = (Kd + 15) // 16 * 16
-        rows = torch.empty(T * (pitch + 8), dtype=torch.uint8, device=like.device)
-        q = rows.data_ptr()
-        scales, raw, ld_raw = q + T * pitch, x.data_ptr(), x.stride(0)
+        rows = x.new_empty(T * (pitch + 8), dtype=torch.uint8)
+        q, raw, ld_raw = rows.data_ptr(), x.data_ptr(), x.stride(0)
+        scales = q + T * pitch
         sums = scales + 4 * T
-    limit, slope, shift = glu if act == ACT_GLU_LIMITED else (cap, 0.0, 0.0)
-    _call(lib().ovb_gemm_i8, _GEMM_I8.pack(q, scales, sums, w.w.data_ptr(), w.scales.data_ptr(), 0 if zps is None else zps.data_ptr(), 0 if bias is None else bias.data_ptr(),
+    _call(lib().ovb_gemm_i8, _GEMM_I8.pack(q, scales, sums, wt.data_ptr(), w.scales.data_ptr(), 0 if zps is None else zps.data_ptr(), 0 if bias is None else bias.data_ptr(),
                                            0 if residual is None else residual.data_ptr(), out.data_ptr(), raw, 0 if gamma is None else gamma.data_ptr(),
-                                           0 if idx is None else idx.data_ptr(), ld_raw, T, N, Kd, pitch, max(out.stride(0), cols),
-                                           0 if residual is None else max(residual.stride(0), cols), act, dtype == torch.float16, bool(out_f32), x.shape[0], limit, slope, shift,
-                                           eps), d, "ovb_gemm_i8")
+                                           0 if idx is None else idx.data_ptr(), ld_raw, T, N, Kd, pitch, ldo, ldr, act, dtype == torch.float16, bool(out_f32),
+                                           like.shape[0] if idx is not None else 0, limit, slope, shift, eps), d, "ovb_gemm_i8")
     return out
+
+
+def _result_pitch(name: str, t: torch.Tensor, dtype, T: int, cols: int) -> int:
+    """The row pitch of a result or residual [T, cols], which has to be of that form."""
+    shape, (ld, step) = t.shape, t.stride() if t.dim() == 2 else (0, 0)
+    if not (len(shape) == 2 and shape[0] == T and shape[1] == cols and t.dtype == dtype and (step == 1 or cols == 1) and (ld >= cols or T <= 1)):
+        raise ValueError("%s has to be %s [%d, %d] with the values of a row side by side" % (name, dtype, T, cols))
+    return max(ld, cols)
 
 
 def gemm(x: torch.Tensor, w: PackedWeight, out: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
@@ -1082,7 +1101,8 @@ def _rope_operands(dtype, D, inv_freq, q_norm, k_norm) -> int:
     if dtype not in _HALVES:
         raise ValueError("bf16 or fp16 heads are expected, not %s" % dtype)
     rot = 2 * inv_freq.numel()
-    _need(inv_freq.dtype == torch.float32 and inv_freq.is_contiguous() and rot <= D, "frequencies are fp32, one for each pair of at most %d dimensions", D)
+    if inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous() or rot > D:
+        raise ValueError("frequencies are fp32, one for each pair of at most %d dimensions" % D)
     for w in (q_norm, k_norm):
         if w is not None and not (w.numel() == D and w.dtype == dtype and w.is_contiguous()):
             raise ValueError("a head norm has %d weights of the heads' type" % D)
@@ -1114,20 +1134,24 @@ def qk_norm_rope(q, k, positions, inv_freq, q_norm=None, k_norm=None, eps=1e-6, 
     dtype = q.dtype
     _need(q.dim() == 4 and k.dim() == 4 and k.dtype == dtype, "queries [B, S, Hq, D] and keys [B, S, Hkv, D] of one type are expected")
     (B, S, Hq, D), (kB, kS, Hkv, kD) = q.shape, k.shape
-    _need(kB == B and kS == S and kD == D and Hq > 0 and Hkv > 0 and D > 0, "queries [B, S, Hq, D] and keys [B, S, Hkv, D] are expected, not %s and %s", tuple(q.shape), tuple(k.shape))
+    if not (kB == B and kS == S and kD == D and Hq > 0 and Hkv > 0 and D > 0):
+        raise ValueError("queries [B, S, Hq, D] and keys [B, S, Hkv, D] are expected, not %s and %s" % (tuple(q.shape), tuple(k.shape)))
     many = positions.dim() == 2
-    _need(positions.dtype == torch.int32 and positions.shape == ((B, S) if many else (S,)) and (S == 1 or positions.stride(-1) == 1), "positions are int32 [S] or [B, S]")
+    if positions.dtype != torch.int32 or positions.shape != ((B, S) if many else (S,)) or (S != 1 and positions.stride(-1) != 1):
+        raise ValueError("positions are int32 [S] or [B, S]")
     rot = _rope_operands(dtype, D, inv_freq, q_norm, k_norm)
-    for t, like in ((q_out, q), (k_out, k)):
-        if t is not None and not (t.shape == like.shape and t.dtype == dtype and _written_once(t)):
-            raise ValueError("outputs have their inputs' shape and type, and no two elements in one place")
+    if q_out is not None or k_out is not None:
+        for t, like in ((q_out, q), (k_out, k)):
+            if t is not None and not (t.shape == like.shape and t.dtype == dtype and _written_once(t)):
+                raise ValueError("outputs have their inputs' shape and type, and no two elements in one place")
     d = _one_device(q, k, positions, inv_freq, q_norm, k_norm, q_out, k_out)
     if q_out is None:
-        q_out = torch.empty((B, S, Hq, D), dtype=dtype, device=q.device)
+        q_out = q.new_empty((B, S, Hq, D))
     if k_out is None:
-        k_out = torch.empty((B, S, Hkv, D), dtype=dtype, device=q.device)
+        k_out = k.new_empty((B, S, Hkv, D))
     qs, ks, qo, ko = q.stride(), k.stride(), q_out.stride(), k_out.stride()
-    _need(qs[3] == 1 and ks[3] == 1 and qo[3] == 1 and ko[3] == 1, "heads have to be contiguous")
+    if not (qs[3] == 1 and ks[3] == 1 and qo[3] == 1 and ko[3] == 1):
+        raise ValueError("heads have to be contiguous")
     if B * S:
         _call(lib().ovb_qk_norm_rope, _QK_ROPE.pack(q.data_ptr(), k.data_ptr(), 0, q_out.data_ptr(), k_out.data_ptr(), 0, 0, 0, 0, positions.data_ptr(), 0, inv_freq.data_ptr(),
                                                     0 if q_norm is None else q_norm.data_ptr(), 0 if k_norm is None else k_norm.data_ptr(), qs[0], qs[1], qs[2], ks[0], ks[1], ks[2],
@@ -1144,25 +1168,27 @@ def qk_norm_rope_kv_write(qkv, positions, slot_map, k_cache, v_cache, inv_freq, 
     offset; negative: not kept; the slots of a call differ) of the caches [num_blocks, Hkv, block_size, D], which are of the type of ``qkv``, or uint8 with
     the fp16 (scale, zero point) tables ``k_meta`` / ``v_meta`` [num_blocks, Hkv, block_size, 2] (D and the rotation multiples of 8, D up to 256).
     A slot behind the cache is not written and shows in the status word."""
-    dtype, u8 = qkv.dtype, k_cache.dtype == torch.uint8
+    dtype, cache_type = qkv.dtype, k_cache.dtype
+    u8 = cache_type == torch.uint8
     width = (Hq + 2 * Hkv) * D
-    _need(qkv.dim() == 2 and min(Hq, Hkv, D, block_size) > 0 and qkv.shape[1] >= width and qkv.stride(1) == 1, "rows [T, %d] with their values side by side are expected, not %s",
-          width, tuple(qkv.shape))
+    if qkv.dim() != 2 or Hq <= 0 or Hkv <= 0 or D <= 0 or block_size <= 0 or qkv.shape[1] < width or qkv.stride(1) != 1:
+        raise ValueError("rows [T, %d] with their values side by side are expected, not %s" % (width, tuple(qkv.shape)))
     T, pitch = qkv.shape[0], qkv.stride(0)
-    for t in (positions, slot_map):
-        if not (t.dtype == torch.int32 and t.dim() == 1 and t.numel() >= T and t.is_contiguous()):
-            raise ValueError("positions and slots are int32, %d values at least" % T)
-    blocks = k_cache.shape[0]
-    for t in (k_cache, v_cache):
-        if not (t.shape == (blocks, Hkv, block_size, D) and t.dtype == (torch.uint8 if u8 else dtype) and t.is_contiguous()):
-            raise ValueError("caches are contiguous [num_blocks, %d, %d, %d] of the type of qkv, or uint8" % (Hkv, block_size, D))
+    if not (positions.dtype == slot_map.dtype == torch.int32 and positions.dim() == slot_map.dim() == 1 and positions.numel() >= T and slot_map.numel() >= T
+            and positions.is_contiguous() and slot_map.is_contiguous()):
+        raise ValueError("positions and slots are int32, %d values at least" % T)
+    blocks, form = k_cache.shape[0], k_cache.shape
+    if not (form[1:] == (Hkv, block_size, D) and v_cache.shape == form and cache_type == v_cache.dtype == (torch.uint8 if u8 else dtype) and k_cache.is_contiguous()
+            and v_cache.is_contiguous()):
+        raise ValueError("caches are contiguous [num_blocks, %d, %d, %d] of the type of qkv, or uint8" % (Hkv, block_size, D))
     if u8:
         for t in (k_meta, v_meta):
             _need(t is not None and t.dtype == torch.float16 and t.shape == (blocks, Hkv, block_size, 2) and t.is_contiguous(),
                   "a uint8 cache needs fp16 tables [num_blocks, %d, %d, 2]", Hkv, block_size)
     rot = _rope_operands(dtype, D, inv_freq, q_norm, k_norm)
     if q_out is None:
-        _need(T <= 1 or pitch >= width, "rows that are written in place must not overlap")
+        if T > 1 and pitch < width:
+            raise ValueError("rows that are written in place must not overlap")
         q_out = qkv
     elif not (q_out.dim() == 2 and q_out.shape[0] == T and q_out.shape[1] >= Hq * D and q_out.stride(1) == 1 and q_out.dtype == dtype and (T <= 1 or q_out.stride(0) >= Hq * D)):
         raise ValueError("q_out has to be [%d, %d] of the type of qkv" % (T, Hq * D))
