@@ -6,7 +6,7 @@
 // order that the MMA reads, and one TMA box of tokens; rows behind the last token and columns behind K come as zeros. Weights are fetched before
 // the kernel that wrote the tokens has finished. The partial sums are integers: they go to shared memory as [token][channel], every CTA of the cluster
 // adds up its share of the tokens over all partials and finishes them, lanes along the channels.
-#include <mutex>
+#include <atomic>
 #include <type_traits>
 
 #include "gemm_i8.cuh"
@@ -363,14 +363,12 @@ __global__ void __launch_bounds__(256) pack_i8_kernel(const uint8_t* __restrict_
 
 template <bool F16, bool FUSED, int FORM>
 static int launch_i8_tile(const cudaLaunchConfig_t& cfg, const CUtensorMap& tm, const I8TileParams& p) {
-    static std::mutex mu;
-    static bool known[64] = {false};
+    static std::atomic<bool> known[64];
     int dev = 0;
     OVB_CHECK_CUDA(cudaGetDevice(&dev));
-    {
-        std::lock_guard<std::mutex> lk(mu);
-        if (!known[dev & 63]) OVB_CHECK_CUDA(cudaFuncSetAttribute(gemm_i8_tile_kernel<F16, FUSED, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
-        known[dev & 63] = true;
+    if (!known[dev & 63].load(std::memory_order_acquire)) {          // (twice at the same time does no harm)
+        OVB_CHECK_CUDA(cudaFuncSetAttribute(gemm_i8_tile_kernel<F16, FUSED, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
+        known[dev & 63].store(true, std::memory_order_release);
     }
     OVB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, gemm_i8_tile_kernel<F16, FUSED, FORM>, tm, p));
     return 0;
@@ -415,6 +413,7 @@ static bool i8_plan(int T, int N, int KB, bool fused, I8Plan* plan) {
     double best_us = fused ? 1e30 : 7.044 + pair_waves * KB * 0.3226 + (pair_waves - 1) * 5.848;
     const double bytes_us = 1.314 + (double)N * KB * 128 / 6.4e6;
     static constexpr int heights[6] = {16, 32, 64, 128, 256, 0};
+    int held[9] = {0, 148, 0, 0, 0, 0, 0, 0, 0};        // CTAs or clusters that the device holds, asked for where a candidate needs it
     for (int i = 0; i < 6; ++i) {
         const int bt = heights[i] ? heights[i] : t16;
         if (bt > t16 || (heights[i] == t16 && i < 5)) continue;          // (the last one is t16 itself)
@@ -427,7 +426,8 @@ static bool i8_plan(int T, int N, int KB, bool fused, I8Plan* plan) {
             for (int S = 1; S <= 8 && S <= KB; S *= 2) {
                 if (S > 1 && tiles * S > 444) break;
                 if (fused && ceil_div(KB, S) * kI8FusedBlock + 3 * kI8TileBytes > room * 1024) continue;      // the row's codes stay in shared memory
-                const int64_t slots = (int64_t)(S == 1 ? 148 : cluster_capacity(S)) * per_sm;
+                if (held[S] == 0) held[S] = cluster_capacity(S);
+                const int64_t slots = (int64_t)held[S] * per_sm;
                 const double waves = (double)((tiles + slots - 1) / slots);
                 const double share = tiles * S <= 148 ? 1 : per_sm;
                 const double issue = 0.1886 * share, bytes = 0.005616 * (16 + bt / 8.0) * share, latency = 1.649 / stages;

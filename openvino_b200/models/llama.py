@@ -25,6 +25,8 @@ def random_float_state(cfg: LlmConfig, seed: int = 0, device="cpu", std: float =
         st[p + "k_proj"] = rn(cfg.num_kv_heads * D, H)
         st[p + "v_proj"] = rn(cfg.num_kv_heads * D, H)
         st[p + "o_proj"] = rn(H, cfg.num_heads * D)
+        if cfg.qk_norm:
+            st[p + "q_norm"], st[p + "k_norm"] = 1.0 + 5 * rn(D), 1.0 + 5 * rn(D)
         if cfg.num_experts:
             st[p + "router"] = rn(cfg.num_experts, H) * 10.0     # spread the routing logits so that the top-k is well separated
             for e in range(cfg.num_experts):
@@ -50,10 +52,11 @@ def effective_state(cfg: LlmConfig, state: Dict[str, torch.Tensor], scale_dtype:
                 q, s, z = quant.quantize_u4_asym(v, cfg.group_size)
                 out[k] = quant.dequantize_u4(q, s.to(scale_dtype), z, cfg.group_size)
             elif cfg.weight_format == "int8":
-                q, s, z = quant.quantize_u8_asym(v, cfg.group_size)
-                s = s.to(scale_dtype)
                 N, Kd = v.shape
-                out[k] = ((q.float().reshape(N, -1, cfg.group_size) - z.float().unsqueeze(-1)) * s.float().unsqueeze(-1)).reshape(N, Kd)
+                g = cfg.group_size or Kd
+                q, s, z = quant.quantize_u8_asym(v, g)
+                s = s.to(scale_dtype)
+                out[k] = ((q.float().reshape(N, -1, g) - z.float().unsqueeze(-1)) * s.float().unsqueeze(-1)).reshape(N, Kd)
             else:
                 out[k] = v.to(torch.bfloat16).float()
         else:
@@ -65,13 +68,19 @@ def _rms(x, g, eps):
     return x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + eps) * g
 
 
-def _rope(x, pos, theta):
-    T, Hh, D = x.shape
-    inv = theta ** (-torch.arange(0, D, 2, device=x.device, dtype=torch.float32) / D)
+def _rope(x, pos, cfg):
+    """x [T, heads, D]: the first ``rotary_dim`` dimensions turn."""
+    inv = torch.tensor(cfg.inv_freq(), device=x.device, dtype=torch.float32)
+    rot = 2 * inv.numel()
     ang = pos.float()[:, None] * inv[None, :]
     cos, sin = ang.cos()[:, None, :], ang.sin()[:, None, :]
-    x1, x2 = x[..., : D // 2], x[..., D // 2:]
-    return torch.cat([x1 * cos - x2 * sin, x2 * cos + x1 * sin], dim=-1)
+    if cfg.rope_interleaved:
+        x1, x2 = x[..., 0:rot:2], x[..., 1:rot:2]
+        turned = torch.stack([x1 * cos - x2 * sin, x2 * cos + x1 * sin], dim=-1).flatten(-2)
+    else:
+        x1, x2 = x[..., : rot // 2], x[..., rot // 2:rot]
+        turned = torch.cat([x1 * cos - x2 * sin, x2 * cos + x1 * sin], dim=-1)
+    return torch.cat([turned, x[..., rot:]], dim=-1)
 
 
 @torch.no_grad()
@@ -87,8 +96,11 @@ def reference_logits(cfg: LlmConfig, state: Dict[str, torch.Tensor], ids: torch.
     for l in range(cfg.num_layers):
         p = "layers.%d." % l
         x = _rms(h, state[p + "input_layernorm"], cfg.rms_eps)
-        q = _rope((x @ state[p + "q_proj"].t()).reshape(S, Hq, D), pos, cfg.rope_theta)
-        k = _rope((x @ state[p + "k_proj"].t()).reshape(S, Hkv, D), pos, cfg.rope_theta)
+        q = (x @ state[p + "q_proj"].t()).reshape(S, Hq, D)
+        k = (x @ state[p + "k_proj"].t()).reshape(S, Hkv, D)
+        if cfg.qk_norm:
+            q, k = (_rms(t, state[p + n], cfg.qk_norm_eps or cfg.rms_eps) for t, n in ((q, "q_norm"), (k, "k_norm")))
+        q, k = _rope(q, pos, cfg), _rope(k, pos, cfg)
         v = (x @ state[p + "v_proj"].t()).reshape(S, Hkv, D)
         k = k.repeat_interleave(Hq // Hkv, dim=1)
         v = v.repeat_interleave(Hq // Hkv, dim=1)

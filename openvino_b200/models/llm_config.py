@@ -23,8 +23,23 @@ class LlmConfig:
     num_experts: int = 0          # 0 = dense FFN
     experts_top_k: int = 2
     weight_format: str = "int4"   # "int4" (u4 asym, group scales + zero points) | "int8" | "bf16" | "fp8"
-    group_size: int = 128
+    group_size: int = 128         # weights that share a scale; 0: the whole row of a weight
     sliding_window: int = 0
+    int8_activations: bool = False                          # int8 weights of whole rows are multiplied in whole numbers with rows quantised one by one
+    qk_norm: bool = False         # RMS norm of every query / key head before the rotation
+    qk_norm_eps: float = 0.0      # 0: rms_eps
+    rotary_dim: int = 0           # dimensions of a head that the position rotates; 0: all
+    rope_interleaved: bool = False                          # dimension pairs (2 i, 2 i + 1) instead of (i, i + rotary_dim / 2)
+    rope_inv_freq: Optional[Tuple[float, ...]] = None       # frequencies one by one (scaled tables); None: powers of rope_theta
+
+    def inv_freq(self) -> List[float]:
+        rot = self.rotary_dim or self.head_dim
+        return list(self.rope_inv_freq) if self.rope_inv_freq is not None else [self.rope_theta ** (-2.0 * i / rot) for i in range(rot // 2)]
+
+    @property
+    def plain_rotation(self) -> bool:
+        """Whole heads turn by powers of one base, halves paired, without head norms: what the step of one native call takes."""
+        return not (self.qk_norm or self.rope_interleaved or self.rope_inv_freq is not None or self.rotary_dim not in (0, self.head_dim))
 
     @property
     def q_size(self) -> int:

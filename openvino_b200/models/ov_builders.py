@@ -40,7 +40,7 @@ def _linear_weight(name: str, w: torch.Tensor, cfg: LlmConfig, compress: Optiona
     N, Kd = w.shape
     if not isinstance(w, torch.Tensor):         # a placeholder of build_llama_random_int4: draw the compressed constants directly
         return _random_compressed_weight(name, N, Kd, cfg, _linear_weight.rng)
-    g = cfg.group_size
+    g = cfg.group_size or Kd
     G = Kd // g
     if compress == "int4":
         q, s, z = quant.quantize_u4_asym(w.float(), g)            # q [N, K] uint8 values 0..15, s/z [N, G]
@@ -121,7 +121,11 @@ def _rms(x: Output, gamma: np.ndarray, eps: float, name: str) -> Output:
 
 
 def _rope(x: Output, cos: Output, sin: Output, D: int) -> Output:
-    """x [B, H, L, D]; cos/sin [B, 1, L, D]: x * cos + rotate_half(x) * sin."""
+    """x [B, H, L, S]; cos/sin [B, 1, L, D]: x * cos + rotate_half(x) * sin over the first D of S dimensions."""
+    S = x.get_partial_shape()[3].get_length()
+    if D < S:
+        turned = _rope(ops.slice(x, _i64([0]), _i64([D]), _i64([1]), _i64([3])).output(0), cos, sin, D)
+        return ops.concat([turned, ops.slice(x, _i64([D]), _i64([S]), _i64([1]), _i64([3])).output(0)], 3).output(0)
     lo = ops.slice(x, _i64([0]), _i64([D // 2]), _i64([1]), _i64([3]))
     hi = ops.slice(x, _i64([D // 2]), _i64([D]), _i64([1]), _i64([3]))
     rot = ops.concat([ops.negative(hi).output(0), lo.output(0)], 3)
@@ -146,7 +150,12 @@ def build_llama(cfg: LlmConfig, state: Dict[str, torch.Tensor], compress: Option
     h = ops.gather(embed, input_ids, _i64(0), name="embed").output(0)             # [B, L, H]
 
     # rotary tables from position ids: [B, L] -> cos/sin [B, 1, L, D]
-    inv_freq = (cfg.rope_theta ** (-np.arange(0, D, 2, dtype=np.float32) / D)).astype(np.float32)
+    if cfg.rope_interleaved:
+        raise ValueError("the builder writes the half-rotate form")
+    rot = cfg.rotary_dim or D
+    inv_freq = (cfg.rope_theta ** (-np.arange(0, rot, 2, dtype=np.float32) / rot)).astype(np.float32)
+    if cfg.rope_inv_freq is not None:
+        inv_freq = np.array(cfg.rope_inv_freq, dtype=np.float32)
     pos = ops.convert(ops.unsqueeze(position_ids, _i64([2])), "f32")               # [B, L, 1]
     ang = ops.multiply(pos, constant(inv_freq.reshape(1, 1, -1)))                  # [B, L, D/2]
     ang = ops.concat([ang.output(0), ang.output(0)], 2)
@@ -178,12 +187,14 @@ def build_llama(cfg: LlmConfig, state: Dict[str, torch.Tensor], compress: Option
         def proj(name, inp, key):
             return ops.matmul(inp, _linear_weight(n + name + ".weight", state[p + key], cfg, compress), False, True, name=n + name).output(0)
 
-        def heads(t: Output, nh: int) -> Output:   # [B, L, nh*D] -> [B, nh, L, D]
+        def heads(t: Output, nh: int, norm: Optional[str] = None) -> Output:   # [B, L, nh*D] -> [B, nh, L, D]
             r = ops.reshape(t, _i64([0, 0, nh, D]), True)
+            if norm is not None and cfg.qk_norm:
+                r = _rms(r.output(0), _f32(state[p + norm]), cfg.qk_norm_eps or cfg.rms_eps, n + "self_attn." + norm)
             return ops.transpose(r, _i64([0, 2, 1, 3])).output(0)
 
-        q = _rope(heads(proj("self_attn.q_proj", x, "q_proj"), Hq), cos, sin, D)
-        k = _rope(heads(proj("self_attn.k_proj", x, "k_proj"), Hkv), cos, sin, D)
+        q = _rope(heads(proj("self_attn.q_proj", x, "q_proj"), Hq, "q_norm"), cos, sin, rot)
+        k = _rope(heads(proj("self_attn.k_proj", x, "k_proj"), Hkv, "k_norm"), cos, sin, rot)
         v = heads(proj("self_attn.v_proj", x, "v_proj"), Hkv)
 
         if stateful:

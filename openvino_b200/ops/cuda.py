@@ -425,9 +425,6 @@ def _call(fn, packed: bytes, device: int, what: str) -> None:
         _check(rc, what)
 
 
-_HALVES = (torch.bfloat16, torch.float16)
-
-
 class QuantizedRows:
     """Rows as signed bytes with one scale each: value = ``q`` * ``scales``. ``sums`` are the sums of the codes, ``dtype`` the 16-bit type that the rows had
     (products of them have it again). The row pitch of ``q`` is a multiple of 16."""
@@ -505,7 +502,7 @@ def _gemm_i8(x, w: "PackedWeight", out, residual, act, out_f32, glu, cap, norm) 
     kind = torch.float32 if out_f32 else dtype
     d = _one_device(like, wt, gamma, idx, out, residual)
     if out is None:
-        out = like.new_empty((T, cols), dtype=kind)
+        out = like.new_empty((T, cols)) if like.dtype == kind else like.new_empty((T, cols), dtype=kind)
         ldo = cols
     else:
         ldo = _result_pitch("out", out, kind, T, cols)
@@ -517,7 +514,7 @@ def _gemm_i8(x, w: "PackedWeight", out, residual, act, out_f32, glu, cap, norm) 
     else:
         # the quantised rows, their scales and sums: memory of the caching allocator, which belongs to the stream
         pitch = (Kd + 15) // 16 * 16
-        rows = x.new_empty(T * (pitch + 8), dtype=torch.uint8)
+        rows = x.new_empty(T * (pitch // 2 + 4))
         q, raw, ld_raw = rows.data_ptr(), x.data_ptr(), x.stride(0)
         scales = q + T * pitch
         sums = scales + 4 * T
@@ -1098,14 +1095,15 @@ def rope_kv_write_u8(qkv, positions, slot_map, k_cache, v_cache, k_meta, v_meta,
 
 def _rope_operands(dtype, D, inv_freq, q_norm, k_norm) -> int:
     """Checks what both forms share; the dimensions that turn."""
-    if dtype not in _HALVES:
+    if dtype != torch.bfloat16 and dtype != torch.float16:
         raise ValueError("bf16 or fp16 heads are expected, not %s" % dtype)
     rot = 2 * inv_freq.numel()
     if inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous() or rot > D:
         raise ValueError("frequencies are fp32, one for each pair of at most %d dimensions" % D)
-    for w in (q_norm, k_norm):
-        if w is not None and not (w.numel() == D and w.dtype == dtype and w.is_contiguous()):
-            raise ValueError("a head norm has %d weights of the heads' type" % D)
+    if q_norm is not None and not (q_norm.dtype == dtype and q_norm.numel() == D and q_norm.is_contiguous()):
+        raise ValueError("a head norm has %d weights of the heads' type" % D)
+    if k_norm is not None and not (k_norm.dtype == dtype and k_norm.numel() == D and k_norm.is_contiguous()):
+        raise ValueError("a head norm has %d weights of the heads' type" % D)
     return rot
 
 
@@ -1132,7 +1130,8 @@ def qk_norm_rope(q, k, positions, inv_freq, q_norm=None, k_norm=None, eps=1e-6, 
                             None if k_out is None else k_out[None])
         return outs[0][0], outs[1][0]
     dtype = q.dtype
-    _need(q.dim() == 4 and k.dim() == 4 and k.dtype == dtype, "queries [B, S, Hq, D] and keys [B, S, Hkv, D] of one type are expected")
+    if q.dim() != 4 or k.dim() != 4 or k.dtype != dtype:
+        raise ValueError("queries [B, S, Hq, D] and keys [B, S, Hkv, D] of one type are expected")
     (B, S, Hq, D), (kB, kS, Hkv, kD) = q.shape, k.shape
     if not (kB == B and kS == S and kD == D and Hq > 0 and Hkv > 0 and D > 0):
         raise ValueError("queries [B, S, Hq, D] and keys [B, S, Hkv, D] are expected, not %s and %s" % (tuple(q.shape), tuple(k.shape)))

@@ -32,6 +32,9 @@ class LayerWeights:
     norm2: torch.Tensor
     gate_up: Optional[K.PackedWeight] = None
     down: Optional[K.PackedWeight] = None
+    # weights [D] of the norms of query and key heads
+    q_norm: Optional[torch.Tensor] = None
+    k_norm: Optional[torch.Tensor] = None
     # MoE: router [E, H]; gate_up / down hold the rank's local experts stacked ([nloc * 2F, H] and [H, nloc * F])
     router: Optional[K.PackedWeight] = None
 
@@ -53,12 +56,21 @@ class LlmWeights:
             q, s, z = quant.quantize_u4_asym(w, cfg.group_size)
             return K.PackedWeight.from_ir_u4(quant.pack_u4(q), s, quant.pack_u4(z), N, Kd, cfg.group_size)
         if cfg.weight_format == "int8":
-            q, s, z = quant.quantize_u8_asym(w, cfg.group_size)
-            return K.PackedWeight.from_ir_u8(q, s, z, N, Kd, cfg.group_size)
+            return LlmWeights._pack_int8(w, cfg)
         if cfg.weight_format == "fp8" and Kd % 128 == 0:
             q, s = quant.quantize_f8_block(w, 128)
             return K.PackedWeight.from_f8_block(q, s, N, Kd, 128)
         return K.PackedWeight.from_dense(w.to(torch.bfloat16))
+
+    @staticmethod
+    def _pack_int8(w: torch.Tensor, cfg: LlmConfig) -> K.PackedWeight:
+        N, Kd = w.shape
+        if cfg.int8_activations:                # one scale per row: products of whole numbers
+            q, s, z = quant.quantize_u8_asym(w, Kd)
+            return K.PackedWeight.from_ir_i8(q, s, z)
+        g = cfg.group_size or Kd
+        q, s, z = quant.quantize_u8_asym(w, g)
+        return K.PackedWeight.from_ir_u8(q, s, z, N, Kd, g)
 
     @staticmethod
     def _random_packed(N: int, Kd: int, cfg: LlmConfig, device, seed: int) -> K.PackedWeight:
@@ -76,8 +88,7 @@ class LlmWeights:
             return K.PackedWeight.from_f8_block(w8, scales, N, Kd, 128)
         w = (torch.randn((N, Kd), device=device, generator=g, dtype=torch.float32) * 0.02)
         if cfg.weight_format == "int8":
-            q, s, z = quant.quantize_u8_asym(w, cfg.group_size)
-            return K.PackedWeight.from_ir_u8(q, s, z, N, Kd, cfg.group_size)
+            return LlmWeights._pack_int8(w, cfg)
         return K.PackedWeight.from_dense(w.to(torch.bfloat16))
 
     @staticmethod
@@ -101,6 +112,8 @@ class LlmWeights:
                 qkv=LlmWeights._random_packed((hq + 2 * hkv) * D, H, cfg, device, s + 1),
                 o=LlmWeights._random_packed(H, hq * D, cfg, device, s + 2),
                 norm2=ones())
+            if cfg.qk_norm:
+                lw.q_norm, lw.k_norm = (torch.ones(D, device=device, dtype=torch.bfloat16) for _ in range(2))
             if cfg.num_experts == 0:
                 lw.gate_up = LlmWeights._random_packed(2 * ffn, H, cfg, device, s + 3)
                 lw.gate_up.swiglu = ffn % 64 == 0 and lw.gate_up.bias is None     # random rows: any row order is a valid interleaving
@@ -157,6 +170,8 @@ class LlmWeights:
                 gate_up=LlmWeights._pack(dev(torch.cat([gate, up], 0)).contiguous(), cfg),
                 down=LlmWeights._pack(dev(down).contiguous(), cfg)))
             layers[-1].gate_up.swiglu = fused_gate
+            if cfg.qk_norm:
+                layers[-1].q_norm, layers[-1].k_norm = (dev(state[p + n]).to(torch.bfloat16).contiguous() for n in ("q_norm", "k_norm"))
         vshard = cfg.vocab_size // tp_size
         lm = state["lm_head"][r * vshard:(r + 1) * vshard]
         return LlmWeights(dev(state["embed_tokens"]).to(torch.bfloat16), layers, dev(state["norm"]).to(torch.bfloat16),
@@ -407,6 +422,11 @@ class CudaLlmExecutor(LlmExecutor):
         max_blocks_per_seq = self.max_blocks_per_seq
         self.hq = cfg.num_heads // self.tp_size
         self.hkv = cfg.num_kv_heads // self.tp_size
+        self.int8 = any(p is not None and p.mode == K.W_I8 for lw in weights.layers for p in (lw.qkv, lw.o, lw.gate_up, lw.down)) or weights.lm_head.mode == K.W_I8
+        if self.int8 and self.tp_size > 1:
+            raise ValueError("products of whole numbers are not summed over tensor-parallel ranks: compile the model without DYNAMIC_QUANTIZATION_GROUP_SIZE")
+        # frequencies of the rotation, for the models that the rotation of whole heads by powers of one base does not serve
+        self.inv_freq = None if cfg.plain_rotation else torch.tensor(cfg.inv_freq(), dtype=torch.float32, device=self.device)
         # KV_CACHE_PRECISION = u8: rows are stored as bytes with one fp16 (scale, zero point) pair per (block, head, slot):
         # half the cache memory and half the decode traffic of the 16-bit cache
         self.k_cache = [torch.zeros((num_kv_blocks, self.hkv, block_size, cfg.head_dim), dtype=torch.uint8 if self.kv_u8 else torch.bfloat16,
@@ -430,7 +450,7 @@ class CudaLlmExecutor(LlmExecutor):
         self._expert_windows = {}
 
     def _is_native(self) -> bool:
-        return self.tp_size == 1 and not self.cfg.num_experts and all(p.mode != K.W_F32 for lw in self.w.layers for p in (lw.qkv, lw.o, lw.gate_up, lw.down))
+        return self.tp_size == 1 and not self.cfg.num_experts and not self.int8 and self.inv_freq is None and all(p.mode != K.W_F32 for lw in self.w.layers for p in (lw.qkv, lw.o, lw.gate_up, lw.down))
 
     # -- one forward pass over the buffers of `sb`
     def _forward(self, sb: StepBuffers, shp: StepShape) -> None:
@@ -449,9 +469,11 @@ class CudaLlmExecutor(LlmExecutor):
         K.resolve_ids(ids, sb.view("tok_src")[:T], self.last_token)
         K.embedding(ids, w.embed, out=h)
         for l, lw in enumerate(w.layers):
-            K.rmsnorm(h, lw.norm1, cfg.rms_eps, out=x)
-            K.gemm(x, lw.qkv, out=qkv, ws=ws)
-            if self.kv_u8:
+            self._normed(h, lw.norm1, x, lw.qkv, qkv)
+            if self.inv_freq is not None:
+                K.qk_norm_rope_kv_write(qkv, positions, slot_map, self.k_cache[l], self.v_cache[l], self.inv_freq, self.hq, self.hkv, D, self.block_size,
+                                        lw.q_norm, lw.k_norm, cfg.qk_norm_eps or cfg.rms_eps, cfg.rope_interleaved, k_meta=self.k_meta[l], v_meta=self.v_meta[l])
+            elif self.kv_u8:
                 K.rope_kv_write_u8(qkv, positions, slot_map, self.k_cache[l], self.v_cache[l], self.k_meta[l], self.v_meta[l], self.hq, self.hkv, D,
                                    cfg.rope_theta, self.block_size)
             else:
@@ -463,8 +485,8 @@ class CudaLlmExecutor(LlmExecutor):
                               max_context_len=shp.max_ctx, max_q_len=shp.max_q_len, sliding_window=cfg.sliding_window,
                               block_size=self.block_size, out=attn, ws=ws, k_meta=self.k_meta[l], v_meta=self.v_meta[l])
             self._row_parallel(attn, lw.o, h, 2 * l)
-            K.rmsnorm(h, lw.norm2, cfg.rms_eps, out=x)
             if cfg.num_experts:
+                K.rmsnorm(h, lw.norm2, cfg.rms_eps, out=x)
                 # every rank holds all tokens (the residual stream is replicated), so "dispatch" is free: a rank runs its
                 # experts on the tokens routed to them (others contribute zeros) and the row-parallel down projection
                 # with its fused all-reduce is the "combine"
@@ -481,21 +503,35 @@ class CudaLlmExecutor(LlmExecutor):
                 K.moe_silu_mul_scale(gu, sb.route[:T], cfg.ffn_size, nloc, self.tp_rank * nloc, out=act)
                 n += 2
             elif getattr(lw.gate_up, "swiglu", False):
-                K.gemm(x, lw.gate_up, out=act, act=K.ACT_SWIGLU, ws=ws)       # silu(gate) * up in the GEMM epilogue
+                self._normed(h, lw.norm2, x, lw.gate_up, act, K.ACT_SWIGLU)    # silu(gate) * up in the GEMM epilogue
                 n -= 1
             else:
-                K.gemm(x, lw.gate_up, out=gu, ws=ws)
+                self._normed(h, lw.norm2, x, lw.gate_up, gu)
                 K.silu_mul(gu, out=act)
             self._row_parallel(act, lw.down, h, 2 * l + 1)
             n += 9
         # logits only for the last token of every sequence
         last_h, last_x = sb.last_h[:B], sb.last_x[:B]
-        K.embedding(sb.view("logit_idx")[:B], h, out=last_h)
-        K.rmsnorm(last_h, w.final_norm, cfg.rms_eps, out=last_x)
         logits = sb.logits[:B]
-        K.gemm(last_x, w.lm_head, out=logits, ws=ws)
+        if w.lm_head.mode == K.W_I8:
+            K.gemm(h, w.lm_head, out=logits, norm=(w.final_norm, cfg.rms_eps, sb.view("logit_idx")[:B]))
+        else:
+            K.embedding(sb.view("logit_idx")[:B], h, out=last_h)
+            K.rmsnorm(last_h, w.final_norm, cfg.rms_eps, out=last_x)
+            K.gemm(last_x, w.lm_head, out=logits, ws=ws)
         self._sample(sb, B)
+        # with products of whole numbers: rows are quantised with their norm in one launch (the output and down projections need one more each); a single
+        # token's rows in none
+        n += 0 if not self.int8 else (2 if T > 1 else -2) * cfg.num_layers - 1 - (B == 1)
         self.kernel_launches += n + 5
+
+    def _normed(self, h: torch.Tensor, norm: torch.Tensor, x: torch.Tensor, wt: K.PackedWeight, out: torch.Tensor, act: int = K.ACT_NONE) -> None:
+        """The product of the normed rows of ``h``; ``x``: room for them where the product does not norm them itself."""
+        if wt.mode == K.W_I8:
+            K.gemm(h, wt, out=out, act=act, norm=(norm, self.cfg.rms_eps))
+        else:
+            K.rmsnorm(h, norm, self.cfg.rms_eps, out=x)
+            K.gemm(x, wt, out=out, act=act, ws=self.ws)
 
     def _forward_native(self, sb: StepBuffers, shp: StepShape) -> None:
         """The pass of a dense model on one GPU as one call into the kernel library, with the results of `_forward` up to the order of 32-bit sums. It takes

@@ -33,6 +33,7 @@ from .._tensor import Tensor, torch_dtype
 from .._types import Type
 from ..ops import generic as G
 from .plugin_config import ConfigOption, OptionVisibility, PluginConfig
+from .llm_import import quantizes_rows
 from .core import CompiledModel, InferRequest, Plugin, ProfilingInfo, VariableState
 
 _FLOAT = ("f32", "f16", "bf16", "f64")
@@ -47,8 +48,9 @@ def _tdtype(t: Type, precision: Optional[torch.dtype]) -> torch.dtype:
 class Ctx:
     """What an operation implementation may use: the device, the compute precision, the kernel library."""
 
-    def __init__(self, device: torch.device, precision: Optional[torch.dtype]):
+    def __init__(self, device: torch.device, precision: Optional[torch.dtype], dynamic_quantization: int = 0):
         self.device, self.precision = device, precision
+        self.dynamic_quantization = dynamic_quantization        # DYNAMIC_QUANTIZATION_GROUP_SIZE
         self.on_gpu = device.type == "cuda"
         self.K = None
         if self.on_gpu:
@@ -80,7 +82,7 @@ def _npuw_function_call(n, ins, ctx):
     key = (str(ctx.device), ctx.precision)
     prog = progs.get(key)
     if prog is None:
-        prog = progs[key] = GraphProgram(f.body, ctx.device, ctx.precision)
+        prog = progs[key] = GraphProgram(f.body, ctx.device, ctx.precision, dynamic_quantization=ctx.dynamic_quantization)
         f.compiles += 1
     f.calls += 1
     prog.ctx.variables = ctx.variables
@@ -907,7 +909,16 @@ def _prepare_fc(n: Node, ins, ctx: Ctx):
             Kd = int(np.prod(wt.shape[1:]))
             scales = torch.from_numpy(np.ascontiguousarray(sc_node.get_tensor_view().to_float32())).reshape(N, -1)
             G = scales.shape[1]
-            if et in ("u4", "u8") and Kd % 64 == 0 and (Kd // G) % 64 == 0:
+            if et in ("u8", "i8") and G == 1 and Kd <= 65536 and ins[0].dtype in (torch.float16, torch.bfloat16) and quantizes_rows(ctx.dynamic_quantization, Kd):
+                # products of whole numbers: a scale per channel, rows of activations quantised one by one
+                np_type, t_type = (np.uint8, torch.uint8) if et == "u8" else (np.int8, torch.int8)
+                wq = torch.from_numpy(np.ascontiguousarray(wt.data).reshape(N, Kd).view(np_type).copy()).to(ctx.device)
+                zp = torch.zeros(1) if et == "i8" else torch.full((1,), 128.0)
+                if zp_node is not None and zp_node.get_type_name() == "Constant" and zp_node.get_tensor_view().size > 0:
+                    zp = torch.from_numpy(np.ascontiguousarray(zp_node.get_tensor_view().to_float32())).reshape(-1)
+                zp = (zp.expand(N) if zp.numel() == 1 else zp.reshape(N)).to(t_type).to(ctx.device)
+                st["packed"] = K.PackedWeight.from_ir_i8(wq, scales.reshape(-1).to(ctx.device), zp, bias=bias.to(ctx.device, ins[0].dtype) if bias is not None and bias.numel() == N else None)
+            elif et in ("u4", "u8") and Kd % 64 == 0 and (Kd // G) % 64 == 0:
                 dev = ctx.device
                 wq = torch.from_numpy(np.ascontiguousarray(wt.data).reshape(-1).view(np.uint8).copy()).to(dev)
                 zp = None
@@ -950,7 +961,7 @@ def _fc(n, ins, ctx):
     st = _prepare_fc(n, ins, ctx)
     pw = st["packed"]
     has_bias = len(ins) > 2 and ins[2].numel() > 0 and ins[2].dim() > 0
-    if pw is not None and x.dtype in (torch.float16, torch.bfloat16) and (pw.mode != ctx.K.W_F16) == (x.dtype == torch.bfloat16):
+    if pw is not None and x.dtype in (torch.float16, torch.bfloat16) and (pw.mode == ctx.K.W_I8 or (pw.mode != ctx.K.W_F16) == (x.dtype == torch.bfloat16)):
         x2 = x.reshape(-1, x.shape[-1])
         if not x2.is_contiguous():
             x2 = _dense(x2)
@@ -1410,10 +1421,10 @@ def supported_op_types() -> List[str]:
 class GraphProgram:
     """A compiled graph: operations in execution order with their implementations and input wiring."""
 
-    def __init__(self, model: Model, device, precision: Optional[torch.dtype] = None, host_fallback: bool = True):
+    def __init__(self, model: Model, device, precision: Optional[torch.dtype] = None, host_fallback: bool = True, dynamic_quantization: int = 0):
         self.model = model
         self.device = torch.device(device)
-        self.ctx = Ctx(self.device, precision)
+        self.ctx = Ctx(self.device, precision, dynamic_quantization)
         self.precision = precision
         self.params = model.get_parameters()
         self.results = model.get_results()
@@ -1556,7 +1567,7 @@ class CudaCompiledModel(CompiledModel):
     def __init__(self, plugin, model, config, runtime_model, device: torch.device, precision):
         super().__init__(plugin, model, config, runtime_model)
         self.device, self.precision = device, precision
-        self.program = GraphProgram(runtime_model, device, precision)
+        self.program = GraphProgram(runtime_model, device, precision, dynamic_quantization=int(config.get(props.hint.dynamic_quantization_group_size, 0) or 0))
         self._out_types = [o.get_element_type() for o in model.outputs]
         # one stream per compiled-model stream: requests of different streams overlap on the GPU
         self._streams = [torch.cuda.Stream(device=device) for _ in range(self._n_streams)] if device.type == "cuda" else [None]
@@ -1782,6 +1793,8 @@ class CudaConfig(PluginConfig):
                                    lambda v: all(p in ("", "TENSOR_PARALLEL", "PIPELINE_PARALLEL") for p in str(v).replace(" ", "").split(",")), R))
         self.register(ConfigOption(props.hint.kv_cache_precision, "bf16", "element type of the paged KV cache: bf16 | f16 | u8",
                                    lambda v: str(v).lower() in ("bf16", "f16", "u8", "dynamic"), R))
+        self.register(ConfigOption(props.hint.dynamic_quantization_group_size, 0, "activations that share a scale in products with 8-bit weights of one scale per channel, "
+                                   "which then run in whole numbers: 0 = off, -1 or a size that covers the row = one scale per row", lambda v: v >= -1, R))
         self.register(ConfigOption(props.cuda.use_cuda_graphs, True, "capture decode steps of the serving program in CUDA graphs", None, R))
         self.register(ConfigOption(props.cuda.serving_program, False, "compile a decoder-only LLM graph into the serving program", None, R))
         self.register(ConfigOption(props.cuda.tensor_parallel_size, 0, "ranks of the tensor-parallel group (0 = the process group's size)", lambda v: 0 <= v <= 8, R))
@@ -1813,6 +1826,9 @@ class CudaServingCompiledModel(CompiledModel):
         from . import llm_import
         self.device = device
         self.llm_config, self._parts = llm_import.analyze(model)
+        rows = [v for v in list(self._parts["lin"].values()) + [self._parts["lm_head"]] if v.whole_rows]
+        if rows and llm_import.quantizes_rows(config.get(props.hint.dynamic_quantization_group_size, 0), max(v.K for v in rows)):
+            self.llm_config = self.llm_config.with_(int8_activations=True)
         policy = str(config.get(props.hint.model_distribution_policy, "") or "")
         self.tp_rank, self.tp_size = 0, 1
         if "TENSOR_PARALLEL" in policy and torch.distributed.is_available() and torch.distributed.is_initialized():
@@ -1868,7 +1884,7 @@ class CudaPlugin(Plugin):
     def supported_properties(self):
         return super().supported_properties() + [props.cuda.use_cuda_graphs, props.cuda.tensor_parallel_size, props.cuda.serving_program, props.device.uuid,
                                                  props.device.architecture, props.device.type, props.optimal_batch_size,
-                                                 props.hint.kv_cache_precision, props.hint.model_distribution_policy]
+                                                 props.hint.kv_cache_precision, props.hint.model_distribution_policy, props.hint.dynamic_quantization_group_size]
 
     def default_config(self):
         d = super().default_config()

@@ -112,8 +112,16 @@ class _Linear:
             o.w = o.w[order]
         return o
 
-    def pack(self, device):
+    @property
+    def whole_rows(self) -> bool:
+        """One scale per row of 8-bit weights: what products of whole numbers take."""
+        return self.compressed and self.kind == "u8" and self.G == 1 and self.K <= 65536
+
+    def pack(self, device, int8: bool = False):
+        """``int8``: for products of whole numbers with quantised rows."""
         from ..ops import cuda as K
+        if int8 and self.whole_rows:
+            return K.PackedWeight.from_ir_i8(self.q.contiguous().to(device), self.scales.reshape(-1).to(device), self.zp.reshape(-1).contiguous().to(device))
         if not self.compressed:
             return K.PackedWeight.from_dense(self.w.to(device).to(torch.bfloat16).contiguous())
         g = self.K // self.G
@@ -129,9 +137,11 @@ _FC = ("FullyConnected", "FullyConnectedCompressed")
 _DEAD_ENDS = ("Parameter", "Constant", "ReadValue", "Result", "Assign")
 
 
-def _nearest_fc_ancestor(out_port) -> Optional[Node]:
+def _nearest_fc_ancestor(out_port, head_size: int = 0, found: Optional[Dict] = None) -> Optional[Node]:
     """Closest FullyConnected node that feeds ``out_port`` (breadth first over all data inputs; shape plumbing, RoPE, the
-    KV-state Concat and the grouped-query broadcast are walked through, parameters / constants / states end a path)."""
+    KV-state Concat and the grouped-query broadcast are walked through, parameters / constants / states end a path). With ``head_size`` the
+    path may also pass the RMS norm of heads of that size; ``found`` collects it and the RoPE node that were passed, the first of each kind."""
+    found = {} if found is None else found
     seen, frontier = set(), [out_port.get_node()]
     while frontier:
         nxt = []
@@ -142,8 +152,15 @@ def _nearest_fc_ancestor(out_port) -> Optional[Node]:
             t = n.get_type_name()
             if t in _FC:
                 return n
+            if t == "RMS" and head_size and "norm" not in found and n.input_value(1).get_partial_shape().is_static \
+                    and int(np.prod(list(n.input_value(1).get_shape()))) == head_size:
+                found["norm"] = n
+                nxt.append(n.input_value(0).get_node())
+                continue
             if t in _DEAD_ENDS or t in ("ScaledDotProductAttention", "PagedAttentionExtension", "RMS"):
                 continue
+            if t == "RoPE":
+                found.setdefault("rope", n)
             for i in range(n.get_input_size()):
                 nxt.append(n.input_value(i).get_node())
         frontier = nxt
@@ -179,6 +196,36 @@ def _one(nodes, what: str) -> Node:
     return nodes[0]
 
 
+def _frequencies(rope: Optional[Node], half: int) -> Optional[np.ndarray]:
+    """The table of ``half`` rotation frequencies behind the cosine input of a RoPE node."""
+    if rope is None:
+        return None
+    seen, frontier = set(), [rope.input_value(1).get_node()]
+    while frontier:
+        nxt = []
+        for n in frontier:
+            if n in seen:
+                continue
+            seen.add(n)
+            if n.get_type_name() == "Constant":
+                if n.get_output_element_type(0).is_real() and int(np.prod(n.get_output_shape(0) or [1])) == half:
+                    v = n.get_tensor_view().to_float32().reshape(-1).astype(np.float64)
+                    if np.isfinite(v).all() and (v > 0).all() and (np.diff(v) <= 0).all():
+                        return v
+                continue
+            nxt.extend(n.input_value(i).get_node() for i in range(n.get_input_size()))
+        frontier = nxt
+    return None
+
+
+def _head_size(att: Node) -> int:
+    """0 where the graph does not say."""
+    if att.get_type_name() == "ScaledDotProductAttention":
+        shape = att.input_value(0).get_partial_shape()
+        return shape[3].get_length() if shape.rank.is_static and len(shape) == 4 and shape[3].is_static else 0
+    return int(att.rt_info.get("k_head_size") or 0)
+
+
 def _gamma(rms: Node) -> torch.Tensor:
     g = rms.input_value(1).get_node()
     if g.get_type_name() == "Convert":
@@ -186,6 +233,13 @@ def _gamma(rms: Node) -> torch.Tensor:
     if g.get_type_name() != "Constant":
         raise NotAnLlm("the scale of %s is not a constant" % rms.get_friendly_name())
     return _const_f32(g).reshape(-1)
+
+
+def quantizes_rows(group_size, K: int) -> bool:
+    """Whether DYNAMIC_QUANTIZATION_GROUP_SIZE asks for one scale per row of ``K`` activations: 0 is off, -1 and sizes that reach over the row are on. Smaller
+    groups are not served: such products keep 16-bit activations."""
+    g = int(group_size or 0)
+    return g < 0 or g >= K > 0
 
 
 def analyze(model: Model) -> Tuple[LlmConfig, Dict]:
@@ -207,8 +261,17 @@ def analyze(model: Model) -> Tuple[LlmConfig, Dict]:
     experts: Dict[int, Dict] = {}
     eps = 1e-6
     last_add = first_norm = None
+    head_eps, rope = 0.0, None
     for l, a in enumerate(att):
-        q, k, v = (_nearest_fc_ancestor(a.input_value(i)) for i in range(3))
+        D = _head_size(a)
+        on_q: Dict = {}
+        on_k: Dict = {}
+        q, k, v = _nearest_fc_ancestor(a.input_value(0), D, on_q), _nearest_fc_ancestor(a.input_value(1), D, on_k), _nearest_fc_ancestor(a.input_value(2))
+        for key, on in (("q_norm", on_q), ("k_norm", on_k)):
+            if "norm" in on:
+                norms[(l, key)] = _gamma(on["norm"])
+                head_eps = float(on["norm"].get_attribute("epsilon"))
+        rope = rope or on_q.get("rope")
         if q is None or k is None or v is None:
             raise NotAnLlm("attention %d is not fed by three projections" % l)
         n1 = q.input_value(0).get_node()
@@ -302,12 +365,33 @@ def analyze(model: Model) -> Tuple[LlmConfig, Dict]:
                 if abs(float(v[0]) - 1.0) < 1e-6 and 0 < v[1] < 1:
                     theta = float(v[1]) ** (-D / 2.0)
                     break
+    # what the graph's RoPE nodes say beyond that: the rotated dimensions, their pairing, and frequencies that are not powers of one base
+    more = {}
+    if rope is not None:
+        at = rope.get_attributes()
+        rot = int(at.get("rotary_ndims") or D)
+        if rot != D:
+            more["rotary_dim"] = rot
+        if at.get("is_interleaved"):
+            more["rope_interleaved"] = True
+        v = _frequencies(rope, rot // 2)
+        if v is not None and rot >= 4:
+            base = (v[1] / v[0]) ** (-rot / 2.0)
+            if abs(v[0] - 1.0) > 1e-6 or np.abs(v * base ** (2.0 * np.arange(rot // 2) / rot) - 1.0).max() > 1e-3:
+                more["rope_inv_freq"] = tuple(float(f) for f in v)
+            elif rot != D:
+                theta = float(base)
+    normed = [key in norms for l in layers for key in ((l, "q_norm"), (l, "k_norm"))]
+    if any(normed):
+        if not all(normed):
+            raise NotAnLlm("head norms in a part of the layers, or of the queries or keys alone, are not served")
+        more.update(qk_norm=True, qk_norm_eps=head_eps)
     first = lin[(layers[0], "q_proj")]
     fmt = {"u4": "int4", "u8": "int8"}[first.kind] if first.compressed else "bf16"
     cfg = LlmConfig(name=model.get_friendly_name() or "llm", vocab_size=embed.shape[0], hidden_size=H, num_layers=len(layers), num_heads=Hq,
                     num_kv_heads=Hkv, head_dim=D, ffn_size=experts[0]["gate"].shape[1] if experts else lin[(layers[0], "gate_proj")].N,
                     rope_theta=theta, rms_eps=eps, weight_format=fmt, group_size=(first.K // first.G) if first.compressed else 128,
-                    num_experts=experts[0]["gate"].shape[0] if experts else 0, experts_top_k=experts[0]["top_k"] if experts else 0)
+                    num_experts=experts[0]["gate"].shape[0] if experts else 0, experts_top_k=experts[0]["top_k"] if experts else 0, **more)
     if experts and len(experts) != len(layers):
         raise NotAnLlm("dense and expert layers in one model are not served")
     # the sliding window of the paged form is an input of the attention operation (0 = none); ALiBi has no kernel yet
@@ -331,8 +415,12 @@ def build_weights(cfg: LlmConfig, parts: Dict, device, tp_rank: int = 0, tp_size
     r = tp_rank
     lin, norms = parts["lin"], parts["norms"]
     bf = lambda t: t.to(device).to(torch.bfloat16).contiguous()
+    int8 = cfg.int8_activations
+    if int8 and tp_size > 1:
+        raise NotAnLlm("products of whole numbers are not summed over tensor-parallel ranks: compile the model without DYNAMIC_QUANTIZATION_GROUP_SIZE")
     layers = []
     for l in parts["layers"]:
+        heads = dict(q_norm=bf(norms[(l, "q_norm")]), k_norm=bf(norms[(l, "k_norm")])) if cfg.qk_norm else {}
         q = lin[(l, "q_proj")].rows(r * hq * D, (r + 1) * hq * D)
         k = lin[(l, "k_proj")].rows(r * hkv * D, (r + 1) * hkv * D)
         v = lin[(l, "v_proj")].rows(r * hkv * D, (r + 1) * hkv * D)
@@ -346,19 +434,19 @@ def build_weights(cfg: LlmConfig, parts: Dict, device, tp_rank: int = 0, tp_size
             gu = torch.cat([torch.cat([ex["gate"][e], ex["up"][e]], 0) for e in local], 0)
             down = torch.cat([ex["down"][e] for e in local], 1)
             pack16 = lambda t: K.PackedWeight.from_dense(t.to(device).to(torch.bfloat16).contiguous())
-            layers.append(LayerWeights(norm1=bf(norms[(l, "input_layernorm")]), qkv=_Linear.stack([q, k, v]).pack(device),
-                                       o=lin[(l, "o_proj")].cols(r * hq * D, (r + 1) * hq * D).pack(device),
+            layers.append(LayerWeights(norm1=bf(norms[(l, "input_layernorm")]), qkv=_Linear.stack([q, k, v]).pack(device, int8),
+                                       o=lin[(l, "o_proj")].cols(r * hq * D, (r + 1) * hq * D).pack(device, int8),
                                        norm2=bf(norms[(l, "post_attention_layernorm")]), gate_up=pack16(gu), down=pack16(down),
-                                       router=lin[(l, "router")].pack(device)))
+                                       router=lin[(l, "router")].pack(device), **heads))
             continue
         gate = lin[(l, "gate_proj")].rows(r * ffn, (r + 1) * ffn)
         up = lin[(l, "up_proj")].rows(r * ffn, (r + 1) * ffn)
         fused_gate = ffn % 64 == 0          # silu(gate) * up in the GEMM epilogue needs the interleaved row order
-        gate_up = (_Linear.interleave(gate, up) if fused_gate else _Linear.stack([gate, up])).pack(device)
+        gate_up = (_Linear.interleave(gate, up) if fused_gate else _Linear.stack([gate, up])).pack(device, int8)
         gate_up.swiglu = fused_gate
-        layers.append(LayerWeights(norm1=bf(norms[(l, "input_layernorm")]), qkv=_Linear.stack([q, k, v]).pack(device),
-                                   o=lin[(l, "o_proj")].cols(r * hq * D, (r + 1) * hq * D).pack(device),
+        layers.append(LayerWeights(norm1=bf(norms[(l, "input_layernorm")]), qkv=_Linear.stack([q, k, v]).pack(device, int8),
+                                   o=lin[(l, "o_proj")].cols(r * hq * D, (r + 1) * hq * D).pack(device, int8),
                                    norm2=bf(norms[(l, "post_attention_layernorm")]), gate_up=gate_up,
-                                   down=lin[(l, "down_proj")].cols(r * ffn, (r + 1) * ffn).pack(device)))
+                                   down=lin[(l, "down_proj")].cols(r * ffn, (r + 1) * ffn).pack(device, int8), **heads))
     vs = cfg.vocab_size // tp_size
-    return LlmWeights(bf(parts["embed"]), layers, bf(parts["final_norm"]), parts["lm_head"].rows(r * vs, (r + 1) * vs).pack(device), tp_rank, tp_size)
+    return LlmWeights(bf(parts["embed"]), layers, bf(parts["final_norm"]), parts["lm_head"].rows(r * vs, (r + 1) * vs).pack(device, int8), tp_rank, tp_size)
