@@ -510,19 +510,32 @@ def _gemm_i8(x, w: "PackedWeight", out, residual, act, out_f32, glu, cap, norm) 
     if T == 0:
         return out
     if quantized:
-        pitch, q, scales, sums, raw, ld_raw = like.stride(0), like.data_ptr(), x.scales.data_ptr(), x.sums.data_ptr(), 0, 0
+        pitch, q, scales, sums, raw, ld_raw, scratch = like.stride(0), like.data_ptr(), x.scales.data_ptr(), x.sums.data_ptr(), 0, 0, 0
     else:
-        # the quantised rows, their scales and sums: memory of the caching allocator, which belongs to the stream
+        # memory for the quantised rows, their scales and sums, from the caching allocator: it belongs to the stream and is given back when the launches
+        # are queued, as a tensor's would be that goes out of scope
         pitch = (Kd + 15) // 16 * 16
-        rows = x.new_empty(T * (pitch // 2 + 4))
-        q, raw, ld_raw = rows.data_ptr(), x.data_ptr(), x.stride(0)
+        stream = torch._C._cuda_getCurrentRawStream(d)
+        q = scratch = _scratch(T * (pitch + 8), stream, d)
+        raw, ld_raw = x.data_ptr(), x.stride(0)
         scales = q + T * pitch
         sums = scales + 4 * T
-    _call(lib().ovb_gemm_i8, _GEMM_I8.pack(q, scales, sums, wt.data_ptr(), w.scales.data_ptr(), 0 if zps is None else zps.data_ptr(), 0 if bias is None else bias.data_ptr(),
-                                           0 if residual is None else residual.data_ptr(), out.data_ptr(), raw, 0 if gamma is None else gamma.data_ptr(),
-                                           0 if idx is None else idx.data_ptr(), ld_raw, T, N, Kd, pitch, ldo, ldr, act, dtype == torch.float16, bool(out_f32),
-                                           like.shape[0] if idx is not None else 0, limit, slope, shift, eps), d, "ovb_gemm_i8")
+    try:
+        _call(lib().ovb_gemm_i8, _GEMM_I8.pack(q, scales, sums, wt.data_ptr(), w.scales.data_ptr(), 0 if zps is None else zps.data_ptr(), 0 if bias is None else bias.data_ptr(),
+                                               0 if residual is None else residual.data_ptr(), out.data_ptr(), raw, 0 if gamma is None else gamma.data_ptr(),
+                                               0 if idx is None else idx.data_ptr(), ld_raw, T, N, Kd, pitch, ldo, ldr, act, dtype == torch.float16, bool(out_f32),
+                                               like.shape[0] if idx is not None else 0, limit, slope, shift, eps), d, "ovb_gemm_i8")
+    finally:
+        if scratch:
+            torch._C._cuda_cudaCachingAllocator_raw_delete(scratch)
     return out
+
+
+def _scratch(nbytes: int, stream: int, device: int) -> int:
+    if device == torch._C._cuda_getDevice():
+        return torch._C._cuda_cudaCachingAllocator_raw_alloc(nbytes, stream)
+    with torch.cuda.device(device):
+        return torch._C._cuda_cudaCachingAllocator_raw_alloc(nbytes, stream)
 
 
 def _result_pitch(name: str, t: torch.Tensor, dtype, T: int, cols: int) -> int:
