@@ -49,45 +49,44 @@ __device__ __forceinline__ void i8_quantize_row(const I8TileParams& p, uint8_t* 
     for (int h = 0; h < kI8Hold; ++h) {
         const int at = tid + h * SPAN;
         x[h] = at < pieces ? __ldcg(src + at) : make_uint4(0, 0, 0, 0);
-        if (p.gamma != nullptr && at < pieces) g[h] = __ldg(static_cast<const uint4*>(p.gamma) + at);
+        g[h] = p.gamma != nullptr && at < pieces ? __ldg(static_cast<const uint4*>(p.gamma) + at) : make_uint4(0, 0, 0, 0);
     }
-    float inv = 1.f;
-    if (p.gamma != nullptr) {
-        // in the order of ovb_quantize_rows for few rows of up to 4096 columns
-        uint64_t ss2 = pair_of(0.f);
-#pragma unroll
-        for (int h = 0; h < kI8Hold; ++h) {
-            float v[8];
-            row_values<E, false>(x[h], x[h], 1.f, v);
-#pragma unroll
-            for (int j = 0; j < 8; j += 2) ss2 = fma2(pair_of(v[j], v[j + 1]), pair_of(v[j], v[j + 1]), ss2);
-        }
-        float ss, ss1;
-        unpair(ss2, ss, ss1);
-        ss += ss1;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (lane == 0) box_f[warp] = ss;
-        meet();
-        ss = box_f[lane % kI8QuantWarps];
-#pragma unroll
-        for (int o = kI8QuantWarps / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        inv = rsqrtf(ss / (float)p.K + p.eps);
-    }
+    // sums in the order of ovb_quantize_rows for few rows of up to 4096 columns
     const bool norm = p.gamma != nullptr;
     uint32_t top = 0;
+    uint64_t ss2 = pair_of(0.f);
 #pragma unroll
-    for (int h = 0; h < kI8Hold; ++h)
-        if (tid + h * SPAN < pieces) top = norm ? top_of8<E, true>(x[h], g[h], inv, top) : top_of8<E, false>(x[h], x[h], 1.f, top);
+    for (int h = 0; h < kI8Hold; ++h) {
+        float v[8];
+        if (norm) {
+            row_values<E, true>(x[h], g[h], v);
+            row_pass<E, true>(x[h], v, top, ss2);
+        } else {
+            row_pass<E, false>(x[h], v, top, ss2);
+        }
+    }
+    float ss, ss1;
+    unpair(ss2, ss, ss1);
+    ss += ss1;
     top = norm ? top : row_top<E, false>(top);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0) box_u[warp] = top;
+    for (int o = 16; o > 0; o >>= 1) {
+        ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    }
+    if (lane == 0) {
+        box_f[warp] = ss;
+        box_u[warp] = top;
+    }
     meet();
-    top = 0;
+    ss = box_f[lane % kI8QuantWarps];
+    top = box_u[lane % kI8QuantWarps];
 #pragma unroll
-    for (int w = 0; w < kI8QuantWarps; ++w) top = max(top, box_u[w]);
-    const float f = row_factor(top);
+    for (int o = kI8QuantWarps / 2; o > 0; o >>= 1) {
+        ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    }
+    const float r = norm ? rsqrtf(ss / (float)p.K + p.eps) : 1.f, f = row_factor(top, r);
     int sum = 0;
 #pragma unroll
     for (int h = 0; h < kI8Hold; ++h) {
@@ -95,8 +94,8 @@ __device__ __forceinline__ void i8_quantize_row(const I8TileParams& p, uint8_t* 
         const bool mine = kb >= kb0 && kb < kb1;
         if (at >= pieces || (!mine && p.w_zp == nullptr)) continue;
         float v[8];
-        if (norm) row_values<E, true>(x[h], g[h], inv, v);
-        else row_values<E, false>(x[h], x[h], 1.f, v);
+        if (norm) row_values<E, true>(x[h], g[h], v);
+        else row_values<E, false>(x[h], x[h], v);
         const uint2 w = f != 0.f ? codes_of8(v, f) : make_uint2(0, 0);
         sum = sum_of8(w, sum);
         if (mine) *reinterpret_cast<uint2*>(codes + (kb - kb0) * kI8FusedBlock + ((at & 15) << 3)) = w;      // row 0 of the swizzle: in order
@@ -109,7 +108,7 @@ __device__ __forceinline__ void i8_quantize_row(const I8TileParams& p, uint8_t* 
     fence_proxy_async_smem();                           // the codes are read by the tensor cores
     meet();
     if (tid == 0) {
-        *row_scale = row_scale_of(top);
+        *row_scale = row_scale_of(top, r);
         sum = 0;
         if (p.w_zp != nullptr)
             for (int w = 0; w < kI8QuantWarps; ++w) sum += box_i[w];

@@ -29,22 +29,23 @@ struct I8Params {
     float act_limit, act_slope, act_shift;
 };
 
-// Quantisation of a row y (x, or x * rsqrt(mean(x^2) + eps) * gamma):  a = max |y|;  q = round_half_even(y * (127 / a));  scale = a / 127;  sum = sum q.
-// Quotients and products are rounded to 32 bits once each. |y| * (127 / a) is at most 127 (1 + 2^-23), so no value has to be clamped. A row whose largest
-// magnitude is below 2^-119, where 127 / a would not be finite, counts as zero (scale 0); one with a value that is not finite gets the scale NaN and codes of
-// zero, so that every result of the row is NaN. The magnitudes are compared as integers, where NaN is the largest.
+// Quantisation of a row y (x, or x * r * gamma with r = rsqrt(mean(x^2) + eps)):  a = max |y|;  q = round_half_even(y * (127 / a));  scale = a / 127;  sum = sum q.
+// Quotients and products are rounded to 32 bits once each. With a norm z = x * gamma is quantised instead of y: r drops out of the codes and is a factor of the
+// scale alone, so the sum of squares and the largest |z| come from one pass over the row (8192 rows of 4096: 28 us with two). |z| * (127 / max |z|) is at most 127 (1 + 2^-23), so no value has to
+// be clamped. A row whose largest magnitude is below 2^-119, where 127 / a would not be finite, counts as zero (scale 0); one with a value that is not
+// finite gets the scale NaN and codes of zero, so that every result of the row is NaN. The magnitudes are compared as integers, where NaN is the largest.
 constexpr uint32_t kNotFinite = 0x7F800000u;
 constexpr float kQuantFloor = 1.5046327690525280e-36f;      // 2^-119
 
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
-__device__ __forceinline__ float row_scale_of(uint32_t top) {
+// What a row is multiplied by to get its codes, 127 / max, or 0 where it has none; `r`: the norm's factor, or 1.
+__device__ __forceinline__ float row_factor(uint32_t top, float r) {
     const float a = __uint_as_float(top);
-    return top >= kNotFinite ? __int_as_float(0x7FFFFFFF) : a < kQuantFloor ? 0.f : __fdiv_rn(a, 127.f);
+    return top >= kNotFinite || a < kQuantFloor || __fmul_rn(a, r) < kQuantFloor ? 0.f : __fdiv_rn(127.f, a);
 }
-// 127 / a, or 0 where the row has no codes
-__device__ __forceinline__ float row_factor(uint32_t top) {
-    const float a = __uint_as_float(top);
-    return top >= kNotFinite || a < kQuantFloor ? 0.f : __fdiv_rn(127.f, a);
+__device__ __forceinline__ float row_scale_of(uint32_t top, float r) {
+    if (top >= kNotFinite || !(r < __int_as_float(0x7F800000))) return __int_as_float(0x7FFFFFFF);
+    return row_factor(top, r) != 0.f ? __fdiv_rn(__fmul_rn(__uint_as_float(top), r), 127.f) : 0.f;
 }
 
 __host__ __device__ inline bool is_gated(int act) { return act == OVB_ACT_SWIGLU || act == OVB_ACT_GLU_LIMITED; }
@@ -72,30 +73,34 @@ __device__ __forceinline__ uint2 codes_of8(const float (&y)[8], float f) {
 }
 __device__ __forceinline__ int sum_of8(uint2 codes, int sum) { return __dp4a((int)codes.y, 0x01010101, __dp4a((int)codes.x, 0x01010101, sum)); }
 
-// Eight values of a row: x, or x * inv * gamma.
+// Eight values of a row: x, or x * gamma.
 template <class E, bool NORM>
-__device__ __forceinline__ void row_values(const uint4& x, const uint4& g, float inv, float (&v)[8]) {
+__device__ __forceinline__ void row_values(const uint4& x, const uint4& g, float (&v)[8]) {
     const E* e = reinterpret_cast<const E*>(&x);
     const E* w = reinterpret_cast<const E*>(&g);
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
         uint64_t y = pair_of(to_float(e[j]), to_float(e[j + 1]));
-        if (NORM) y = mul2(mul2(y, pair_of(inv)), pair_of(to_float(w[j]), to_float(w[j + 1])));
+        if (NORM) y = mul2(y, pair_of(to_float(w[j]), to_float(w[j + 1])));
         unpair(y, v[j], v[j + 1]);
     }
 }
-// The largest magnitude of eight values, as the bits of fp32. Without a norm the 16-bit values are compared as pairs of integers.
+// One pass over eight values: the largest magnitude (with a norm the bits of fp32, without one a pair of 16-bit magnitudes: see row_top) and, with a norm,
+// the sum of squares of x.
 template <class E, bool NORM>
-__device__ __forceinline__ uint32_t top_of8(const uint4& x, const uint4& g, float inv, uint32_t top) {
+__device__ __forceinline__ void row_pass(const uint4& x, const float (&v)[8], uint32_t& top, uint64_t& ss2) {
     if (NORM) {
-        float v[8];
-        row_values<E, true>(x, g, inv, v);
+        const E* e = reinterpret_cast<const E*>(&x);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = max(top, magnitude(v[j]));
-        return top;
+        for (int j = 0; j < 8; j += 2) {
+            const uint64_t y = pair_of(to_float(e[j]), to_float(e[j + 1]));
+            ss2 = fma2(y, y, ss2);
+            top = max(top, max(magnitude(v[j]), magnitude(v[j + 1])));
+        }
+    } else {
+        constexpr uint32_t M = 0x7FFF7FFFu;
+        top = __vmaxu2(top, __vmaxu2(__vmaxu2(x.x & M, x.y & M), __vmaxu2(x.z & M, x.w & M)));
     }
-    constexpr uint32_t M = 0x7FFF7FFFu;                 // (here `top` is a pair of 16-bit magnitudes: see row_top)
-    return __vmaxu2(top, __vmaxu2(__vmaxu2(x.x & M, x.y & M), __vmaxu2(x.z & M, x.w & M)));
 }
 template <class E, bool NORM>
 __device__ __forceinline__ uint32_t row_top(uint32_t top) {

@@ -2,8 +2,9 @@
 //
 // The arithmetic is in gemm_i8.cuh; the norm's sums are held in 32 bits.
 //
-// What bounds it: memory, three bytes per value (two of them usually from L2). A row stays in registers between the passes: every thread holds HOLD
-// pieces of eight columns.
+// What bounds it: memory, three bytes per value (two of them usually from L2). A row is read once and stays in registers until its largest magnitude is known:
+// every thread holds HOLD pieces of eight columns, as they came or, with a norm, times the weights. Measured without and with a norm: 8192 x 4096 16.4 and
+// 21.9 us, 8192 x 8192 29.8 and 43.8 us (6.8 and 4.6 TB/s; the weights are read again by every row, from L1), 64 x 4096 1.8 and 2.0 us, of which most is the launch.
 #include "gemm_i8.cuh"
 
 namespace ovb {
@@ -21,9 +22,12 @@ struct QuantParams {
     float eps;
 };
 
-constexpr int kManyRows = 1024;
+// From so many rows on, a row gets few warps with more of it each, which are enough to fill the machine and spend less on meeting; below it many warps, for the
+// time of one row. 600 rows, many warps and few: 2.9 and 2.3 us (2048 columns), 3.9 and 3.3 (4096), 5.2 and 4.5 (8192); 400 rows: 2.0 and 2.1, 2.5 and 2.5,
+// 4.3 and 3.9; 8192 rows of 4096: 20.3 and 16.4.
+constexpr int kManyRows = 512;
 
-// The sum (largest) over the warps that share a row; every thread gets it.
+// f over the warps that share a row; every thread gets it.
 template <int WPR, class T, class F>
 __device__ __forceinline__ T over_row(T v, T* box, F&& f) {
 #pragma unroll
@@ -37,9 +41,32 @@ __device__ __forceinline__ T over_row(T v, T* box, F&& f) {
     for (int o = WPR / 2; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
+// The sum of s and the largest t, one barrier for both.
+template <int WPR>
+__device__ __forceinline__ void over_row(float& s, uint32_t& t, float* box_s, uint32_t* box_t) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, o);
+        t = max(t, __shfl_xor_sync(0xffffffffu, t, o));
+    }
+    if (WPR == 1) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (lane == 0) {
+        box_s[warp] = s;
+        box_t[warp] = t;
+    }
+    __syncthreads();
+    s = box_s[lane % WPR];
+    t = box_t[lane % WPR];
+#pragma unroll
+    for (int o = WPR / 2; o > 0; o >>= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, o);
+        t = max(t, __shfl_xor_sync(0xffffffffu, t, o));
+    }
+}
 
-__device__ __forceinline__ void row_result(const QuantParams& p, int row, uint32_t top, int sum) {
-    p.scale[row] = row_scale_of(top);
+__device__ __forceinline__ void row_result(const QuantParams& p, int row, uint32_t top, float r, int sum) {
+    p.scale[row] = row_scale_of(top, r);
     p.sum[row] = sum;
 }
 
@@ -62,56 +89,46 @@ __global__ void __launch_bounds__(WPR < 4 ? 128 : WPR * 32) quantize_rows_kernel
     if (row >= p.rows) return;              // whole warps, and only where rows do not share a block's barriers
     const uint4* src = reinterpret_cast<const uint4*>(static_cast<const E*>(p.x) + (size_t)source_row(p, row) * p.ldx);
     const uint4* gamma = static_cast<const uint4*>(p.gamma);
-    constexpr bool HELD = NORM && HOLD <= 4;            // with more pieces the weights do not fit the registers beside the row: they are read again
-    uint4 x[HOLD], g[HELD ? HOLD : 1];
+    uint4 x[HOLD], g[NORM ? HOLD : 1];
 #pragma unroll
-    for (int h = 0; h < HOLD; ++h) x[h] = at + h * SPAN < pieces ? __ldcg(src + at + h * SPAN) : make_uint4(0, 0, 0, 0);
-    if (HELD) {
-#pragma unroll
-        for (int h = 0; h < HOLD; ++h)
-            if (at + h * SPAN < pieces) g[h] = __ldg(gamma + at + h * SPAN);
+    for (int h = 0; h < HOLD; ++h) {
+        const bool in = at + h * SPAN < pieces;
+        x[h] = in ? __ldcg(src + at + h * SPAN) : make_uint4(0, 0, 0, 0);
+        if (NORM) g[h] = in ? __ldg(gamma + at + h * SPAN) : make_uint4(0, 0, 0, 0);
     }
-    float inv = 1.f;
+    uint32_t top = 0;
+    uint64_t ss2 = pair_of(0.f);
+    float v[NORM ? HOLD : 1][8];
+#pragma unroll
+    for (int h = 0; h < HOLD; ++h) {
+        if (NORM) row_values<E, NORM>(x[h], g[h % (NORM ? HOLD : 1)], v[h % (NORM ? HOLD : 1)]);
+        row_pass<E, NORM>(x[h], v[h % (NORM ? HOLD : 1)], top, ss2);
+    }
+    float r = 1.f;
+    top = row_top<E, NORM>(top);
     if (NORM) {
-        uint64_t ss2 = pair_of(0.f);
-#pragma unroll
-        for (int h = 0; h < HOLD; ++h) {
-            float v[8];
-            row_values<E, false>(x[h], x[h], 1.f, v);
-#pragma unroll
-            for (int j = 0; j < 8; j += 2) ss2 = fma2(pair_of(v[j], v[j + 1]), pair_of(v[j], v[j + 1]), ss2);
-        }
         float ss, ss1;
         unpair(ss2, ss, ss1);
-        ss = over_row<WPR>(ss + ss1, box_f, [](float a, float b) { return a + b; });
-        inv = rsqrtf(ss / (float)p.cols + p.eps);
+        ss += ss1;
+        over_row<WPR>(ss, top, box_f, box_u);
+        r = rsqrtf(ss / (float)p.cols + p.eps);
+    } else {
+        top = over_row<WPR>(top, box_u, [](uint32_t a, uint32_t b) { return max(a, b); });
     }
-    auto weights = [&](int h) {
-        if (NORM && !HELD) g[0] = __ldg(gamma + at + h * SPAN);
-    };
-    uint32_t top = 0;
-#pragma unroll
-    for (int h = 0; h < HOLD; ++h)
-        if (at + h * SPAN < pieces) {
-            weights(h);
-            top = top_of8<E, NORM>(x[h], g[HELD ? h : 0], inv, top);
-        }
-    top = over_row<WPR>(row_top<E, NORM>(top), box_u, [](uint32_t a, uint32_t b) { return max(a, b); });
-    const float f = row_factor(top);
+    const float f = row_factor(top, r);
     uint2* dst = reinterpret_cast<uint2*>(p.q + (size_t)row * p.ldq);
     int sum = 0;
 #pragma unroll
     for (int h = 0; h < HOLD; ++h)
         if (at + h * SPAN < pieces) {
-            float v[8];
-            weights(h);
-            row_values<E, NORM>(x[h], g[HELD ? h : 0], inv, v);
-            const uint2 w = f != 0.f ? codes_of8(v, f) : make_uint2(0, 0);
+            float (&y)[8] = v[h % (NORM ? HOLD : 1)];
+            if (!NORM) row_values<E, NORM>(x[h], x[h], y);
+            const uint2 w = f != 0.f ? codes_of8(y, f) : make_uint2(0, 0);
             sum = sum_of8(w, sum);
             dst[at + h * SPAN] = w;
         }
     sum = over_row<WPR>(sum, box_i, [](int a, int b) { return a + b; });
-    if (at == 0) row_result(p, row, top, sum);
+    if (at == 0) row_result(p, row, top, r, sum);
 }
 
 // Any width, pitch and alignment: a block per row, which is read once for each pass.
@@ -124,18 +141,16 @@ __global__ void __launch_bounds__(256) quantize_rows_any_kernel(const QuantParam
     const int row = blockIdx.x;
     const E* src = static_cast<const E*>(p.x) + (size_t)source_row(p, row) * p.ldx;
     const E* gamma = static_cast<const E*>(p.gamma);
-    float inv = 1.f;
-    if (gamma != nullptr) {
-        float ss = 0.f;
-        for (int k = threadIdx.x; k < p.cols; k += 256) ss = fmaf(to_float(src[k]), to_float(src[k]), ss);
-        ss = over_row<8>(ss, box_f, [](float a, float b) { return a + b; });
-        inv = rsqrtf(ss / (float)p.cols + p.eps);
-    }
-    auto value = [&](int k) { return gamma != nullptr ? to_float(src[k]) * inv * to_float(gamma[k]) : to_float(src[k]); };
+    auto value = [&](int k) { return gamma != nullptr ? __fmul_rn(to_float(src[k]), to_float(gamma[k])) : to_float(src[k]); };
+    float ss = 0.f, r = 1.f;
     uint32_t top = 0;
-    for (int k = threadIdx.x; k < p.cols; k += 256) top = max(top, magnitude(value(k)));
-    top = over_row<8>(top, box_u, [](uint32_t a, uint32_t b) { return max(a, b); });
-    const float f = row_factor(top);
+    for (int k = threadIdx.x; k < p.cols; k += 256) {
+        ss = fmaf(to_float(src[k]), to_float(src[k]), ss);
+        top = max(top, magnitude(value(k)));
+    }
+    over_row<8>(ss, top, box_f, box_u);
+    if (gamma != nullptr) r = rsqrtf(ss / (float)p.cols + p.eps);
+    const float f = row_factor(top, r);
     int sum = 0;
     for (int k = threadIdx.x; k < p.cols; k += 256) {
         const int c = f != 0.f ? __float2int_rn(__fmul_rn(value(k), f)) : 0;
@@ -143,7 +158,7 @@ __global__ void __launch_bounds__(256) quantize_rows_any_kernel(const QuantParam
         p.q[(size_t)row * p.ldq + k] = (uint8_t)(c & 0xFF);
     }
     sum = over_row<8>(sum, box_i, [](int a, int b) { return a + b; });
-    if (threadIdx.x == 0) row_result(p, row, top, sum);
+    if (threadIdx.x == 0) row_result(p, row, top, r, sum);
 }
 
 template <class E, bool NORM>
@@ -152,14 +167,14 @@ static cudaError_t run_quantize(const QuantParams& p, cudaStream_t stream) {
                        ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.gamma)) & 15) == 0 && (reinterpret_cast<uintptr_t>(p.q) & 7) == 0;
     if (!whole || p.cols > 32768) return launch_pdl(quantize_rows_any_kernel<E>, dim3(p.rows), dim3(256), 0, stream, p);
     auto go = [&](auto kern, int wpr) { return launch_pdl(kern, dim3(wpr < 4 ? (p.rows + 4 / wpr - 1) / (4 / wpr) : p.rows), dim3(wpr < 4 ? 128 : wpr * 32), 0, stream, p); };
-    // Many rows: few warps to a row, with more of it each (from so many on that they fill the machine); few rows: many warps, for the time of one row.
     const bool many = p.rows >= kManyRows;
     if (p.cols <= 512) return go(quantize_rows_kernel<E, NORM, 1, 2>, 1);
     if (p.cols <= 1024) return go(quantize_rows_kernel<E, NORM, 1, 4>, 1);
     if (p.cols <= 2048) return many ? go(quantize_rows_kernel<E, NORM, 1, 8>, 1) : go(quantize_rows_kernel<E, NORM, 8, 1>, 8);
     if (p.cols <= 4096) return many ? go(quantize_rows_kernel<E, NORM, 4, 4>, 4) : go(quantize_rows_kernel<E, NORM, 8, 2>, 8);
     if (p.cols <= 8192) return many ? go(quantize_rows_kernel<E, NORM, 4, 8>, 4) : go(quantize_rows_kernel<E, NORM, 16, 2>, 16);
-    if (p.cols <= 16384) return many ? go(quantize_rows_kernel<E, NORM, 8, 8>, 8) : go(quantize_rows_kernel<E, NORM, 16, 4>, 16);
+    // with a norm eight pieces take too many registers here: 1024 rows of 14336 in 13.9 us, in 12.9 with four
+    if (p.cols <= 16384) return many && !NORM ? go(quantize_rows_kernel<E, false, 8, 8>, 8) : go(quantize_rows_kernel<E, NORM, 16, 4>, 16);
     return go(quantize_rows_kernel<E, NORM, 16, 8>, 16);
 }
 
