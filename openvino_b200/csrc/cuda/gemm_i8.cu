@@ -384,10 +384,12 @@ static int launch_i8_tile(int form, const cudaLaunchConfig_t& cfg, const CUtenso
 
 // A single token's row is quantised by the product's kernel: whole aligned pieces of eight columns, as many as eight warps hold. (us with a norm, one launch / two:
 // 1 x 6144 x 4096 9.6 / 9.8, where the second launch also costs the host 2.5. With four rows the kernel's own way costs more than it saves: 4 x 4096 x 4096
-// 10.2 / 8.3.)
+// 10.2 / 8.3.) Every CTA reads the whole row at a time of its own, so a result in the row's place has it quantised first, by a launch of its own.
 static bool i8_fuses(const ovb_gemm_i8_args* a) {
     const auto bits = [](const void* x) { return reinterpret_cast<uintptr_t>(x); };
-    return a->raw != nullptr && a->T == 1 && a->K % 8 == 0 && a->K <= kI8QuantWarps * 32 * kI8Hold * 8 && (a->row_idx == nullptr || a->ld_raw % 8 == 0) &&
+    const uintptr_t rows = a->row_idx != nullptr ? ((uintptr_t)(a->raw_rows - 1) * (uintptr_t)a->ld_raw + (uintptr_t)a->K) * 2 : (uintptr_t)a->K * 2;
+    const bool apart = bits(a->out) >= bits(a->raw) + rows || bits(a->raw) >= bits(a->out) + (uintptr_t)a->N * 4;
+    return apart && a->raw != nullptr && a->T == 1 && a->K % 8 == 0 && a->K <= kI8QuantWarps * 32 * kI8Hold * 8 && (a->row_idx == nullptr || a->ld_raw % 8 == 0) &&
            ((bits(a->raw) | bits(a->gamma)) & 15) == 0;
 }
 

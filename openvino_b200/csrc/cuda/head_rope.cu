@@ -308,7 +308,7 @@ extern "C" int ovb_qk_norm_rope(const ovb_qk_rope_args* a, ovb_stream_t stream_)
     using namespace ovb;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     OVB_REQUIRE(a && a->q && a->q_out && a->k && a->positions, "ovb_qk_norm_rope: null operand");
-    OVB_REQUIRE(a->B > 0 && a->S > 0 && a->Hq > 0 && a->Hkv > 0 && (int64_t)a->B * a->S <= INT32_MAX, "ovb_qk_norm_rope: empty problem B=%d S=%d Hq=%d Hkv=%d", a->B, a->S, a->Hq, a->Hkv);
+    OVB_REQUIRE(a->B > 0 && a->S > 0 && a->Hq > 0 && a->Hkv > 0 && (int64_t)a->B * a->S <= INT32_MAX - kRopeThreads, "ovb_qk_norm_rope: empty or too large a problem B=%d S=%d Hq=%d Hkv=%d", a->B, a->S, a->Hq, a->Hkv);
     OVB_REQUIRE(a->D > 0 && a->D % 2 == 0 && a->D <= 4096 && a->rot >= 0 && a->rot % 2 == 0 && a->rot <= a->D, "ovb_qk_norm_rope: head size %d, rotation %d", a->D, a->rot);
     OVB_REQUIRE(a->rot == 0 || a->inv_freq, "ovb_qk_norm_rope: a rotation needs frequencies");
     const bool cache = a->k_cache != nullptr;

@@ -432,6 +432,14 @@ class QuantizedRows:
     __slots__ = ("q", "scales", "sums", "dtype")
 
     def __init__(self, q, scales, sums, dtype):
+        if q.dim() != 2 or q.dtype != torch.int8 or (dtype != torch.bfloat16 and dtype != torch.float16):
+            raise ValueError("codes are int8 [T, K] of bf16 or fp16 rows, not %s %s of %s" % (q.dtype, tuple(q.shape), dtype))
+        T, device = q.shape[0], q.get_device()
+        for t, kind in ((scales, torch.float32), (sums, torch.int32)):
+            if t.shape != (T,) or t.dtype != kind or not t.is_contiguous() or t.get_device() != device:
+                raise ValueError("scales are fp32 and sums int32, %d values in order on the device of the codes" % T)
+        if T and (q.stride(1) != 1 and q.shape[1] != 1 or q.stride(0) % 16 or q.stride(0) < q.shape[1]):
+            raise ValueError("codes of a row lie side by side, with a row pitch that is a multiple of 16")
         self.q, self.scales, self.sums, self.dtype = q, scales, sums, dtype
 
     @property

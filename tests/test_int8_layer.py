@@ -224,6 +224,25 @@ def test_product_with_the_norm_in_front(K, T):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 5, 600])
+def test_results_in_the_place_of_the_rows(K, T):
+    """x + W norm(x) written over x: rows are quantised before the first result is stored."""
+    Kd = 4096
+    x = torch.randn((T, Kd), generator=gen(T), device="cuda").bfloat16()
+    gamma = (1 + 0.2 * torch.randn(Kd, generator=gen(2), device="cuda")).bfloat16()
+    w, s, z = weight(Kd, Kd, "signed_zp", 3)
+    pw = K.PackedWeight.from_ir_i8(w, s, z)
+    want = K.gemm(K.quantize_rows(x, norm=(gamma, 1e-5)), pw, residual=x)
+    for _ in range(8):
+        h = x.clone()
+        assert torch.equal(K.gemm(h, pw, out=h, residual=h, norm=(gamma, 1e-5)), want)
+    many = torch.cat([x, x])[:T + 1].contiguous()           # one row of several, picked by its index, over another
+    pick = torch.zeros(1, dtype=torch.int32, device="cuda")
+    one = K.gemm(many, pw, norm=(gamma, 1e-5, pick))
+    assert torch.equal(K.gemm(many, pw, out=many[:1], norm=(gamma, 1e-5, pick)), one)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("T,N,Kd", [(1, 128, 65536), (20, 130, 65536), (300, 256, 65536)])
 def test_largest_sums_stay_exact(K, T, N, Kd):
     x = torch.ones((T, Kd), device="cuda", dtype=torch.bfloat16)
@@ -578,6 +597,19 @@ def test_products_are_refused(call):
     from openvino_b200.ops import cuda as K
     with pytest.raises(ValueError):
         call(K, torch.zeros((4, 64)).bfloat16(), cpu_weight())
+
+
+@pytest.mark.parametrize("change", [
+    dict(q=torch.zeros((4, 64), dtype=torch.uint8)), dict(q=torch.zeros(64, dtype=torch.int8)), dict(q=torch.zeros((4, 60), dtype=torch.int8)),
+    dict(q=torch.zeros((64, 4), dtype=torch.int8).t()), dict(q=torch.zeros((1, 64), dtype=torch.int8).expand(4, 64)), dict(scales=torch.ones(3)), dict(scales=torch.ones(4).half()),
+    dict(scales=torch.ones((4, 1))), dict(scales=torch.ones(8)[::2]), dict(sums=torch.zeros(4)), dict(sums=torch.zeros(5, dtype=torch.int32)), dict(dtype=torch.float32),
+])
+def test_quantised_rows_hold_together(change):
+    from openvino_b200.ops import cuda as K
+    good = dict(q=torch.zeros((4, 64), dtype=torch.int8), scales=torch.ones(4), sums=torch.zeros(4, dtype=torch.int32), dtype=torch.bfloat16)
+    assert K.QuantizedRows(**good).shape == (4, 64)
+    with pytest.raises(ValueError):
+        K.QuantizedRows(**dict(good, **change))
 
 
 HEADS = dict(q=torch.zeros((1, 4, 2, 64)).half(), k=torch.zeros((1, 4, 1, 64)).half(), positions=torch.zeros(4, dtype=torch.int32), inv_freq=torch.ones(32))
