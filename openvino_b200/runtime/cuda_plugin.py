@@ -79,7 +79,7 @@ def _npuw_function_call(n, ins, ctx):
     from .npuw import function_of
     f = function_of(n)
     progs = f.__dict__.setdefault("_cuda_programs", {})
-    key = (str(ctx.device), ctx.precision)
+    key = (str(ctx.device), ctx.precision, ctx.dynamic_quantization)
     prog = progs.get(key)
     if prog is None:
         prog = progs[key] = GraphProgram(f.body, ctx.device, ctx.precision, dynamic_quantization=ctx.dynamic_quantization)
