@@ -73,7 +73,7 @@ def _rope(x, pos, cfg):
     inv = torch.tensor(cfg.inv_freq(), device=x.device, dtype=torch.float32)
     rot = 2 * inv.numel()
     ang = pos.float()[:, None] * inv[None, :]
-    cos, sin = ang.cos()[:, None, :], ang.sin()[:, None, :]
+    cos, sin = ang.cos()[:, None, :] * cfg.rope_scale, ang.sin()[:, None, :] * cfg.rope_scale
     if cfg.rope_interleaved:
         x1, x2 = x[..., 0:rot:2], x[..., 1:rot:2]
         turned = torch.stack([x1 * cos - x2 * sin, x2 * cos + x1 * sin], dim=-1).flatten(-2)

@@ -31,6 +31,7 @@ class LlmConfig:
     rotary_dim: int = 0           # dimensions of a head that the position rotates; 0: all
     rope_interleaved: bool = False                          # dimension pairs (2 i, 2 i + 1) instead of (i, i + rotary_dim / 2)
     rope_inv_freq: Optional[Tuple[float, ...]] = None       # frequencies one by one (scaled tables); None: powers of rope_theta
+    rope_scale: float = 1.0       # what cos and sin are multiplied by
 
     def inv_freq(self) -> List[float]:
         rot = self.rotary_dim or self.head_dim
@@ -39,7 +40,7 @@ class LlmConfig:
     @property
     def plain_rotation(self) -> bool:
         """Whole heads turn by powers of one base, halves paired, without head norms: what the step of one native call takes."""
-        return not (self.qk_norm or self.rope_interleaved or self.rope_inv_freq is not None or self.rotary_dim not in (0, self.head_dim))
+        return not (self.qk_norm or self.rope_interleaved or self.rope_inv_freq is not None or self.rope_scale != 1.0 or self.rotary_dim not in (0, self.head_dim))
 
     @property
     def q_size(self) -> int:

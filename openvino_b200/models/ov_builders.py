@@ -159,8 +159,11 @@ def build_llama(cfg: LlmConfig, state: Dict[str, torch.Tensor], compress: Option
     pos = ops.convert(ops.unsqueeze(position_ids, _i64([2])), "f32")               # [B, L, 1]
     ang = ops.multiply(pos, constant(inv_freq.reshape(1, 1, -1)))                  # [B, L, D/2]
     ang = ops.concat([ang.output(0), ang.output(0)], 2)
-    cos = ops.unsqueeze(ops.cos(ang), _i64([1])).output(0)
-    sin = ops.unsqueeze(ops.sin(ang), _i64([1])).output(0)
+    cos, sin = ops.cos(ang), ops.sin(ang)
+    if cfg.rope_scale != 1.0:
+        cos, sin = (ops.multiply(t, constant(np.array(cfg.rope_scale, dtype=np.float32))) for t in (cos, sin))
+    cos = ops.unsqueeze(cos, _i64([1])).output(0)
+    sin = ops.unsqueeze(sin, _i64([1])).output(0)
 
     # additive causal + padding mask [B, 1, L, S]: position of key j must be <= position of query i and mask[j] == 1
     shape_ids = ops.shape_of(input_ids)

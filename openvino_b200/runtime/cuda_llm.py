@@ -472,7 +472,7 @@ class CudaLlmExecutor(LlmExecutor):
             self._normed(h, lw.norm1, x, lw.qkv, qkv)
             if self.inv_freq is not None:
                 K.qk_norm_rope_kv_write(qkv, positions, slot_map, self.k_cache[l], self.v_cache[l], self.inv_freq, self.hq, self.hkv, D, self.block_size,
-                                        lw.q_norm, lw.k_norm, cfg.qk_norm_eps or cfg.rms_eps, cfg.rope_interleaved, k_meta=self.k_meta[l], v_meta=self.v_meta[l])
+                                        lw.q_norm, lw.k_norm, cfg.qk_norm_eps or cfg.rms_eps, cfg.rope_interleaved, cfg.rope_scale, k_meta=self.k_meta[l], v_meta=self.v_meta[l])
             elif self.kv_u8:
                 K.rope_kv_write_u8(qkv, positions, slot_map, self.k_cache[l], self.v_cache[l], self.k_meta[l], self.v_meta[l], self.hq, self.hkv, D,
                                    cfg.rope_theta, self.block_size)

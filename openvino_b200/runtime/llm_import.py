@@ -196,26 +196,67 @@ def _one(nodes, what: str) -> Node:
     return nodes[0]
 
 
-def _frequencies(rope: Optional[Node], half: int) -> Optional[np.ndarray]:
-    """The table of ``half`` rotation frequencies behind the cosine input of a RoPE node."""
-    if rope is None:
+class _Rotation:
+    """What a RoPE node and the graph behind its cosine input say: the dimensions that turn, their pairing, the table of frequencies (None where no constant
+    looks like one) and the factor of cos and sin. Scalar factors of the angles are taken into the table."""
+
+    def __init__(self, rope: Node, head_size: int):
+        at = rope.get_attributes()
+        self.rot = int(at.get("rotary_ndims") or head_size)
+        self.interleaved = bool(at.get("is_interleaved"))
+        self.freq, self.scale = None, 1.0
+        factor, half = 1.0, self.rot // 2
+        seen, frontier = set(), [(rope.input_value(1).get_node(), False)]
+        while frontier:
+            nxt = []
+            for n, of_angle in frontier:
+                if n in seen:
+                    continue
+                seen.add(n)
+                kind = n.get_type_name()
+                if kind == "Constant":
+                    if self.freq is None and n.get_output_element_type(0).is_real() and int(np.prod(n.get_output_shape(0) or [1])) == half:
+                        v = n.get_tensor_view().to_float32().reshape(-1).astype(np.float64)
+                        if np.isfinite(v).all() and (v > 0).all() and (np.diff(v) <= 0).all():
+                            self.freq = v
+                    continue
+                if kind in ("Multiply", "Divide"):
+                    for i in range(2):
+                        c = _scalar(n.input_value(i).get_node())
+                        if c and (kind == "Multiply" or i == 1):
+                            c = c if kind == "Multiply" else 1.0 / c
+                            factor, self.scale = (factor * c, self.scale) if of_angle else (factor, self.scale * c)
+                nxt.extend((n.input_value(i).get_node(), of_angle or kind == "Cos") for i in range(n.get_input_size()))
+            frontier = nxt
+        if self.freq is not None and half > 1:
+            self.freq = self.freq * factor
+
+    def same(self, other: "_Rotation") -> bool:
+        if (self.rot, self.interleaved, self.freq is None) != (other.rot, other.interleaved, other.freq is None) or abs(self.scale / other.scale - 1.0) > 1e-3:
+            return False
+        return self.freq is None or bool(np.allclose(self.freq, other.freq, rtol=1e-3))
+
+
+def _scalar(n: Node) -> Optional[float]:
+    """The value of a real constant of one element (behind a Convert)."""
+    if n.get_type_name() == "Convert":
+        n = n.input_value(0).get_node()
+    if n.get_type_name() != "Constant" or not n.get_output_element_type(0).is_real() or int(np.prod(n.get_output_shape(0) or [1])) != 1:
         return None
-    seen, frontier = set(), [rope.input_value(1).get_node()]
-    while frontier:
-        nxt = []
-        for n in frontier:
-            if n in seen:
-                continue
-            seen.add(n)
-            if n.get_type_name() == "Constant":
-                if n.get_output_element_type(0).is_real() and int(np.prod(n.get_output_shape(0) or [1])) == half:
-                    v = n.get_tensor_view().to_float32().reshape(-1).astype(np.float64)
-                    if np.isfinite(v).all() and (v > 0).all() and (np.diff(v) <= 0).all():
-                        return v
-                continue
-            nxt.extend(n.input_value(i).get_node() for i in range(n.get_input_size()))
-        frontier = nxt
-    return None
+    return float(n.get_tensor_view().to_float32().reshape(-1)[0])
+
+
+def _head_norm(found: Dict, projection: Optional[Node]) -> Optional[Node]:
+    """The norm of heads that was passed on the way to their projection."""
+    norm = found.get("norm")
+    if norm is None:
+        return None
+    below: Dict = {}
+    if _nearest_fc_ancestor(norm.input_value(0), 0, below) != projection:
+        return None                             # a norm of something else, met through shapes
+    if "rope" in below:
+        raise NotAnLlm("head norms behind the rotation are not served")
+    return norm
 
 
 def _head_size(att: Node) -> int:
@@ -261,17 +302,23 @@ def analyze(model: Model) -> Tuple[LlmConfig, Dict]:
     experts: Dict[int, Dict] = {}
     eps = 1e-6
     last_add = first_norm = None
-    head_eps, rope = 0.0, None
+    head_eps: Dict[float, None] = {}
+    rotation = None
     for l, a in enumerate(att):
         D = _head_size(a)
         on_q: Dict = {}
         on_k: Dict = {}
         q, k, v = _nearest_fc_ancestor(a.input_value(0), D, on_q), _nearest_fc_ancestor(a.input_value(1), D, on_k), _nearest_fc_ancestor(a.input_value(2))
-        for key, on in (("q_norm", on_q), ("k_norm", on_k)):
-            if "norm" in on:
-                norms[(l, key)] = _gamma(on["norm"])
-                head_eps = float(on["norm"].get_attribute("epsilon"))
-        rope = rope or on_q.get("rope")
+        for key, on, projection in (("q_norm", on_q, q), ("k_norm", on_k, k)):
+            norm = _head_norm(on, projection)
+            if norm is not None:
+                norms[(l, key)] = _gamma(norm)
+                head_eps[float(norm.get_attribute("epsilon"))] = None
+            if "rope" in on:
+                r = _Rotation(on["rope"], D)
+                rotation = rotation or r
+                if not rotation.same(r):
+                    raise NotAnLlm("rotations that differ between layers, or between queries and keys, are not served")
         if q is None or k is None or v is None:
             raise NotAnLlm("attention %d is not fed by three projections" % l)
         n1 = q.input_value(0).get_node()
@@ -367,14 +414,14 @@ def analyze(model: Model) -> Tuple[LlmConfig, Dict]:
                     break
     # what the graph's RoPE nodes say beyond that: the rotated dimensions, their pairing, and frequencies that are not powers of one base
     more = {}
-    if rope is not None:
-        at = rope.get_attributes()
-        rot = int(at.get("rotary_ndims") or D)
+    if rotation is not None:
+        rot, v = rotation.rot, rotation.freq
         if rot != D:
             more["rotary_dim"] = rot
-        if at.get("is_interleaved"):
+        if rotation.interleaved:
             more["rope_interleaved"] = True
-        v = _frequencies(rope, rot // 2)
+        if abs(rotation.scale - 1.0) > 1e-6:
+            more["rope_scale"] = rotation.scale
         if v is not None and rot >= 4:
             base = (v[1] / v[0]) ** (-rot / 2.0)
             if abs(v[0] - 1.0) > 1e-6 or np.abs(v * base ** (2.0 * np.arange(rot // 2) / rot) - 1.0).max() > 1e-3:
@@ -385,7 +432,9 @@ def analyze(model: Model) -> Tuple[LlmConfig, Dict]:
     if any(normed):
         if not all(normed):
             raise NotAnLlm("head norms in a part of the layers, or of the queries or keys alone, are not served")
-        more.update(qk_norm=True, qk_norm_eps=head_eps)
+        if len(head_eps) != 1:
+            raise NotAnLlm("head norms of different epsilon are not served")
+        more.update(qk_norm=True, qk_norm_eps=next(iter(head_eps)))
     first = lin[(layers[0], "q_proj")]
     fmt = {"u4": "int4", "u8": "int8"}[first.kind] if first.compressed else "bf16"
     cfg = LlmConfig(name=model.get_friendly_name() or "llm", vocab_size=embed.shape[0], hidden_size=H, num_layers=len(layers), num_heads=Hq,

@@ -6,7 +6,7 @@ import torch
 import openvino_b200 as ov
 from openvino_b200 import passes
 from openvino_b200 import properties as props
-from openvino_b200.models import llama
+from openvino_b200.models import llama, ov_builders
 from openvino_b200.models.llm_config import TINY_LLAMA, TINY_MOE
 from openvino_b200.models.ov_builders import build_llama
 from openvino_b200.runtime import llm_import
@@ -66,6 +66,53 @@ def test_head_norms_and_rotations_are_recognised(form, in_pages, tmp_path):
         for l in range(2):
             for key in ("q_norm", "k_norm"):
                 assert torch.allclose(parts["norms"][(l, key)], state["layers.%d.%s" % (l, key)].float())
+
+
+@pytest.mark.parametrize("in_pages", [False, True])
+def test_factors_of_the_rotation_are_recognised(in_pages):
+    cfg = SMALL.with_(rope_scale=1.25)
+    state = llama.random_float_state(cfg, seed=4, std=0.05)
+    m = build_llama(cfg, state)
+    ids = np.array([[5, 9, 200, 17, 3]], dtype=np.int64)
+    want = llama.reference_logits(cfg, {k: v.float() for k, v in state.items()}, torch.tensor(ids[0])).numpy()
+    assert np.abs(ov.Core().compile_model(m, "CPU")(feed_of(ids))[0][0] - want).max() < 1e-3 * np.abs(want).max()
+    got, _ = llm_import.analyze(paged(m) if in_pages else m)
+    assert abs(got.rope_scale - 1.25) < 1e-6 and got.rope_inv_freq is None and not got.plain_rotation
+
+
+def test_angles_with_a_factor_are_another_table(monkeypatch):
+    """positions * frequencies / 4: as if the frequencies were a quarter."""
+    cos, sin = ov_builders.ops.cos, ov_builders.ops.sin
+    quarter = lambda a: ov_builders.ops.divide(a, ov_builders.constant(np.array(4.0, dtype=np.float32)))
+    monkeypatch.setattr(ov_builders.ops, "cos", lambda a: cos(quarter(a)))
+    monkeypatch.setattr(ov_builders.ops, "sin", lambda a: sin(quarter(a)))
+    got, _ = llm_import.analyze(build_llama(SMALL, llama.random_float_state(SMALL, seed=1, std=0.05)))
+    assert got.rope_scale == 1.0 and np.allclose(got.inv_freq(), np.array(SMALL.inv_freq()) / 4, rtol=1e-3)
+
+
+def test_norms_behind_the_rotation_are_refused(monkeypatch):
+    rope = ov_builders._rope
+    count = iter(range(100))
+    monkeypatch.setattr(ov_builders, "_rope", lambda x, c, s, D: ov_builders._rms(rope(x, c, s, D), np.full(128, 1.5, np.float32), 1e-6, "late%d" % next(count)))
+    with pytest.raises(llm_import.NotAnLlm, match="behind the rotation"):
+        llm_import.analyze(build_llama(SMALL, llama.random_float_state(SMALL, seed=1, std=0.05)))
+
+
+def test_rotations_and_epsilons_that_differ_are_refused(monkeypatch):
+    state = llama.random_float_state(SMALL.with_(qk_norm=True), seed=1, std=0.05)
+    rope, rms, calls = ov_builders._rope, ov_builders._rms, []
+
+    def other(x, c, s, D):
+        calls.append(1)
+        f = ov_builders.constant(np.array(1.0 if len(calls) <= 2 else 1.5, dtype=np.float32))           # the second layer's cos and sin
+        return rope(x, ov_builders.ops.multiply(c, f).output(0), ov_builders.ops.multiply(s, f).output(0), D)
+    with monkeypatch.context() as m:
+        m.setattr(ov_builders, "_rope", other)
+        with pytest.raises(llm_import.NotAnLlm, match="rotations that differ"):
+            llm_import.analyze(build_llama(SMALL, state))
+    monkeypatch.setattr(ov_builders, "_rms", lambda x, g, eps, name: rms(x, g, 1e-3 if name.endswith("k_norm") else eps, name))
+    with pytest.raises(llm_import.NotAnLlm, match="epsilon"):
+        llm_import.analyze(build_llama(SMALL.with_(qk_norm=True), state))
 
 
 def test_plain_decoders_keep_their_configuration():
@@ -137,6 +184,7 @@ EXECUTORS = {
     "head_norms": (dict(qk_norm=True, weight_format="bf16"), BF16_LOGITS),
     "interleaved": (dict(rope_interleaved=True, rotary_dim=64, weight_format="int4"), BF16_LOGITS),
     "scaled_norms_int4": (dict(qk_norm=True, rope_inv_freq=SCALED), BF16_LOGITS),
+    "scaled_turns": (dict(rope_scale=1.25, rope_inv_freq=SCALED, weight_format="bf16"), BF16_LOGITS),
     "int8": (dict(weight_format="int8", int8_activations=True, group_size=0), INT8_LOGITS),
     "int8_head_norms": (dict(weight_format="int8", int8_activations=True, group_size=0, qk_norm=True, qk_norm_eps=1e-6), INT8_LOGITS),
 }
