@@ -409,6 +409,7 @@ def _one_device(first: torch.Tensor, *others) -> int:
     for t in others:
         if t is not None and t.get_device() != d:
             d = -1
+            break
     if d < 0:
         raise ValueError("the operands have to be on one CUDA device")
     return d
@@ -1116,15 +1117,14 @@ def rope_kv_write_u8(qkv, positions, slot_map, k_cache, v_cache, k_meta, v_meta,
 
 def _rope_operands(dtype, D, inv_freq, q_norm, k_norm) -> int:
     """Checks what both forms share; the dimensions that turn."""
-    if dtype != torch.bfloat16 and dtype != torch.float16:
+    if dtype is not torch.float16 and dtype is not torch.bfloat16:
         raise ValueError("bf16 or fp16 heads are expected, not %s" % dtype)
     rot = 2 * inv_freq.numel()
-    if inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous() or rot > D:
+    if inv_freq.dtype is not torch.float32 or rot > D or not inv_freq.is_contiguous():
         raise ValueError("frequencies are fp32, one for each pair of at most %d dimensions" % D)
-    if q_norm is not None and not (q_norm.dtype == dtype and q_norm.numel() == D and q_norm.is_contiguous()):
-        raise ValueError("a head norm has %d weights of the heads' type" % D)
-    if k_norm is not None and not (k_norm.dtype == dtype and k_norm.numel() == D and k_norm.is_contiguous()):
-        raise ValueError("a head norm has %d weights of the heads' type" % D)
+    for w in (q_norm, k_norm):
+        if w is not None and (w.dtype is not dtype or w.numel() != D or not w.is_contiguous()):
+            raise ValueError("a head norm has %d weights of the heads' type" % D)
     return rot
 
 
@@ -1145,38 +1145,44 @@ def qk_norm_rope(q, k, positions, inv_freq, q_norm=None, k_norm=None, eps=1e-6, 
     q [B, S, Hq, D] and k [B, S, Hkv, D], bf16 or fp16 (or [S, H, D]): views with any strides whose heads are contiguous; ``positions`` int32 [B, S] or [S].
     The first 2 * len(``inv_freq``) dimensions turn by positions * inv_freq (fp32; the product is formed in 64 bits), halves paired, or neighbours with
     ``interleaved``; cos and sin are multiplied by ``mult``. The outputs may be q and k themselves."""
-    if q.dim() == 3:
+    if q.ndim == 3:
         _need(k.dim() == 3 and positions.dim() == 1, "queries [S, H, D] need keys of that form and positions [S]")
         outs = qk_norm_rope(q[None], k[None], positions, inv_freq, q_norm, k_norm, eps, interleaved, mult, None if q_out is None else q_out[None],
                             None if k_out is None else k_out[None])
         return outs[0][0], outs[1][0]
-    dtype = q.dtype
-    if q.dim() != 4 or k.dim() != 4 or k.dtype != dtype:
+    dtype, shape, kshape = q.dtype, q.shape, k.shape
+    if len(shape) != 4 or len(kshape) != 4 or k.dtype is not dtype:
         raise ValueError("queries [B, S, Hq, D] and keys [B, S, Hkv, D] of one type are expected")
-    (B, S, Hq, D), (kB, kS, Hkv, kD) = q.shape, k.shape
+    B, S, Hq, D = shape
+    kB, kS, Hkv, kD = kshape
     if not (kB == B and kS == S and kD == D and Hq > 0 and Hkv > 0 and D > 0):
-        raise ValueError("queries [B, S, Hq, D] and keys [B, S, Hkv, D] are expected, not %s and %s" % (tuple(q.shape), tuple(k.shape)))
-    many = positions.dim() == 2
-    if positions.dtype != torch.int32 or positions.shape != ((B, S) if many else (S,)) or (S != 1 and positions.stride(-1) != 1):
+        raise ValueError("queries [B, S, Hq, D] and keys [B, S, Hkv, D] are expected, not %s and %s" % (tuple(shape), tuple(kshape)))
+    steps = positions.stride()
+    many = len(steps) == 2
+    if positions.dtype is not torch.int32 or positions.shape != ((B, S) if many else (S,)) or (steps[-1] != 1 and S != 1):
         raise ValueError("positions are int32 [S] or [B, S]")
     rot = _rope_operands(dtype, D, inv_freq, q_norm, k_norm)
     if q_out is not None or k_out is not None:
         for t, like in ((q_out, q), (k_out, k)):
-            if t is not None and not (t.shape == like.shape and t.dtype == dtype and _written_once(t)):
+            if t is not None and not (t.shape == like.shape and t.dtype is dtype and _written_once(t)):
                 raise ValueError("outputs have their inputs' shape and type, and no two elements in one place")
     d = _one_device(q, k, positions, inv_freq, q_norm, k_norm, q_out, k_out)
+    # (like a contiguous tensor takes less of the host than from its sizes)
     if q_out is None:
-        q_out = q.new_empty((B, S, Hq, D))
+        q_out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((B, S, Hq, D))
     if k_out is None:
-        k_out = k.new_empty((B, S, Hkv, D))
-    qs, ks, qo, ko = q.stride(), k.stride(), q_out.stride(), k_out.stride()
-    if not (qs[3] == 1 and ks[3] == 1 and qo[3] == 1 and ko[3] == 1):
+        k_out = torch.empty_like(k) if k.is_contiguous() else k.new_empty((B, S, Hkv, D))
+    q0, q1, q2, q3 = q.stride()
+    k0, k1, k2, k3 = k.stride()
+    qo0, qo1, qo2, qo3 = q_out.stride()
+    ko0, ko1, ko2, ko3 = k_out.stride()
+    if not (q3 == k3 == qo3 == ko3 == 1):
         raise ValueError("heads have to be contiguous")
     if B * S:
         _call(lib().ovb_qk_norm_rope, _QK_ROPE.pack(q.data_ptr(), k.data_ptr(), 0, q_out.data_ptr(), k_out.data_ptr(), 0, 0, 0, 0, positions.data_ptr(), 0, inv_freq.data_ptr(),
-                                                    0 if q_norm is None else q_norm.data_ptr(), 0 if k_norm is None else k_norm.data_ptr(), qs[0], qs[1], qs[2], ks[0], ks[1], ks[2],
-                                                    0, 0, 0, qo[0], qo[1], qo[2], ko[0], ko[1], ko[2], positions.stride(0) if many else 0, 0, B, S, Hq, Hkv, D, rot, 0,
-                                                    bool(interleaved), dtype == torch.float16, 0, eps, mult), d, "ovb_qk_norm_rope")
+                                                    0 if q_norm is None else q_norm.data_ptr(), 0 if k_norm is None else k_norm.data_ptr(), q0, q1, q2, k0, k1, k2,
+                                                    0, 0, 0, qo0, qo1, qo2, ko0, ko1, ko2, steps[0] if many else 0, 0, B, S, Hq, Hkv, D, rot, 0,
+                                                    1 if interleaved else 0, dtype is torch.float16, 0, eps, mult), d, "ovb_qk_norm_rope")
     return q_out, k_out
 
 
@@ -1189,16 +1195,18 @@ def qk_norm_rope_kv_write(qkv, positions, slot_map, k_cache, v_cache, inv_freq, 
     the fp16 (scale, zero point) tables ``k_meta`` / ``v_meta`` [num_blocks, Hkv, block_size, 2] (D and the rotation multiples of 8, D up to 256).
     A slot behind the cache is not written and shows in the status word."""
     dtype, cache_type = qkv.dtype, k_cache.dtype
-    u8 = cache_type == torch.uint8
-    width = (Hq + 2 * Hkv) * D
-    if qkv.dim() != 2 or Hq <= 0 or Hkv <= 0 or D <= 0 or block_size <= 0 or qkv.shape[1] < width or qkv.stride(1) != 1:
-        raise ValueError("rows [T, %d] with their values side by side are expected, not %s" % (width, tuple(qkv.shape)))
-    T, pitch = qkv.shape[0], qkv.stride(0)
-    if not (positions.dtype == slot_map.dtype == torch.int32 and positions.dim() == slot_map.dim() == 1 and positions.numel() >= T and slot_map.numel() >= T
+    u8 = cache_type is torch.uint8
+    queries, width = Hq * D, (Hq + 2 * Hkv) * D
+    shape, pitches = qkv.shape, qkv.stride()
+    if len(shape) != 2 or Hq <= 0 or Hkv <= 0 or D <= 0 or block_size <= 0 or shape[1] < width or pitches[1] != 1:
+        raise ValueError("rows [T, %d] with their values side by side are expected, not %s" % (width, tuple(shape)))
+    T, pitch = shape[0], pitches[0]
+    if not (positions.dtype is slot_map.dtype is torch.int32 and positions.ndim == slot_map.ndim == 1 and positions.numel() >= T and slot_map.numel() >= T
             and positions.is_contiguous() and slot_map.is_contiguous()):
         raise ValueError("positions and slots are int32, %d values at least" % T)
-    blocks, form = k_cache.shape[0], k_cache.shape
-    if not (form[1:] == (Hkv, block_size, D) and v_cache.shape == form and cache_type == v_cache.dtype == (torch.uint8 if u8 else dtype) and k_cache.is_contiguous()
+    form = k_cache.shape
+    blocks = form[0]
+    if not (form[1:] == (Hkv, block_size, D) and v_cache.shape == form and (u8 or cache_type is dtype) and v_cache.dtype is cache_type and k_cache.is_contiguous()
             and v_cache.is_contiguous()):
         raise ValueError("caches are contiguous [num_blocks, %d, %d, %d] of the type of qkv, or uint8" % (Hkv, block_size, D))
     if u8:
@@ -1209,17 +1217,19 @@ def qk_norm_rope_kv_write(qkv, positions, slot_map, k_cache, v_cache, inv_freq, 
     if q_out is None:
         if T > 1 and pitch < width:
             raise ValueError("rows that are written in place must not overlap")
-        q_out = qkv
-    elif not (q_out.dim() == 2 and q_out.shape[0] == T and q_out.shape[1] >= Hq * D and q_out.stride(1) == 1 and q_out.dtype == dtype and (T <= 1 or q_out.stride(0) >= Hq * D)):
-        raise ValueError("q_out has to be [%d, %d] of the type of qkv" % (T, Hq * D))
-    d = _one_device(qkv, positions, slot_map, k_cache, v_cache, inv_freq, q_norm, k_norm, q_out, *((k_meta, v_meta) if u8 else ()))
+        q_out, q_pitch = qkv, pitch
+    else:
+        oshape, (q_pitch, step) = q_out.shape, q_out.stride() if q_out.ndim == 2 else (0, 0)
+        if not (step == 1 and oshape[0] == T and oshape[1] >= queries and q_out.dtype is dtype and (q_pitch >= queries or T <= 1)):
+            raise ValueError("q_out has to be [%d, %d] of the type of qkv" % (T, queries))
+    d = _one_device(qkv, positions, slot_map, k_cache, v_cache, inv_freq, q_norm, k_norm, q_out, k_meta if u8 else None, v_meta if u8 else None)
     if T:
-        at, head = qkv.data_ptr(), D * 2
-        _call(lib().ovb_qk_norm_rope, _QK_ROPE.pack(at, at + Hq * head, at + (Hq + Hkv) * head, q_out.data_ptr(), 0, k_cache.data_ptr(), v_cache.data_ptr(), k_meta.data_ptr() if u8 else 0,
-                                                    v_meta.data_ptr() if u8 else 0, positions.data_ptr(), slot_map.data_ptr(), inv_freq.data_ptr(),
+        at = qkv.data_ptr()
+        _call(lib().ovb_qk_norm_rope, _QK_ROPE.pack(at, at + queries * 2, at + (Hq + Hkv) * D * 2, q_out.data_ptr(), 0, k_cache.data_ptr(), v_cache.data_ptr(),
+                                                    k_meta.data_ptr() if u8 else 0, v_meta.data_ptr() if u8 else 0, positions.data_ptr(), slot_map.data_ptr(), inv_freq.data_ptr(),
                                                     0 if q_norm is None else q_norm.data_ptr(), 0 if k_norm is None else k_norm.data_ptr(), 0, pitch, D, 0, pitch, D, 0, pitch, D,
-                                                    0, q_out.stride(0), D, 0, 0, 0, 0, blocks * block_size, 1, T, Hq, Hkv, D, rot, block_size, bool(interleaved),
-                                                    dtype == torch.float16, u8, eps, mult), d, "ovb_qk_norm_rope")
+                                                    0, q_pitch, D, 0, 0, 0, 0, blocks * block_size, 1, T, Hq, Hkv, D, rot, block_size, 1 if interleaved else 0,
+                                                    dtype is torch.float16, u8, eps, mult), d, "ovb_qk_norm_rope")
 
 
 def paged_attention(q, k_cache, v_cache, past_lens, subsequence_begins, block_indices, block_indices_begins, Hq, Hkv, D,
