@@ -32,7 +32,9 @@ struct I8TileParams : I8Params {
 };
 
 // The row of a single token, quantised by eight warps into the swizzled operand of the MMA ([k-block][16 rows][128 bytes]; the other rows are not set,
-// their sums are not read). Every CTA needs the largest magnitude of the whole row, so it reads it whole, and keeps the codes of its k-blocks.
+// their sums are not read). Every CTA needs the largest magnitude of the whole row, so it reads it whole, and keeps the codes of its k-blocks. The loops stop
+// behind the last piece in use: with all eight worked through whatever K is, the arithmetic of empty pieces took more than the row's own (1 x 6144 x 4096 with
+// a norm 13.2 us, 7.0 without them).
 template <class E>
 __device__ __forceinline__ void i8_quantize_row(const I8TileParams& p, uint8_t* codes, int kb0, int kb1, float* row_scale, int* row_sum, float* box_f, uint32_t* box_u, int* box_i) {
     constexpr int SPAN = kI8QuantWarps * 32;
@@ -47,6 +49,7 @@ __device__ __forceinline__ void i8_quantize_row(const I8TileParams& p, uint8_t* 
     const uint4* src = reinterpret_cast<const uint4*>(static_cast<const E*>(p.raw) + row * p.ld_raw);
 #pragma unroll
     for (int h = 0; h < kI8Hold; ++h) {
+        if (h * SPAN >= pieces) break;
         const int at = tid + h * SPAN;
         x[h] = at < pieces ? __ldcg(src + at) : make_uint4(0, 0, 0, 0);
         g[h] = p.gamma != nullptr && at < pieces ? __ldg(static_cast<const uint4*>(p.gamma) + at) : make_uint4(0, 0, 0, 0);
@@ -57,6 +60,7 @@ __device__ __forceinline__ void i8_quantize_row(const I8TileParams& p, uint8_t* 
     uint64_t ss2 = pair_of(0.f);
 #pragma unroll
     for (int h = 0; h < kI8Hold; ++h) {
+        if (h * SPAN >= pieces) break;
         float v[8];
         if (norm) {
             row_values<E, true>(x[h], g[h], v);
@@ -90,6 +94,7 @@ __device__ __forceinline__ void i8_quantize_row(const I8TileParams& p, uint8_t* 
     int sum = 0;
 #pragma unroll
     for (int h = 0; h < kI8Hold; ++h) {
+        if (h * SPAN >= pieces) break;
         const int at = tid + h * SPAN, kb = at >> 4;
         const bool mine = kb >= kb0 && kb < kb1;
         if (at >= pieces || (!mine && p.w_zp == nullptr)) continue;
@@ -382,14 +387,17 @@ static int launch_i8_tile(int form, const cudaLaunchConfig_t& cfg, const CUtenso
     }
 }
 
-// A single token's row is quantised by the product's kernel: whole aligned pieces of eight columns, as many as eight warps hold. (us with a norm, one launch / two:
-// 1 x 6144 x 4096 9.6 / 9.8, where the second launch also costs the host 2.5. With four rows the kernel's own way costs more than it saves: 4 x 4096 x 4096
-// 10.2 / 8.3.) Every CTA reads the whole row at a time of its own, so a result in the row's place has it quantised first, by a launch of its own.
+// A single token's row is quantised by the product's kernel: whole aligned pieces of eight columns, as many as eight warps hold. us with a norm, one launch / two
+// (whose second also costs the host 2.5): 1024 x 1024 3.9 / 5.3, 6144 x 4096 6.9 / 9.8, 14336 x 4096 11.3 / 13.5, 4096 x 14336 13.7 / 14.0; with larger
+// weights the CTAs that follow on an SM each quantise the row again: 10240 x 8192 20.3 / 18.4, 28672 x 4096 23.7 / 22.6, 128256 x 4096 86.5 / 79.1. More rows
+// take a microsecond each, one behind the other (4 x 4096 x 4096 10.5 / 8.5).
+// Every CTA reads the whole row at a time of its own, so a result in the row's place has it quantised first, by a launch of its own.
+constexpr int64_t kI8FusedWeights = 64 << 20;       // bytes
 static bool i8_fuses(const ovb_gemm_i8_args* a) {
     const auto bits = [](const void* x) { return reinterpret_cast<uintptr_t>(x); };
     const uintptr_t rows = a->row_idx != nullptr ? ((uintptr_t)(a->raw_rows - 1) * (uintptr_t)a->ld_raw + (uintptr_t)a->K) * 2 : (uintptr_t)a->K * 2;
     const bool apart = bits(a->out) >= bits(a->raw) + rows || bits(a->raw) >= bits(a->out) + (uintptr_t)a->N * 4;
-    return apart && a->raw != nullptr && a->T == 1 && a->K % 8 == 0 && a->K <= kI8QuantWarps * 32 * kI8Hold * 8 && (a->row_idx == nullptr || a->ld_raw % 8 == 0) &&
+    return apart && a->raw != nullptr && a->T == 1 && (int64_t)a->N * a->K <= kI8FusedWeights && a->K % 8 == 0 && a->K <= kI8QuantWarps * 32 * kI8Hold * 8 && (a->row_idx == nullptr || a->ld_raw % 8 == 0) &&
            ((bits(a->raw) | bits(a->gamma)) & 15) == 0;
 }
 
@@ -405,7 +413,7 @@ struct I8Plan {
 //    products, the bytes that an SM takes (both shared by the CTAs of an SM) or the latency that its stages hide, whichever is longest; the exchange of
 //    partial sums; never less than the weights take from memory
 //  * pairs: waves of 256 x 256 tiles
-// us, 1 x 6144 x 4096 7.1; 64 x 28672 x 4096 21.6 (pairs 26.7); 256 x 28672 x 4096 39.5, pairs 30.2; 512 x 4096 x 4096 13.3, pairs 15.0; 999 x 8192 x 8192
+// us, 1 x 6144 x 4096 6.9; 64 x 28672 x 4096 21.6 (pairs 26.7); 256 x 28672 x 4096 39.5, pairs 30.2; 512 x 4096 x 4096 13.3, pairs 15.0; 999 x 8192 x 8192
 // 62.9, pairs 47.8.
 static bool i8_plan(int T, int N, int KB, bool fused, I8Plan* plan) {
     const int tiles_n = ceil_div(N, TILE_N), t16 = T > 256 ? 256 : (T + 15) / 16 * 16;
@@ -534,6 +542,7 @@ int ovb_gemm_i8(const ovb_gemm_i8_args* a, ovb_stream_t stream_) {
     OVB_REQUIRE(a->residual == nullptr || !a->out_f32, "ovb_gemm_i8: a residual belongs to a 16-bit output");
     const int cols = gated ? a->N / 2 : a->N;
     OVB_REQUIRE(a->ldo >= cols && (a->residual == nullptr || a->ldr >= cols), "ovb_gemm_i8: row pitch of the output %d or residual %d below %d columns", a->ldo, a->ldr, cols);
+    OVB_REQUIRE(a->raw == nullptr || (a->ld_raw >= 0 && (a->row_idx == nullptr || a->raw_rows > 0)), "ovb_gemm_i8: row indices need the number of rows, rows their pitch");
     I8Plan plan;
     const int KB = ceil_div(a->K, kI8BlockK);
     const bool fused = i8_fuses(a) && i8_plan(a->T, a->N, KB, true, &plan);
