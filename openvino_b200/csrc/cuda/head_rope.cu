@@ -8,8 +8,9 @@
 // 4e-3 off, more than a bf16 rounding of the result. The angles of a token are the same for all heads: a block computes them once, in shared
 // memory, while its first heads are on their way. Sums, norms and rotation are held in 32 bits, every result is rounded once.
 //
-// What bounds it: memory, each head read and written once. A lane holds two pieces of a head: the partner of a
-// dimension is in the same lane, and the lanes of a head need shuffles for the sum of squares only.
+// What bounds it: memory, each head read and written once; next to it the instructions, about 250 for a warp's round of four heads of 128. A lane holds two
+// pieces of a head: the partner of a dimension is in the same lane, and the lanes of a head need shuffles for the sum of squares only. Measured: 8 x 1024 tokens
+// of 64 + 8 + 8 heads of 128 into a 16-bit cache 60.7 us (5.5 TB/s), 4 x 2048 tokens of 32 + 8 heads, half of each turned 32.2 us (5.2 TB/s), 1 token 2.8 us.
 #include "gemm_common.cuh"
 
 namespace ovb {
@@ -18,13 +19,18 @@ struct HeadRopeParams : ovb_qk_rope_args {
     int* status;
     int src_step[3], dst_step[3]; // from head to head, queries, keys, values: elements, bytes
     int heads;                    // of a token, all kinds
-    int parts, per_warp;          // warps of a token and their heads
+    int rounds_q, rounds_k, rounds;                     // of a warp over the query heads, the key heads, all heads of a token
+    int parts, per_warp;          // warps of a token and their rounds
     float inv_d;
 };
 
 constexpr int kRopeThreads = 128;
-constexpr int kRopeBlocks = 5;    // resident on an SM
-constexpr int kRopeAhead = 2;     // rounds of heads that a warp has in flight
+// Blocks resident on an SM, and rounds of heads that a warp has in flight besides the one at work: many warps with one round each where there are tokens for
+// them, deeper warps where a token's heads are spread over warps and few rounds are left to each. us, many / few: 8 x 1024 tokens of 64 + 8 + 8 heads of 128
+// 60.7 / 71.5, 1500 tokens of 32 + 8 + 8 11.7 / 13.4, 700 tokens 7.1 / 6.0, 200 tokens 4.8 / 4.1.
+constexpr int rope_blocks(bool many) { return many ? 7 : 5; }
+constexpr int rope_ahead(bool many) { return many ? 1 : 2; }
+constexpr int kRopeManyTokens = 148 * 7;
 
 __device__ __forceinline__ float2 turn_of(int position, float inv_freq, float mult) {
     const double turns = (double)position * (double)inv_freq * 0.15915494309189533577;
@@ -96,15 +102,17 @@ struct Piece {
 };
 
 // Heads and rotations of whole pieces, aligned heads. LANES lanes share a head, each with two pieces of CH elements: the partners of its CH pairs, or 2 CH
-// neighbours. A warp works alone, on a token's heads or a part of them, with the heads of kRopeAhead rounds on their way.
-template <class E, bool INTER, int CH, int LANES, bool U8>
-__global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) head_rope_kernel(const __grid_constant__ HeadRopeParams p) {
+// neighbours. A warp works alone, on a token's heads or a part of them, with the heads of the next rounds on their way. The heads of a round are of one kind
+// (queries, keys, values), so everything that depends on the kind is the same for the warp. The norm's weights are multiplied into the cosines and sines when
+// the kind changes; values on their way to a 16-bit cache are copied as they are.
+template <class E, bool INTER, int CH, int LANES, bool U8, bool MANY>
+__global__ void __launch_bounds__(kRopeThreads, rope_blocks(MANY)) head_rope_kernel(const __grid_constant__ HeadRopeParams p) {
     __shared__ float2 turn_of_warp[kRopeThreads / 32][128];
-    constexpr int GROUPS = 32 / LANES;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int GROUPS = 32 / LANES, AHEAD = rope_ahead(MANY);
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int id = blockIdx.x * (kRopeThreads / 32) + warp, t = id / p.parts;
     const int group = lane / LANES, l = lane % LANES;
-    const int h_begin = (id - t * p.parts) * p.per_warp, h_end = min(p.heads, h_begin + p.per_warp);
+    const int begin = (id - t * p.parts) * p.per_warp, end = min(p.rounds, begin + p.per_warp);
     const bool own = l * 2 * CH < p.D;                  // this lane has elements
     const int pair0 = l * CH, half = p.rot >> 1;
     const bool turns = own && pair0 < half;
@@ -113,14 +121,19 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) head_rope_kernel(co
     pdl_enter();
     if (t >= p.B * p.S) return;                         // whole warps, which share nothing
     const TokenRows<E> rows = token_rows<E, U8>(p, t);
-    auto kind_of = [&](int h) { return h < p.Hq ? 0 : h < p.Hq + p.Hkv ? 1 : 2; };
-    auto index_of = [&](int h, int kind) { return kind == 0 ? h : kind == 1 ? h - p.Hq : h - p.Hq - p.Hkv; };
+    auto kind_of = [&](int round) { return round < p.rounds_q ? 0 : round < p.rounds_q + p.rounds_k ? 1 : 2; };
+    // this lane's head of a round, among those of its kind; negative: none
+    auto head_of = [&](int round, int kind) {
+        const int h = (round - (kind == 0 ? 0 : kind == 1 ? p.rounds_q : p.rounds_q + p.rounds_k)) * GROUPS + group;
+        return own && h < (kind == 0 ? p.Hq : p.Hkv) ? h : -1;
+    };
     auto pick = [&](const auto& of, int kind) { return kind == 0 ? of[0] : kind == 1 ? of[1] : of[2]; };
-    Piece<E, CH> r0[kRopeAhead], r1[kRopeAhead];
-    auto fetch = [&](int h, Piece<E, CH>& a, Piece<E, CH>& c) {
-        if (h < h_end && own) {
-            const int kind = kind_of(h);
-            const E* src = pick(rows.src, kind) + (int64_t)index_of(h, kind) * pick(p.src_step, kind);
+    Piece<E, CH> r0[AHEAD], r1[AHEAD];
+    auto fetch = [&](int round, Piece<E, CH>& a, Piece<E, CH>& c) {
+        if (round >= end) return;
+        const int kind = kind_of(round), h = head_of(round, kind);
+        if (h >= 0) {
+            const E* src = pick(rows.src, kind) + (int64_t)h * pick(p.src_step, kind);
             a.load(src + o0);
             c.load(src + o1);
         } else {
@@ -129,86 +142,115 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) head_rope_kernel(co
         }
     };
 #pragma unroll
-    for (int i = 0; i < kRopeAhead; ++i) fetch(h_begin + i * GROUPS + group, r0[i], r1[i]);
+    for (int i = 0; i < AHEAD; ++i) fetch(begin + i, r0[i], r1[i]);
     float2* turn = turn_of_warp[warp];
     const int position = p.positions[(t / p.S) * p.pos_batch + t % p.S];
     for (int i = lane; i < half; i += 32) turn[i] = turn_of(position, p.inv_freq[i], p.mult);
     __syncwarp();
     if (rows.outside && lane == 0) report_status(p.status, STATUS_BAD_INDEX);
-    float cs[CH], sn[CH];
+    // of an element and of its partner, in the first and in the second piece; the weights alone where nothing turns
+    float fa[CH], ga[CH], fc[CH], gc[CH];
+    const E* weight = nullptr;
+    auto factors = [&](int kind) {
+        weight = static_cast<const E*>(kind == 0 ? p.q_norm : p.k_norm);
 #pragma unroll
-    for (int j = 0; j < CH; ++j) {
-        const float2 u = turns ? turn[pair0 + j] : make_float2(1.f, 0.f);
-        cs[j] = u.x;
-        sn[j] = u.y;
-    }
-    for (int base = h_begin; base < h_end; base += GROUPS * kRopeAhead) {
+        for (int j = 0; j < CH; ++j) fa[j] = fc[j] = 1.f;
+        if (weight != nullptr && own) {
+            Piece<E, CH> w0, w1;
+            w0.load(weight + o0);
+            w1.load(weight + o1);
+            w0.unpack(fa);
+            w1.unpack(fc);
+        }
+        if (!turns) return;
 #pragma unroll
-        for (int i = 0; i < kRopeAhead; ++i) {
-            const int h = base + i * GROUPS + group;
-            if (base + i * GROUPS >= h_end) break;      // the same for the whole warp
-            const bool live = h < h_end && own;
-            const int kind = kind_of(h);
+        for (int j = 0; j < CH; ++j) {
+            if (INTER) {
+                if (j % 2) continue;
+                const float2 u = turn[pair0 + j / 2], v = turn[pair0 + (CH + j) / 2];
+                const float a0 = fa[j], a1 = fa[j + 1], c0 = fc[j], c1 = fc[j + 1];
+                fa[j] = a0 * u.x;
+                ga[j] = -a1 * u.y;
+                fa[j + 1] = a1 * u.x;
+                ga[j + 1] = a0 * u.y;
+                fc[j] = c0 * v.x;
+                gc[j] = -c1 * v.y;
+                fc[j + 1] = c1 * v.x;
+                gc[j + 1] = c0 * v.y;
+            } else {
+                const float2 u = turn[pair0 + j];
+                ga[j] = -fc[j] * u.y;
+                gc[j] = fa[j] * u.y;
+                fa[j] *= u.x;
+                fc[j] *= u.x;
+            }
+        }
+    };
+    int current = -1;
+    for (int base = begin; base < end; base += AHEAD) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const int round = base + i;
+            if (round >= end) break;
+            const int kind = kind_of(round), h = head_of(round, kind);
+            Piece<E, CH> x0 = r0[i], x1 = r1[i];
+            fetch(round + AHEAD, r0[i], r1[i]);
+            uint8_t* dst = h >= 0 ? pick(rows.dst, kind) : nullptr;
+            if (dst != nullptr) dst += (int64_t)h * pick(p.dst_step, kind);
             float a[CH], c[CH];
-            r0[i].unpack(a);
-            r1[i].unpack(c);
-            fetch(h + kRopeAhead * GROUPS, r0[i], r1[i]);
-            if (p.q_norm != nullptr || p.k_norm != nullptr) {
-                uint64_t ss2 = pair_of(0.f);
+            if (kind != 2) {
+                if (kind != current) factors(current = kind);
+                x0.unpack(a);
+                x1.unpack(c);
+                if (weight != nullptr) {
+                    uint64_t ss2 = pair_of(0.f);
 #pragma unroll
-                for (int j = 0; j < CH; j += 2) ss2 = fma2(pair_of(a[j], a[j + 1]), pair_of(a[j], a[j + 1]), fma2(pair_of(c[j], c[j + 1]), pair_of(c[j], c[j + 1]), ss2));
-                float ss, ss1;
-                unpair(ss2, ss, ss1);
-                ss += ss1;
+                    for (int j = 0; j < CH; j += 2) ss2 = fma2(pair_of(a[j], a[j + 1]), pair_of(a[j], a[j + 1]), fma2(pair_of(c[j], c[j + 1]), pair_of(c[j], c[j + 1]), ss2));
+                    float ss, ss1;
+                    unpair(ss2, ss, ss1);
+                    ss += ss1;
 #pragma unroll
-                for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                const E* weight = static_cast<const E*>(kind == 0 ? p.q_norm : kind == 1 ? p.k_norm : nullptr);
-                if (weight != nullptr && own) {
-                    const float inv = rsqrtf(fmaf(ss, p.inv_d, p.eps));
-                    Piece<E, CH> w0, w1;                // the same lines for all heads: they stay in L1 (held in registers they are spilled)
-                    float wa[CH], wc[CH];
-                    w0.load(weight + o0);
-                    w1.load(weight + o1);
-                    w0.unpack(wa);
-                    w1.unpack(wc);
+                    for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                    const uint64_t inv = pair_of(rsqrtf(fmaf(ss, p.inv_d, p.eps)));
 #pragma unroll
                     for (int j = 0; j < CH; j += 2) {
-                        unpair(mul2(mul2(pair_of(a[j], a[j + 1]), pair_of(inv)), pair_of(wa[j], wa[j + 1])), a[j], a[j + 1]);
-                        unpair(mul2(mul2(pair_of(c[j], c[j + 1]), pair_of(inv)), pair_of(wc[j], wc[j + 1])), c[j], c[j + 1]);
+                        unpair(mul2(pair_of(a[j], a[j + 1]), inv), a[j], a[j + 1]);
+                        unpair(mul2(pair_of(c[j], c[j + 1]), inv), c[j], c[j + 1]);
                     }
                 }
-            }
-            if (turns && kind != 2) {
-                if (INTER) {
+                if (turns) {
 #pragma unroll
                     for (int j = 0; j < CH; j += 2) {
-                        const float a0 = a[j], c0 = c[j];
-                        a[j] = a0 * cs[j / 2] - a[j + 1] * sn[j / 2];
-                        a[j + 1] = a[j + 1] * cs[j / 2] + a0 * sn[j / 2];
-                        c[j] = c0 * cs[(CH + j) / 2] - c[j + 1] * sn[(CH + j) / 2];
-                        c[j + 1] = c[j + 1] * cs[(CH + j) / 2] + c0 * sn[(CH + j) / 2];
+                        if (INTER) {
+                            const float a0 = a[j], c0 = c[j];
+                            a[j] = fmaf(a[j + 1], ga[j], a0 * fa[j]);
+                            a[j + 1] = fmaf(a0, ga[j + 1], a[j + 1] * fa[j + 1]);
+                            c[j] = fmaf(c[j + 1], gc[j], c0 * fc[j]);
+                            c[j + 1] = fmaf(c0, gc[j + 1], c[j + 1] * fc[j + 1]);
+                        } else {
+                            const uint64_t a2 = pair_of(a[j], a[j + 1]), c2 = pair_of(c[j], c[j + 1]);
+                            unpair(fma2(c2, pair_of(ga[j], ga[j + 1]), mul2(a2, pair_of(fa[j], fa[j + 1]))), a[j], a[j + 1]);
+                            unpair(fma2(a2, pair_of(gc[j], gc[j + 1]), mul2(c2, pair_of(fc[j], fc[j + 1]))), c[j], c[j + 1]);
+                        }
                     }
                 } else {
 #pragma unroll
-                    for (int j = 0; j < CH; j += 2) {
-                        const uint64_t a2 = pair_of(a[j], a[j + 1]), c2 = pair_of(c[j], c[j + 1]), co = pair_of(cs[j], cs[j + 1]), si = pair_of(sn[j], sn[j + 1]);
-                        unpair(fma2(c2, pair_of(-sn[j], -sn[j + 1]), mul2(a2, co)), a[j], a[j + 1]);
-                        unpair(fma2(a2, si, mul2(c2, co)), c[j], c[j + 1]);
+                    for (int j = 0; j < CH; ++j) {
+                        a[j] *= fa[j];
+                        c[j] *= fc[j];
                     }
                 }
+                x0.pack(a);
+                x1.pack(c);
+            } else if (U8) {
+                x0.unpack(a);
+                x1.unpack(c);
             }
-            uint8_t* dst = live ? pick(rows.dst, kind) : nullptr;
-            if (dst != nullptr) dst += (int64_t)index_of(h, kind) * pick(p.dst_step, kind);
-            if (!U8 || kind == 0) {
-                if (dst != nullptr) {
-                    Piece<E, CH> w0, w1;
-                    w0.pack(a);
-                    w1.pack(c);
-                    w0.store(reinterpret_cast<E*>(dst) + o0);
-                    w1.store(reinterpret_cast<E*>(dst) + o1);
-                }
+            if ((!U8 || kind == 0) && dst != nullptr) {
+                x0.store(reinterpret_cast<E*>(dst) + o0);
+                x1.store(reinterpret_cast<E*>(dst) + o1);
             }
-            if (U8) {
+            if (U8 && kind != 0) {
                 // the arithmetic of ovb_rope_kv_write_u8: the pair is stored as fp16, so rows are quantised with the values that the reader will see
                 float mn = INFINITY, mx = -INFINITY;
                 if (own) {
@@ -223,7 +265,7 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) head_rope_kernel(co
                     mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
                 }
-                if (dst != nullptr && kind != 0) {
+                if (dst != nullptr) {
                     float scale = __half2float(__float2half_rn((mx - mn) * (1.0f / 255.0f)));
                     if (!(scale > 0.f)) scale = 1.0f;
                     const float zp = __half2float(__float2half_rn(-mn / scale));
@@ -239,7 +281,7 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) head_rope_kernel(co
                         reinterpret_cast<uint32_t*>(dst + o0)[j] = w0[j];
                         reinterpret_cast<uint32_t*>(dst + o1)[j] = w1[j];
                     }
-                    if (l == 0) static_cast<__half2*>(kind == 2 ? p.v_meta : p.k_meta)[rows.row + (int64_t)index_of(h, kind) * p.block_size] = __floats2half2_rn(scale, zp);
+                    if (l == 0) static_cast<__half2*>(kind == 2 ? p.v_meta : p.k_meta)[rows.row + (int64_t)h * p.block_size] = __floats2half2_rn(scale, zp);
                 }
             }
         }
@@ -286,20 +328,26 @@ __global__ void __launch_bounds__(kRopeThreads) head_rope_any_kernel(const __gri
     }
 }
 
-template <class E, bool INTER, int CH, bool U8>
+template <class E, bool INTER, int CH, bool U8, bool MANY>
 static cudaError_t run_head_rope(const HeadRopeParams& p, dim3 grid, int lanes, cudaStream_t stream) {
     constexpr int FEW = 32 / CH;
-    auto kern = lanes == FEW ? head_rope_kernel<E, INTER, CH, FEW, U8> : lanes == 2 * FEW ? head_rope_kernel<E, INTER, CH, 2 * FEW, U8> : head_rope_kernel<E, INTER, CH, 4 * FEW, U8>;
+    auto kern = lanes == FEW       ? head_rope_kernel<E, INTER, CH, FEW, U8, MANY>
+                : lanes == 2 * FEW ? head_rope_kernel<E, INTER, CH, 2 * FEW, U8, MANY>
+                                   : head_rope_kernel<E, INTER, CH, 4 * FEW, U8, MANY>;
     return launch_pdl(kern, grid, dim3(kRopeThreads), 0, stream, p);
 }
+template <class E, bool INTER, int CH, bool U8>
+static cudaError_t run_head_rope(const HeadRopeParams& p, dim3 grid, int lanes, bool many, cudaStream_t stream) {
+    return many ? run_head_rope<E, INTER, CH, U8, true>(p, grid, lanes, stream) : run_head_rope<E, INTER, CH, U8, false>(p, grid, lanes, stream);
+}
 template <class E, bool INTER>
-static cudaError_t run_head_rope(const HeadRopeParams& p, dim3 grid, int ch, int lanes, cudaStream_t stream) {
-    if (ch == 8) return p.kv_u8 ? run_head_rope<E, INTER, 8, true>(p, grid, lanes, stream) : run_head_rope<E, INTER, 8, false>(p, grid, lanes, stream);
-    return p.kv_u8 ? run_head_rope<E, INTER, 4, true>(p, grid, lanes, stream) : run_head_rope<E, INTER, 4, false>(p, grid, lanes, stream);
+static cudaError_t run_head_rope(const HeadRopeParams& p, dim3 grid, int ch, int lanes, bool many, cudaStream_t stream) {
+    if (ch == 8) return p.kv_u8 ? run_head_rope<E, INTER, 8, true>(p, grid, lanes, many, stream) : run_head_rope<E, INTER, 8, false>(p, grid, lanes, many, stream);
+    return p.kv_u8 ? run_head_rope<E, INTER, 4, true>(p, grid, lanes, many, stream) : run_head_rope<E, INTER, 4, false>(p, grid, lanes, many, stream);
 }
 template <class E>
-static cudaError_t run_head_rope(const HeadRopeParams& p, dim3 grid, int ch, int lanes, cudaStream_t stream) {
-    return p.interleaved ? run_head_rope<E, true>(p, grid, ch, lanes, stream) : run_head_rope<E, false>(p, grid, ch, lanes, stream);
+static cudaError_t run_head_rope(const HeadRopeParams& p, dim3 grid, int ch, int lanes, bool many, cudaStream_t stream) {
+    return p.interleaved ? run_head_rope<E, true>(p, grid, ch, lanes, many, stream) : run_head_rope<E, false>(p, grid, ch, lanes, many, stream);
 }
 
 }  // namespace ovb
@@ -343,14 +391,18 @@ extern "C" int ovb_qk_norm_rope(const ovb_qk_rope_args* a, ovb_stream_t stream_)
         return 0;
     }
     // parts of a token's heads: as many as rounds while all warps are resident at a time, fewer with more tokens
-    const int lanes = (a->D <= 64 ? 32 : a->D <= 128 ? 64 : 128) / ch, groups = 32 / lanes, rounds = ceil_div(p.heads, groups);
-    const int64_t room = 148ll * kRopeBlocks * (kRopeThreads / 32);
+    const int lanes = (a->D <= 64 ? 32 : a->D <= 128 ? 64 : 128) / ch, groups = 32 / lanes;
+    p.rounds_q = ceil_div(a->Hq, groups);
+    p.rounds_k = ceil_div(a->Hkv, groups);
+    p.rounds = p.rounds_q + p.rounds_k * (cache ? 2 : 1);
+    const bool many = tokens >= kRopeManyTokens;
+    const int64_t room = 148ll * rope_blocks(many) * (kRopeThreads / 32);
     int parts = (int)(room / tokens);
-    parts = parts < 1 ? 1 : parts > rounds ? rounds : parts;
-    p.per_warp = ceil_div(rounds, parts) * groups;
-    p.parts = ceil_div(p.heads, p.per_warp);
+    parts = parts < 1 ? 1 : parts > p.rounds ? p.rounds : parts;
+    p.per_warp = ceil_div(p.rounds, parts);
+    p.parts = ceil_div(p.rounds, p.per_warp);
     const int64_t blocks = ((int64_t)tokens * p.parts + kRopeThreads / 32 - 1) / (kRopeThreads / 32);
     OVB_REQUIRE(blocks <= INT32_MAX, "ovb_qk_norm_rope: %d tokens", tokens);
-    OVB_CHECK_CUDA(a->f16 ? run_head_rope<__half>(p, dim3((unsigned)blocks), ch, lanes, stream) : run_head_rope<__nv_bfloat16>(p, dim3((unsigned)blocks), ch, lanes, stream));
+    OVB_CHECK_CUDA(a->f16 ? run_head_rope<__half>(p, dim3((unsigned)blocks), ch, lanes, many, stream) : run_head_rope<__nv_bfloat16>(p, dim3((unsigned)blocks), ch, lanes, many, stream));
     return 0;
 }

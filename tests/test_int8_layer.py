@@ -493,6 +493,17 @@ def test_append_to_bytes(K, T, D, rot, interleaved, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("T,Hq,Hkv,D,rot", [(1036, 3, 1, 128, 128), (2300, 12, 4, 64, 32), (1500, 5, 3, 80, 40), (1200, 9, 2, 256, 64), (4700, 2, 2, 96, 96)])
+def test_many_tokens(K, T, Hq, Hkv, D, rot, interleaved, dtype):
+    """From 1036 tokens on a warp works on whole tokens, in a form of the kernel of its own."""
+    test_heads(K, 2, T // 2, Hq, Hkv, D, rot, interleaved, dtype)
+    test_append(K, T, Hq, Hkv, D, rot, 16, interleaved, D != 64, dtype)
+    test_append_to_bytes(K, T, D, rot, interleaved, dtype)
+
+
+@pytest.mark.gpu
 def test_slots_behind_the_cache_are_not_written(K):
     qkv = torch.randn((3, 4 * 64), generator=gen(1), device="cuda").bfloat16()
     big = torch.zeros((6, 1, 4, 64), dtype=torch.bfloat16, device="cuda")
