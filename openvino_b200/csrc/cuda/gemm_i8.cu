@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(i8_threads(FUSED)) gemm_i8_tile_kernel(const _
 #pragma unroll
                         for (int j = 0; j < 4; ++j) v[j] = i8_gate(p, v[j], __shfl_down_sync(0xffffffffu, v[j], 16));
                     }
-                    if (FORM == kI8Any && p.act != OVB_ACT_NONE) apply_act_n(v, p);
+                    if (FORM == kI8Any) i8_act_n(v, p);
                     const size_t at = (size_t)(t0 + t) * p.ldo + col;
                     if (WHOLE) {
                         if (!GATED && p.residual != nullptr) {

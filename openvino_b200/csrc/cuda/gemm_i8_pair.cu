@@ -208,8 +208,8 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
                     values(r + 16, column(job, RUNS - 1, step), u);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) v[i] = i8_gate(p, v[i], u[i]);
-                } else if (FORM == kI8Any && p.act != OVB_ACT_NONE) {
-                    apply_act_n(v, p);
+                } else if (FORM == kI8Any) {
+                    i8_act_n(v, p);
                 }
             };
             // 16-bit results: the box holds the 32 columns of the job, first of the residual, then of the result. WHOLE: aligned pieces of eight columns

@@ -210,6 +210,39 @@ def test_product_activations(K, T, N, Kd, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 6, 300])
+def test_rows_that_are_not_finite_show_behind_every_activation(K, T):
+    x = torch.randn((T, 256), generator=gen(T), device="cuda").bfloat16()
+    x[T - 1, 7] = math.nan
+    w, s, z = weight(256, 256, "unsigned", 1)
+    pw = K.PackedWeight.from_ir_i8(w, s, z)
+    for act in range(K.ACT_NONE, K.ACT_SOFTCAP + 1):
+        got = K.gemm(x, pw, act=act, glu=(7.0, 1.7, 1.0), cap=3.0)
+        assert got[T - 1].isnan().all() and got[:T - 1].isfinite().all(), act
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [3, 300])
+def test_activations_at_the_ends_of_their_range(K, T):
+    """Scales that carry the arguments from 2^-12 to 2^60: what saturates does so, what is small keeps its digits."""
+    F, N, Kd = torch.nn.functional, 256, 64
+    x = torch.randn((T, Kd), generator=gen(T), device="cuda").bfloat16()
+    w, s, _ = weight(N, Kd, "signed", 1)
+    s = torch.exp2(torch.linspace(-20, 52, N, device="cuda"))
+    pw, rows = K.PackedWeight.from_ir_i8(w, s), K.quantize_rows(x)
+    v, off = value64(rows, w, s, None)
+    for act, f, more in ((K.ACT_SILU, F.silu, {}), (K.ACT_GELU_TANH, lambda t: F.gelu(t, approximate="tanh"), {}), (K.ACT_SOFTCAP, lambda t: 30 * torch.tanh(t / 30), {"cap": 30.0})):
+        want = f(v)
+        # 2^-20 of the value, or where it vanishes of the argument's share that an exponential leaves (of the cap, once it is felt)
+        own = 2.0 ** -20 * (torch.minimum(v.abs(), torch.tensor(30.0, device="cuda", dtype=torch.float64)) + (want.abs()))
+        bound = off.clamp(max=1e30) * 1.14 + own
+        bound = torch.where(v.abs() > 1e6, want.abs() * 2.0 ** -20 + 2.0 ** -25, bound)
+        got = K.gemm(rows, pw, act=act, out_f32=True, **more).double()
+        assert got.isfinite().all()
+        within(got, want, bound + 2.0 ** -25, "activation %d" % act)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("T", [1, 4, 20, 300])
 def test_product_with_the_norm_in_front(K, T):
     N, Kd, dtype = 640, 2048, torch.bfloat16
