@@ -3,8 +3,8 @@
 // What bounds it: the tensor pipe, and in long runs the power cap. A pair of SMs works on 256 tokens (the M side, 128 to each SM) x 256 channels; every CTA
 // loads its 128 tokens and half of the weight rows, 32 KB for 256 x 256 x 128 products. The kernel is persistent and the accumulator exists twice in tensor
 // memory (2 x 256 columns), so that the epilogue of a tile runs under the main loop of the next. Measured: 8192 x 28672 x 4096 with the gate 590 us (3.26
-// POP/s; 2 x 1.67 is twice the measured bf16 rate), 999 x 8192 x 8192 47.5 us (2.8 POP/s: 128 tiles on 74 pairs), 333 x 4096 x 14336 28 us. Tiles of 128
-// channels and pairs that share K were slower at all of 607 measured sizes where they would fill the machine better.
+// POP/s; twice the measured bf16 rate is 3.34), 999 x 8192 x 8192 47.5 us (2.8 POP/s: 128 tiles on 74 pairs), 333 x 4096 x 14336 28 us. Tiles of 128
+// channels and pairs that share K gave nothing at sizes where they fill the machine better.
 //  * warp 0: producer (TMA boxes of both operands; both CTAs' bytes are counted on the even CTA's barrier), warp 1 of the even CTA: MMAs of the pair
 //  * warps 4 .. 11: epilogue. Tokens are the lanes, so a thread holds one row: adjacent channels lie in its registers, a gate and its up value too, and
 //    results leave in whole 32-byte sectors. Scales, zero points and biases of the channels come from shared memory, the same for all lanes.
