@@ -177,13 +177,26 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
             cs[tid] = n < p.N ? __ldg(p.w_scale + n) : 0.f;
             cb[tid] = n < p.N && p.bias != nullptr ? to_float(static_cast<const E*>(p.bias)[n]) : 0.f;
             cz[tid] = n < p.N && p.w_zp != nullptr ? __ldg(p.w_zp + n) : 0;
+            const int first_row = t - lane, rows = min(32, p.T - first_row);           // of this warp; rows may be negative
+            // The residual's 32 columns of a job, in aligned pieces of eight, are fetched a job ahead, the first ones before the products are complete.
+            const bool res = !GATED && p.residual != nullptr, res_ahead = res && p.whole;
+            uint4 ahead[GATED ? 1 : 4];
+            auto fetch = [&](int job) {
+                if (GATED) return;
+                const E* from = static_cast<const E*>(p.residual) + (size_t)first_row * p.ldr + n0 + job * 32;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = i * 8 + (lane >> 2), c = (lane & 3) * 8;
+                    if (r < rows && n0 + job * 32 + c < out_cols) ahead[GATED ? 0 : i] = __ldcg(reinterpret_cast<const uint4*>(from + (size_t)r * p.ldr + c));
+                }
+            };
+            if (res_ahead) fetch(half);
             // one thread polls and says how it ended; the others wait at the barrier, so that all eight warps go on or leave together
             if (tid == 0) went_well[buf] = mbar_wait(&acc_full[buf], acc_phase, abort_flag, p.status) ? 1 : 0;
             asm volatile("bar.sync 1, 256;" ::: "memory");
             if (!went_well[buf]) break;
             tc_fence_after_sync();
             const uint32_t src = tmem_base + (uint32_t(q * 32) << 16) + uint32_t(buf * 256);
-            const int first_row = t - lane, rows = min(32, p.T - first_row);           // of this warp; rows may be negative
             auto values = [&](const uint32_t* r, int c, float* v) {
 #pragma unroll
                 for (int i = 0; i < 16; i += 4) {
@@ -220,18 +233,21 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
 #pragma unroll 1
                 for (int job = half; job < JOBS; job += 2) {
                     const int col = (GATED ? n0 >> 1 : n0) + job * 32;
-                    const bool res = !GATED && p.residual != nullptr;
                     if (res) {
-                        const E* from = static_cast<const E*>(p.residual) + (size_t)first_row * p.ldr + col;
                         if (WHOLE) {
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const int r = i * 8 + (lane >> 2), c = (lane & 3) * 8;
-                                if (r < rows && col + c < out_cols) *in_box(r, lane & 3) = __ldcg(reinterpret_cast<const uint4*>(from + (size_t)r * p.ldr + c));
-                            }
+                            for (int i = 0; i < 4; ++i) *in_box(i * 8 + (lane >> 2), lane & 3) = ahead[GATED ? 0 : i];
+                            if (job + 2 < JOBS) fetch(job + 2);
                         } else {
-                            for (int r = 0; r < rows; ++r)
-                                if (col + lane < out_cols) reinterpret_cast<E*>(in_box(r, lane >> 3))[lane & 7] = from[(size_t)r * p.ldr + lane];
+                            const E* from = static_cast<const E*>(p.residual) + (size_t)first_row * p.ldr + col;
+                            for (int r0 = 0; r0 < rows; r0 += 16) {
+                                E e[16];
+#pragma unroll
+                                for (int i = 0; i < 16; ++i)
+                                    if (r0 + i < rows && col + lane < out_cols) e[i] = from[(size_t)(r0 + i) * p.ldr + lane];
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) reinterpret_cast<E*>(in_box(r0 + i, lane >> 3))[lane & 7] = e[i];
+                            }
                         }
                         __syncwarp();
                     }

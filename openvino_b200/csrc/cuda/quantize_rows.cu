@@ -76,25 +76,68 @@ __device__ __forceinline__ int source_row(const QuantParams& p, int row) {
     return r < 0 || r >= p.x_rows ? 0 : r;
 }
 
-// Rows of whole, aligned pieces of eight columns. WPR warps share a row; blocks of max(4, WPR) warps.
-template <class E, bool NORM, int WPR, int HOLD>
+// The pieces at, at + SPAN, .. of a row at any place and of any width, zero behind its end. Loads are of the aligned 16-byte blocks that hold a byte of the row (an
+// allocation that holds one byte of such a block holds it whole); a piece is shifted out of its block and the next, which the neighbouring lane holds.
+template <class E, int HOLD, int SPAN>
+__device__ __forceinline__ void load_pieces(const E* row, int cols, int at, uint4 (&x)[HOLD]) {
+    const int off = (int)(reinterpret_cast<uintptr_t>(row) & 15), lane = threadIdx.x & 31, blocks = (off + cols * 2 + 15) >> 4;
+    const uint4* from = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(row) - off);
+#pragma unroll
+    for (int h = 0; h < HOLD; ++h) x[h] = at + h * SPAN < blocks ? __ldcg(from + at + h * SPAN) : make_uint4(0, 0, 0, 0);
+    if (off != 0) {                         // the same for the warp
+        uint4 behind[HOLD];
+#pragma unroll
+        for (int h = 0; h < HOLD; ++h) behind[h] = lane == 31 && at + h * SPAN + 1 < blocks ? __ldcg(from + at + h * SPAN + 1) : make_uint4(0, 0, 0, 0);
+        const bool two = off & 8, one = off & 4;
+        const int bits = (off & 2) * 8;
+#pragma unroll
+        for (int h = 0; h < HOLD; ++h) {
+            uint32_t w[8] = {x[h].x, x[h].y, x[h].z, x[h].w, behind[h].x, behind[h].y, behind[h].z, behind[h].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t next = __shfl_down_sync(0xffffffffu, w[j], 1);
+                if (lane != 31) w[4 + j] = next;
+            }
+#pragma unroll
+            for (int j = 0; j < 6; ++j) w[j] = two ? w[j + 2] : w[j];
+#pragma unroll
+            for (int j = 0; j < 5; ++j) w[j] = one ? w[j + 1] : w[j];
+            x[h] = make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < HOLD; ++h) {
+        const int left = cols - 8 * (at + h * SPAN);
+        auto keep = [&](int j) { return left >= 2 * j + 2 ? 0xFFFFFFFFu : left == 2 * j + 1 ? 0xFFFFu : 0u; };
+        x[h] = make_uint4(x[h].x & keep(0), x[h].y & keep(1), x[h].z & keep(2), x[h].w & keep(3));
+    }
+}
+
+// Rows in pieces of eight columns, whole and aligned ones or (SHIFT) of any place and width. WPR warps share a row; blocks of max(4, WPR) warps.
+template <class E, bool NORM, int WPR, int HOLD, bool SHIFT>
 __global__ void __launch_bounds__(WPR < 4 ? 128 : WPR * 32) quantize_rows_kernel(const QuantParams p) {
     constexpr int RPB = WPR < 4 ? 4 / WPR : 1, SPAN = WPR * 32;
     __shared__ float box_f[16];
     __shared__ uint32_t box_u[16];
     __shared__ int box_i[16];
     const int row = blockIdx.x * RPB + (RPB > 1 ? (int)threadIdx.x / SPAN : 0), at = threadIdx.x % SPAN;
-    const int pieces = p.cols >> 3;
+    const int pieces = SHIFT ? (p.cols + 7) >> 3 : p.cols >> 3;
     pdl_enter();
     if (row >= p.rows) return;              // whole warps, and only where rows do not share a block's barriers
-    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const E*>(p.x) + (size_t)source_row(p, row) * p.ldx);
+    const E* line = static_cast<const E*>(p.x) + (size_t)source_row(p, row) * p.ldx;
+    const uint4* src = reinterpret_cast<const uint4*>(line);
     const uint4* gamma = static_cast<const uint4*>(p.gamma);
     uint4 x[HOLD], g[NORM ? HOLD : 1];
+    if (SHIFT) {
+        load_pieces<E, HOLD, SPAN>(line, p.cols, at, x);
+        if (NORM) load_pieces<E, NORM ? HOLD : 1, SPAN>(static_cast<const E*>(p.gamma), p.cols, at, g);
+    } else {
 #pragma unroll
-    for (int h = 0; h < HOLD; ++h) {
-        const bool in = at + h * SPAN < pieces;
-        x[h] = in ? __ldcg(src + at + h * SPAN) : make_uint4(0, 0, 0, 0);
-        if (NORM) g[h] = in ? __ldg(gamma + at + h * SPAN) : make_uint4(0, 0, 0, 0);
+        for (int h = 0; h < HOLD; ++h) {
+            const bool in = at + h * SPAN < pieces;
+            x[h] = in ? __ldcg(src + at + h * SPAN) : make_uint4(0, 0, 0, 0);
+            if (NORM) g[h] = in ? __ldg(gamma + at + h * SPAN) : make_uint4(0, 0, 0, 0);
+        }
     }
     uint32_t top = 0;
     uint64_t ss2 = pair_of(0.f);
@@ -125,13 +168,17 @@ __global__ void __launch_bounds__(WPR < 4 ? 128 : WPR * 32) quantize_rows_kernel
             if (!NORM) row_values<E, NORM>(x[h], x[h], y);
             const uint2 w = f != 0.f ? codes_of8(y, f) : make_uint2(0, 0);
             sum = sum_of8(w, sum);
-            dst[at + h * SPAN] = w;
+            if (!SHIFT || (at + h * SPAN) * 8 + 8 <= p.cols) {
+                dst[at + h * SPAN] = w;
+            } else {
+                for (int j = 0; j < p.cols % 8; ++j) reinterpret_cast<uint8_t*>(dst + at + h * SPAN)[j] = (uint8_t)((j < 4 ? w.x >> (8 * j) : w.y >> (8 * (j - 4))) & 0xFF);
+            }
         }
     sum = over_row<WPR>(sum, box_i, [](int a, int b) { return a + b; });
     if (at == 0) row_result(p, row, top, r, sum);
 }
 
-// Any width, pitch and alignment: a block per row, which is read once for each pass.
+// More columns, or codes at any place: a block per row, which is read once for each pass.
 template <class E>
 __global__ void __launch_bounds__(256) quantize_rows_any_kernel(const QuantParams p) {
     __shared__ float box_f[16];
@@ -161,21 +208,26 @@ __global__ void __launch_bounds__(256) quantize_rows_any_kernel(const QuantParam
     if (threadIdx.x == 0) row_result(p, row, top, r, sum);
 }
 
-template <class E, bool NORM>
+template <class E, bool NORM, bool SHIFT>
 static cudaError_t run_quantize(const QuantParams& p, cudaStream_t stream) {
-    const bool whole = p.cols % 8 == 0 && p.ldx % 8 == 0 && p.ldq % 8 == 0 &&
-                       ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.gamma)) & 15) == 0 && (reinterpret_cast<uintptr_t>(p.q) & 7) == 0;
-    if (!whole || p.cols > 32768) return launch_pdl(quantize_rows_any_kernel<E>, dim3(p.rows), dim3(256), 0, stream, p);
     auto go = [&](auto kern, int wpr) { return launch_pdl(kern, dim3(wpr < 4 ? (p.rows + 4 / wpr - 1) / (4 / wpr) : p.rows), dim3(wpr < 4 ? 128 : wpr * 32), 0, stream, p); };
     const bool many = p.rows >= kManyRows;
-    if (p.cols <= 512) return go(quantize_rows_kernel<E, NORM, 1, 2>, 1);
-    if (p.cols <= 1024) return go(quantize_rows_kernel<E, NORM, 1, 4>, 1);
-    if (p.cols <= 2048) return many ? go(quantize_rows_kernel<E, NORM, 1, 8>, 1) : go(quantize_rows_kernel<E, NORM, 8, 1>, 8);
-    if (p.cols <= 4096) return many ? go(quantize_rows_kernel<E, NORM, 4, 4>, 4) : go(quantize_rows_kernel<E, NORM, 8, 2>, 8);
-    if (p.cols <= 8192) return many ? go(quantize_rows_kernel<E, NORM, 4, 8>, 4) : go(quantize_rows_kernel<E, NORM, 16, 2>, 16);
+    if (p.cols <= 512) return go(quantize_rows_kernel<E, NORM, 1, 2, SHIFT>, 1);
+    if (p.cols <= 1024) return go(quantize_rows_kernel<E, NORM, 1, 4, SHIFT>, 1);
+    if (p.cols <= 2048) return many ? go(quantize_rows_kernel<E, NORM, 1, 8, SHIFT>, 1) : go(quantize_rows_kernel<E, NORM, 8, 1, SHIFT>, 8);
+    if (p.cols <= 4096) return many ? go(quantize_rows_kernel<E, NORM, 4, 4, SHIFT>, 4) : go(quantize_rows_kernel<E, NORM, 8, 2, SHIFT>, 8);
+    if (p.cols <= 8192) return many ? go(quantize_rows_kernel<E, NORM, 4, 8, SHIFT>, 4) : go(quantize_rows_kernel<E, NORM, 16, 2, SHIFT>, 16);
     // with a norm eight pieces take too many registers here: 1024 rows of 14336 in 13.9 us, in 12.9 with four
-    if (p.cols <= 16384) return many && !NORM ? go(quantize_rows_kernel<E, false, 8, 8>, 8) : go(quantize_rows_kernel<E, NORM, 16, 4>, 16);
-    return go(quantize_rows_kernel<E, NORM, 16, 8>, 16);
+    if (p.cols <= 16384) return many && !NORM ? go(quantize_rows_kernel<E, false, 8, 8, SHIFT>, 8) : go(quantize_rows_kernel<E, NORM, 16, 4, SHIFT>, 16);
+    return go(quantize_rows_kernel<E, NORM, 16, 8, SHIFT>, 16);
+}
+template <class E, bool NORM>
+static cudaError_t run_quantize(const QuantParams& p, cudaStream_t stream) {
+    const auto bits = [](const void* x) { return reinterpret_cast<uintptr_t>(x); };
+    if (p.cols > 32768 || p.ldq % 8 != 0 || (bits(p.q) & 7) != 0 || ((bits(p.x) | bits(p.gamma)) & 1) != 0)
+        return launch_pdl(quantize_rows_any_kernel<E>, dim3(p.rows), dim3(256), 0, stream, p);
+    const bool whole = p.cols % 8 == 0 && p.ldx % 8 == 0 && ((bits(p.x) | bits(p.gamma)) & 15) == 0;
+    return whole ? run_quantize<E, NORM, false>(p, stream) : run_quantize<E, NORM, true>(p, stream);
 }
 
 }  // namespace ovb

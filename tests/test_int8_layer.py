@@ -116,6 +116,47 @@ def test_rows_of_other_strides(K):
         assert torch.equal(r.q.cpu(), q) and torch.equal(r.scales.cpu(), scale) and torch.equal(r.sums.cpu(), total)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [3, 515])
+@pytest.mark.parametrize("cols", [1, 7, 9, 16, 23, 100, 513, 1030, 2049, 4097, 8200, 16401, 32767, 32769])
+def test_rows_at_any_place(K, rows, cols):
+    """Views that start at every 16-bit place of a 16-byte piece, with odd and even pitches: the codes of the rows, and with a norm the same bits wherever they lie."""
+    norm_want = None
+    for off in range(9):
+        wide = torch.full((rows, cols + 9 + off % 2), math.nan, device="cuda", dtype=torch.bfloat16)
+        view = wide[:, off:off + cols]
+        view.copy_(torch.randn((rows, cols), generator=gen(cols), device="cuda"))
+        r = K.quantize_rows(view)
+        q, scale, total = codes_of(view)
+        assert torch.equal(r.q.cpu(), q) and torch.equal(r.scales.cpu(), scale) and torch.equal(r.sums.cpu(), total)
+        gamma = torch.empty(cols + 8, device="cuda", dtype=torch.bfloat16)[off % 8:off % 8 + cols]
+        gamma.copy_(1 + 0.3 * torch.randn(cols, generator=gen(2), device="cuda"))
+        n = K.quantize_rows(view, norm=(gamma, 1e-3))
+        norm_want = norm_want or n
+        assert torch.equal(n.q, norm_want.q) and torch.equal(n.scales, norm_want.scales) and torch.equal(n.sums, norm_want.sums)
+    K.check_status("quantize_rows")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,N", [(300, 514), (300, 520), (700, 1024), (513, 1003)])
+def test_residuals_of_many_tokens(K, T, N):
+    """The residual in rows of other pitches than the result's, of any alignment, and in the result's own place."""
+    Kd = 256
+    w, s, z = weight(N, Kd, "signed_zp", 3)
+    rows = K.quantize_rows(torch.randn((T, Kd), generator=gen(T), device="cuda").bfloat16())
+    for pw in (K.PackedWeight.from_ir_i8(w, s), K.PackedWeight.from_ir_i8(w, s, z)):
+        plain = K.gemm(rows, pw, out_f32=True)
+        for off, pad in ((0, 0), (0, 8), (3, 5), (8, 16)):
+            wide = torch.randn((T, N + off + pad), generator=gen(N), device="cuda").bfloat16()
+            res, keep = wide[:, off:off + N], wide.clone()
+            want = (plain + res.float()).bfloat16()
+            assert torch.equal(K.gemm(rows, pw, residual=res), want) and torch.equal(wide, keep)
+            assert torch.equal(K.gemm(rows, pw, residual=res, out=res), want)
+            keep[:, off:off + N] = want
+            assert torch.equal(wide, keep)
+    K.check_status("gemm_i8")
+
+
 # ------------------------------------------------------------------------------------------------ products
 def weight(N, Kd, form, seed):
     g = gen(seed)
