@@ -4,7 +4,9 @@
 //
 // What bounds it: memory, three bytes per value (two of them usually from L2). A row is read once and stays in registers until its largest magnitude is known:
 // every thread holds HOLD pieces of eight columns, as they came or, with a norm, times the weights. Measured without and with a norm: 8192 x 4096 16.4 and
-// 21.9 us, 8192 x 8192 29.8 and 43.8 us (6.8 and 4.6 TB/s; the weights are read again by every row, from L1), 64 x 4096 1.8 and 2.0 us, of which most is the launch.
+// 21.2 us, 8192 x 8192 29.7 and 43.7 us (6.8 and 4.6 TB/s; with a norm the instructions, 16 for a value, fill three quarters of the issue slots), 64 x 4096
+// 1.8 and 2.0 us, of which most is the launch. Rows that do not lie in whole aligned pieces: 999 x 1333 3.5 and 3.9 us, 8192 x 500 5.5 and 7.5, 8192 x 4097
+// 38 and 51 (value by value, in a block per row: 4.6 and 5.6, 17.9 and 21.3, 36 and 46).
 #include "gemm_i8.cuh"
 
 namespace ovb {
