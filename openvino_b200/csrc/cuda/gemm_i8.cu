@@ -399,7 +399,8 @@ constexpr int64_t kI8FusedWeights = 64 << 20;       // bytes
 static bool i8_fuses(const ovb_gemm_i8_args* a) {
     const auto bits = [](const void* x) { return reinterpret_cast<uintptr_t>(x); };
     const uintptr_t rows = a->row_idx != nullptr ? ((uintptr_t)(a->raw_rows - 1) * (uintptr_t)a->ld_raw + (uintptr_t)a->K) * 2 : (uintptr_t)a->K * 2;
-    const bool apart = bits(a->out) >= bits(a->raw) + rows || bits(a->raw) >= bits(a->out) + (uintptr_t)a->N * 4;
+    const uintptr_t result = (uintptr_t)(is_gated(a->act) ? a->N / 2 : a->N) * (a->out_f32 ? 4 : 2);
+    const bool apart = bits(a->out) >= bits(a->raw) + rows || bits(a->raw) >= bits(a->out) + result;
     return apart && a->raw != nullptr && a->T == 1 && (int64_t)a->N * a->K <= kI8FusedWeights && a->K % 8 == 0 && a->K <= kI8QuantWarps * 32 * kI8Hold * 8 && (a->row_idx == nullptr || a->ld_raw % 8 == 0) &&
            ((bits(a->raw) | bits(a->gamma)) & 15) == 0;
 }
