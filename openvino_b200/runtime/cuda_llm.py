@@ -65,7 +65,7 @@ class LlmWeights:
     @staticmethod
     def _pack_int8(w: torch.Tensor, cfg: LlmConfig) -> K.PackedWeight:
         N, Kd = w.shape
-        if cfg.int8_activations:                # one scale per row: products of whole numbers
+        if cfg.int8_activations and Kd <= 65536:                # one scale per row: products of whole numbers
             q, s, z = quant.quantize_u8_asym(w, Kd)
             return K.PackedWeight.from_ir_i8(q, s, z)
         g = cfg.group_size or Kd

@@ -212,6 +212,24 @@ def test_logits_of_prefills_chunks_and_single_tokens(name, kv):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("more", [dict(weight_format="int8", int8_activations=True, group_size=0), dict(qk_norm=True, rope_inv_freq=SCALED)])
+def test_experts(more):
+    """Decoders with experts: their products in whole numbers, and head norms in front of their attention."""
+    from openvino_b200.ops import cuda as K
+    cfg = TINY_MOE.with_(**more)
+    state = llama.random_float_state(cfg, seed=5, std=0.05)
+    eff = {k: v.cuda() for k, v in llama.effective_state(cfg, state).items()}
+    ex = executor(cfg, state, use_cuda_graphs=False)
+    ids = torch.randint(0, cfg.vocab_size, (41,), generator=torch.Generator().manual_seed(2))
+    want = llama.reference_logits(cfg, eff, ids.cuda())
+    bound = INT8_LOGITS if cfg.int8_activations else BF16_LOGITS
+    assert ex.int8 == cfg.int8_activations
+    assert off(prefill(ex, ids[:40].numpy()), want[39]) < bound
+    assert off(prefill(ex, ids[40:].numpy(), 40), want[40]) < bound
+    K.check_status("experts")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("name", ["int8_head_norms", "scaled_norms_int4"])
 def test_generation_with_captured_steps(name):
     """Prompts of several lengths through the batching pipeline, decode steps as CUDA graphs: every token is the reference's best under the same earlier
