@@ -471,7 +471,7 @@ def quantize_rows(x: torch.Tensor, norm=None) -> QuantizedRows:
     """bf16 or fp16 rows -> signed bytes: with a = max |row|, code = round(value * (127 / a)), halves to even, scale = a / 127.
 
     ``norm`` (weights, eps[, row indices]): RMS norm of the rows (of the indexed rows) of ``x`` first, in 32 bits. A row without a value of at least 2^-119 is
-    zero; one with a value that is not finite has the scale NaN, and so have all products with it."""
+    zero; one with a value that is not finite has the scale NaN, and so have all products with it (with a norm: a value of the row times its weight)."""
     T, gamma, eps, idx = _raw_rows(x, norm)
     d = _one_device(x, gamma, idx)
     cols = x.shape[1]
@@ -1190,7 +1190,7 @@ def qk_norm_rope_kv_write(qkv, positions, slot_map, k_cache, v_cache, inv_freq, 
                           mult=1.0, q_out=None, k_meta=None, v_meta=None) -> None:
     """``qk_norm_rope`` of the rows of a fused projection ``qkv`` [T, (Hq + 2 Hkv) * D], keys and values going to the paged cache.
 
-    Queries go to ``q_out`` [T, Hq * D], by default their own place in ``qkv``; key and value rows to the slots ``slot_map`` (int32, block * block_size +
+    Queries go to ``q_out`` [T, Hq * D], by default their own place in ``qkv``, else memory that its heads do not use; key and value rows to the slots ``slot_map`` (int32, block * block_size +
     offset; negative: not kept; the slots of a call differ) of the caches [num_blocks, Hkv, block_size, D], which are of the type of ``qkv``, or uint8 with
     the fp16 (scale, zero point) tables ``k_meta`` / ``v_meta`` [num_blocks, Hkv, block_size, 2] (D and the rotation multiples of 8, D up to 256).
     A slot behind the cache is not written and shows in the status word."""
