@@ -143,7 +143,9 @@ __global__ void __launch_bounds__(i8_threads(FUSED)) gemm_i8_tile_kernel(const _
     const int n0 = tile * TILE_N, t0 = blockIdx.y * p.bt;
     const int kb0 = (int)((int64_t)p.KB * split / p.splits), kb1 = (int)((int64_t)p.KB * (split + 1) / p.splits);
     const int stage_bytes = kI8TileBytes + (FUSED ? 0 : p.bt * kI8BlockK);
-    uint8_t* stages = FUSED ? smem + (kb1 - kb0) * kI8FusedBlock : smem;                // fused: the rows' codes come first
+    // fused: the row's codes come first. The partial sums take the stages' place and are read by the other CTAs at this CTA's own offset, so room is left for the
+    // largest share of the cluster, whichever this one is.
+    uint8_t* stages = FUSED ? smem + (p.KB + p.splits - 1) / p.splits * kI8FusedBlock : smem;
     const uint32_t tmem_cols = p.bt <= 32 ? 32u : p.bt <= 64 ? 64u : p.bt <= 128 ? 128u : 256u;
     if (threadIdx.x == 0) {
         for (int s = 0; s < p.stages; ++s) {
