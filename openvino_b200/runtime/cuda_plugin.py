@@ -913,7 +913,7 @@ def _prepare_fc(n: Node, ins, ctx: Ctx):
                 # products of whole numbers: a scale per channel, rows of activations quantised one by one
                 np_type, t_type = (np.uint8, torch.uint8) if et == "u8" else (np.int8, torch.int8)
                 wq = torch.from_numpy(np.ascontiguousarray(wt.data).reshape(N, Kd).view(np_type).copy()).to(ctx.device)
-                zp = torch.zeros(1) if et == "i8" else torch.full((1,), 128.0)
+                zp = torch.zeros(1)                     # a graph without zero points subtracts nothing
                 if zp_node is not None and zp_node.get_type_name() == "Constant" and zp_node.get_tensor_view().size > 0:
                     zp = torch.from_numpy(np.ascontiguousarray(zp_node.get_tensor_view().to_float32())).reshape(-1)
                 zp = (zp.expand(N) if zp.numel() == 1 else zp.reshape(N)).to(t_type).to(ctx.device)
@@ -921,14 +921,14 @@ def _prepare_fc(n: Node, ins, ctx: Ctx):
             elif et in ("u4", "u8") and Kd % 64 == 0 and (Kd // G) % 64 == 0:
                 dev = ctx.device
                 wq = torch.from_numpy(np.ascontiguousarray(wt.data).reshape(-1).view(np.uint8).copy()).to(dev)
-                zp = None
+                zp = torch.zeros(1)                     # a graph without zero points subtracts nothing
                 if zp_node is not None and zp_node.get_type_name() == "Constant" and zp_node.get_tensor_view().size > 0:
                     zp = torch.from_numpy(np.ascontiguousarray(zp_node.get_tensor_view().to_float32())).reshape(-1)
-                    zp = (zp.expand(N * G) if zp.numel() == 1 else zp).reshape(N, G).to(torch.uint8).to(dev)
+                zp = (zp.expand(N * G) if zp.numel() == 1 else zp).reshape(N, G).to(torch.uint8).contiguous().to(dev)
                 b16 = bias.to(torch.bfloat16) if bias is not None and bias.numel() == N else None
                 sc16 = scales.to(torch.float16).contiguous().to(dev)
                 if et == "u4":
-                    st["packed"] = K.PackedWeight.from_ir_u4(wq.reshape(-1), sc16, zp.contiguous() if zp is not None else None, N, Kd, Kd // G,
+                    st["packed"] = K.PackedWeight.from_ir_u4(wq.reshape(-1), sc16, zp, N, Kd, Kd // G,
                                                              zp_is_u8=True, bias=b16)
                 else:
                     st["packed"] = K.PackedWeight.from_ir_u8(wq.reshape(N, Kd), sc16, zp, N, Kd, Kd // G, bias=b16)

@@ -56,7 +56,7 @@ class _Linear:
             zp_node = fc.input_value(4).get_node() if fc.get_input_size() > 4 else None
             zp = _const_f32(zp_node).reshape(-1) if zp_node is not None and zp_node.get_type_name() == "Constant" and zp_node.get_tensor_view().size else None
             if zp is None:
-                zp = torch.full((1,), 8.0 if self.kind == "u4" else 128.0)
+                zp = torch.zeros(1)                                                    # a graph without zero points subtracts nothing
             self.zp = (zp.expand(self.N * self.G) if zp.numel() == 1 else zp).reshape(self.N, self.G).to(torch.uint8)
         else:
             self.w = _const_f32(w).reshape(self.N, self.K)

@@ -1,0 +1,86 @@
+"""Compressed weights whose graphs leave something out: zero points (missing ones are 0), scales for every channel."""
+import numpy as np
+import pytest
+import torch
+
+import openvino_b200 as ov
+from openvino_b200 import opset as ops
+from openvino_b200 import properties as props
+from openvino_b200._tensor import Tensor
+from openvino_b200._types import Type
+from openvino_b200.models import llama, ov_builders
+from openvino_b200.models.llm_config import TINY_LLAMA
+from openvino_b200.models.ov_builders import build_llama
+from openvino_b200.runtime import llm_import
+
+SMALL = TINY_LLAMA.with_(vocab_size=320)
+RANGES = {"u4": (0, 16), "u8": (0, 256), "i8": (-128, 128)}
+
+
+def product(kind, N, Kd, zero_point=None, one_scale=False, seed=3):
+    """(model of one product with a compressed weight, the weight's values in 64 bits, what is added up without zero points)."""
+    rng = np.random.default_rng(seed)
+    q = rng.integers(*RANGES[kind], (N, Kd))
+    s = np.full((1, 1), 0.0123, np.float16) if one_scale else ((0.5 + rng.random((N, 1))) / 100).astype(np.float16)
+    x = ops.parameter([-1, Kd], "f32", "x")
+    qt = Tensor(q.astype(np.float32)).astype(getattr(Type, kind)) if kind == "u4" else q.astype(np.uint8 if kind == "u8" else np.int8)
+    w = ops.convert(ops.constant(qt), "f16")
+    if zero_point is not None:
+        w = ops.subtract(w, ops.constant(np.asarray(zero_point, np.float16)))
+    w = ops.convert(ops.multiply(w, ops.constant(s)), "f32")
+    z = 0.0 if zero_point is None else np.asarray(zero_point, np.float64)
+    return ov.Model([ops.result(ops.matmul(x, w.output(0), False, True))], [x], "product"), (q - z) * s.astype(np.float64)
+
+
+def check(m, w64, rows, precision, group):
+    """The compiled product against the formula. Four roundings to 16 bits at most between the inputs and a result (row, scale, weight, result; the sums are held in
+    32 bits); with quantised rows a value is half a step of a / 127 off, a the row's largest."""
+    Kd = w64.shape[1]
+    x = np.abs(np.random.default_rng(rows).standard_normal((rows, Kd))).astype(np.float32) + 0.25       # (one sign: a wrong zero point cannot cancel)
+    cm = ov.Core().compile_model(m, "CUDA", {props.hint.inference_precision: precision, props.hint.dynamic_quantization_group_size: group})
+    got = cm(x)[0].astype(np.float64)
+    want = x.astype(np.float64) @ w64.T
+    size = x.astype(np.float64) @ np.abs(w64).T
+    eps = 2.0 ** -8 if precision == "bf16" else 2.0 ** -11
+    bound = (4 * eps + 2.0 ** -11) * size
+    if group:
+        bound += x.max(1, keepdims=True) / 254 * (1 + 4 * eps) * np.abs(w64).sum(1)
+    worst = float((np.abs(got - want) / bound).max())
+    assert worst <= 1
+    return cm
+
+
+@pytest.mark.parametrize("kind", RANGES)
+def test_missing_zero_points_are_zero_on_the_host(kind):
+    m, w64 = product(kind, 24, 64)
+    x = np.random.default_rng(1).standard_normal((5, 64)).astype(np.float32)
+    assert np.abs(ov.Core().compile_model(m, "CPU")(x)[0] - x @ w64.T).max() < 2.0 ** -9 * (np.abs(x) @ np.abs(w64).T).max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("precision", ["bf16", "f16"])
+@pytest.mark.parametrize("group", [0, -1])
+@pytest.mark.parametrize("kind,N,Kd", [("u8", 160, 128), ("u8", 75, 96), ("i8", 160, 128), ("i8", 75, 96), ("u4", 128, 128)])
+def test_missing_zero_points_are_zero(kind, N, Kd, group, precision):
+    m, w64 = product(kind, N, Kd)
+    for rows in (1, 13):
+        check(m, w64, rows, precision, group)
+
+
+def without_zero_points(monkeypatch):
+    """Weights of built decoders lose the Subtract of their zero points."""
+    subtract = ov_builders.ops.subtract
+
+    def bare(a, b):
+        node = a.get_node() if hasattr(a, "get_node") else a
+        return a if node.get_type_name() == "Convert" and node.input_value(0).get_element_type() in (Type.u4, Type.u8) else subtract(a, b)
+    monkeypatch.setattr(ov_builders.ops, "subtract", bare)
+
+
+@pytest.mark.parametrize("compress", ["int8", "int4"])
+def test_missing_zero_points_are_zero_in_the_serving_import(compress, monkeypatch):
+    without_zero_points(monkeypatch)
+    cfg = SMALL.with_(group_size=0 if compress == "int8" else 128)
+    _, parts = llm_import.analyze(build_llama(cfg, llama.random_float_state(cfg, seed=1, std=0.05), compress=compress))
+    linears = list(parts["lin"].values()) + [parts["lm_head"]]
+    assert all(v.compressed and not v.zp.any() and v.zp.shape == v.scales.shape for v in linears)
