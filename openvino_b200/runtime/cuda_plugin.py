@@ -882,6 +882,15 @@ def _sdpa(n, ins, ctx):
     return [F.scaled_dot_product_attention(q, k.to(q.dtype), v.to(q.dtype), attn_mask=None if causal else mask, is_causal=bool(causal) and mask is None, scale=scale)]
 
 
+def _group_values(node: Optional[Node], N: int, G: int = 0) -> torch.Tensor:
+    """Constant scales or zero points of a compressed weight as fp32 [N, G] (``G`` 0: as many groups as there are values). One zero point stands for all;
+    without any they are 0."""
+    v = torch.zeros(1)
+    if node is not None and node.get_tensor_view().size > 0:
+        v = torch.from_numpy(np.ascontiguousarray(node.get_tensor_view().to_float32())).reshape(-1)
+    return v.expand(N * G).reshape(N, G) if v.numel() == 1 and G else v.reshape(N, G or -1)
+
+
 def _prepare_fc(n: Node, ins, ctx: Ctx):
     """Pack the constant weight of a FullyConnected(-Compressed) once: tile layout for the tcgen05 GEMM."""
     st = ctx.cache.get(id(n))
@@ -907,31 +916,31 @@ def _prepare_fc(n: Node, ins, ctx: Ctx):
             et = wt.element_type.name
             N = wt.shape[0]
             Kd = int(np.prod(wt.shape[1:]))
-            scales = torch.from_numpy(np.ascontiguousarray(sc_node.get_tensor_view().to_float32())).reshape(N, -1)
+            if any(c is not None and c.get_type_name() != "Constant" for c in (sc_node, zp_node)):
+                ctx.cache[id(n)] = st                   # expanded with the values of every call
+                return st
+            scales = _group_values(sc_node, N)
             G = scales.shape[1]
-            if et in ("u8", "i8") and G == 1 and Kd <= 65536 and ins[0].dtype in (torch.float16, torch.bfloat16) and quantizes_rows(ctx.dynamic_quantization, Kd):
+            zp = _group_values(zp_node, N, G)
+            # tables of zero points hold bytes; others are expanded with their weights
+            lo, hi = {"u4": (0, 15), "u8": (0, 255), "i8": (-128, 127)}.get(et, (0, 0))
+            held = bool(((zp == zp.round()) & (zp >= lo) & (zp <= hi)).all())
+            if held and et in ("u8", "i8") and G == 1 and Kd <= 65536 and ins[0].dtype in (torch.float16, torch.bfloat16) and quantizes_rows(ctx.dynamic_quantization, Kd):
                 # products of whole numbers: a scale per channel, rows of activations quantised one by one
                 np_type, t_type = (np.uint8, torch.uint8) if et == "u8" else (np.int8, torch.int8)
                 wq = torch.from_numpy(np.ascontiguousarray(wt.data).reshape(N, Kd).view(np_type).copy()).to(ctx.device)
-                zp = torch.zeros(1)                     # a graph without zero points subtracts nothing
-                if zp_node is not None and zp_node.get_type_name() == "Constant" and zp_node.get_tensor_view().size > 0:
-                    zp = torch.from_numpy(np.ascontiguousarray(zp_node.get_tensor_view().to_float32())).reshape(-1)
-                zp = (zp.expand(N) if zp.numel() == 1 else zp.reshape(N)).to(t_type).to(ctx.device)
-                st["packed"] = K.PackedWeight.from_ir_i8(wq, scales.reshape(-1).to(ctx.device), zp, bias=bias.to(ctx.device, ins[0].dtype) if bias is not None and bias.numel() == N else None)
-            elif et in ("u4", "u8") and Kd % 64 == 0 and (Kd // G) % 64 == 0:
+                st["packed"] = K.PackedWeight.from_ir_i8(wq, scales.reshape(-1).to(ctx.device), zp.reshape(-1).to(t_type).to(ctx.device),
+                                                         bias=bias.to(ctx.device, ins[0].dtype) if bias is not None and bias.numel() == N else None)
+            elif held and et in ("u4", "u8") and Kd % 64 == 0 and (Kd // G) % 64 == 0:
                 dev = ctx.device
                 wq = torch.from_numpy(np.ascontiguousarray(wt.data).reshape(-1).view(np.uint8).copy()).to(dev)
-                zp = torch.zeros(1)                     # a graph without zero points subtracts nothing
-                if zp_node is not None and zp_node.get_type_name() == "Constant" and zp_node.get_tensor_view().size > 0:
-                    zp = torch.from_numpy(np.ascontiguousarray(zp_node.get_tensor_view().to_float32())).reshape(-1)
-                zp = (zp.expand(N * G) if zp.numel() == 1 else zp).reshape(N, G).to(torch.uint8).contiguous().to(dev)
+                z8 = zp.to(torch.uint8).contiguous().to(dev)
                 b16 = bias.to(torch.bfloat16) if bias is not None and bias.numel() == N else None
                 sc16 = scales.to(torch.float16).contiguous().to(dev)
                 if et == "u4":
-                    st["packed"] = K.PackedWeight.from_ir_u4(wq.reshape(-1), sc16, zp, N, Kd, Kd // G,
-                                                             zp_is_u8=True, bias=b16)
+                    st["packed"] = K.PackedWeight.from_ir_u4(wq.reshape(-1), sc16, z8, N, Kd, Kd // G, zp_is_u8=True, bias=b16)
                 else:
-                    st["packed"] = K.PackedWeight.from_ir_u8(wq.reshape(N, Kd), sc16, zp, N, Kd, Kd // G, bias=b16)
+                    st["packed"] = K.PackedWeight.from_ir_u8(wq.reshape(N, Kd), sc16, z8, N, Kd, Kd // G, bias=b16)
     ctx.cache[id(n)] = st
     return st
 
@@ -949,6 +958,8 @@ def _dequant_weight(n: Node, ins, ctx: Ctx) -> torch.Tensor:
         z = z.reshape(-1)
         z = (z.expand(N * G) if z.numel() == 1 else z).reshape(N, G)
         w = ((wf.reshape(N, G, -1) - z.unsqueeze(-1)) * s.unsqueeze(-1)).reshape(N, -1)
+        if any(n.input_value(i).get_node().get_type_name() != "Constant" for i in [1, 3, 4][:n.get_input_size() - 2]):
+            return w.to(ctx.device)                     # of this call only
         st["w"] = w.to(ctx.device)
     return st["w"]
 

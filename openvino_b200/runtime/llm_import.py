@@ -57,6 +57,8 @@ class _Linear:
             zp = _const_f32(zp_node).reshape(-1) if zp_node is not None and zp_node.get_type_name() == "Constant" and zp_node.get_tensor_view().size else None
             if zp is None:
                 zp = torch.zeros(1)                                                    # a graph without zero points subtracts nothing
+            if not bool(((zp == zp.round()) & (zp >= 0) & (zp <= (15 if self.kind == "u4" else 255))).all()):
+                raise NotAnLlm("zero points of %s that are not whole numbers of the weight's type are not served" % fc.get_friendly_name())
             self.zp = (zp.expand(self.N * self.G) if zp.numel() == 1 else zp).reshape(self.N, self.G).to(torch.uint8)
         else:
             self.w = _const_f32(w).reshape(self.N, self.K)

@@ -1,4 +1,4 @@
-"""Compressed weights whose graphs leave something out: zero points (missing ones are 0), scales for every channel."""
+"""Compressed weights whose graphs leave something out: zero points (missing ones are 0), a scale for every channel, or that hold unusual ones."""
 import numpy as np
 import pytest
 import torch
@@ -84,3 +84,37 @@ def test_missing_zero_points_are_zero_in_the_serving_import(compress, monkeypatc
     _, parts = llm_import.analyze(build_llama(cfg, llama.random_float_state(cfg, seed=1, std=0.05), compress=compress))
     linears = list(parts["lin"].values()) + [parts["lm_head"]]
     assert all(v.compressed and not v.zp.any() and v.zp.shape == v.scales.shape for v in linears)
+
+
+# ------------------------------------------------------------------------------------------------ zero points that are not whole numbers of the weight's type
+def test_zero_points_between_whole_numbers_are_not_served(monkeypatch):
+    subtract = ov_builders.ops.subtract
+
+    def between(a, b):
+        node = b.get_node() if hasattr(b, "get_node") else b
+        if node.get_type_name() != "Convert" or node.input_value(0).get_element_type() != Type.u8:
+            return subtract(a, b)
+        z = np.float16(node.input_value(0).get_node().get_tensor_view().to_float32()) + np.float16(0.5)
+        return subtract(a, ov_builders.constant(z))
+    monkeypatch.setattr(ov_builders.ops, "subtract", between)
+    cfg = SMALL.with_(group_size=0)
+    with pytest.raises(llm_import.NotAnLlm, match="whole numbers"):
+        llm_import.analyze(build_llama(cfg, llama.random_float_state(cfg, seed=1, std=0.05), compress="int8"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", [0, -1])
+@pytest.mark.parametrize("kind,zero_point", [("u8", 127.5), ("u8", -3.0), ("u8", 300.0), ("i8", 0.5), ("i8", 130.0), ("u4", 7.5)])
+def test_zero_points_outside_the_weights_type(kind, zero_point, group):
+    """Such weights are multiplied as the graph says, expanded."""
+    m, w64 = product(kind, 128, 128, zero_point)
+    cm = check(m, w64, 13, "bf16", group)
+    assert all(st["packed"] is None for st in cm.program.ctx.cache.values() if isinstance(st, dict) and "packed" in st)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", [0, -1])
+@pytest.mark.parametrize("kind,zero_point", [("u8", 0.0), ("u8", 255.0), ("i8", -128.0), ("i8", 127.0), ("u4", 15.0)])
+def test_zero_points_at_the_ends_of_the_weights_type(kind, zero_point, group):
+    m, w64 = product(kind, 128, 128, zero_point)
+    check(m, w64, 13, "bf16", group)
