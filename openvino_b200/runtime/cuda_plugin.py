@@ -883,12 +883,12 @@ def _sdpa(n, ins, ctx):
 
 
 def _group_values(node: Optional[Node], N: int, G: int = 0) -> torch.Tensor:
-    """Constant scales or zero points of a compressed weight as fp32 [N, G] (``G`` 0: as many groups as there are values). One zero point stands for all;
-    without any they are 0."""
+    """Constant scales or zero points of a compressed weight as fp32 [N, G] (``G`` 0: as many groups as there are values). One value stands for all; without any,
+    as a graph without zero points has it, they are 0."""
     v = torch.zeros(1)
     if node is not None and node.get_tensor_view().size > 0:
         v = torch.from_numpy(np.ascontiguousarray(node.get_tensor_view().to_float32())).reshape(-1)
-    return v.expand(N * G).reshape(N, G) if v.numel() == 1 and G else v.reshape(N, G or -1)
+    return v.expand(N * max(G, 1)).reshape(N, -1) if v.numel() == 1 else v.reshape(N, G or -1)
 
 
 def _prepare_fc(n: Node, ins, ctx: Ctx):
@@ -952,7 +952,8 @@ def _dequant_weight(n: Node, ins, ctx: Ctx) -> torch.Tensor:
         wf = torch.from_numpy(np.ascontiguousarray(w_node.get_tensor_view().to_float32())) if w_node.get_type_name() == "Constant" else ins[1].float().cpu()
         N = wf.shape[0]
         wf = wf.reshape(N, -1)
-        s = ins[3].float().cpu().reshape(N, -1)
+        s = ins[3].float().cpu().reshape(-1)
+        s = (s.expand(N) if s.numel() == 1 else s).reshape(N, -1)
         G = s.shape[1]
         z = ins[4].float().cpu() if len(ins) > 4 and ins[4].numel() > 0 else torch.zeros(1)
         z = z.reshape(-1)

@@ -51,7 +51,8 @@ class _Linear:
             if self.kind not in ("u4", "u8"):
                 raise NotAnLlm("compressed weight type %s is not supported by the serving program" % self.kind)
             self.q = torch.from_numpy(np.ascontiguousarray(view.data).reshape(-1).view(np.uint8).copy()).reshape(self.N, -1)
-            self.scales = _const_f32(fc.input_value(3).get_node()).reshape(self.N, -1)
+            scales = _const_f32(fc.input_value(3).get_node()).reshape(-1)
+            self.scales = (scales.expand(self.N) if scales.numel() == 1 else scales).reshape(self.N, -1)
             self.G = self.scales.shape[1]
             zp_node = fc.input_value(4).get_node() if fc.get_input_size() > 4 else None
             zp = _const_f32(zp_node).reshape(-1) if zp_node is not None and zp_node.get_type_name() == "Constant" and zp_node.get_tensor_view().size else None

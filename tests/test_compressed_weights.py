@@ -118,3 +118,29 @@ def test_zero_points_outside_the_weights_type(kind, zero_point, group):
 def test_zero_points_at_the_ends_of_the_weights_type(kind, zero_point, group):
     m, w64 = product(kind, 128, 128, zero_point)
     check(m, w64, 13, "bf16", group)
+
+
+# ------------------------------------------------------------------------------------------------ one scale for the whole weight
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", [0, -1])
+@pytest.mark.parametrize("kind,N,Kd", [("u8", 160, 128), ("u8", 75, 96), ("i8", 75, 96), ("u4", 128, 128)])
+@pytest.mark.parametrize("zero_point", [None, 5.0])
+def test_one_scale_for_a_whole_weight(kind, N, Kd, zero_point, group):
+    m, w64 = product(kind, N, Kd, zero_point, one_scale=True)
+    for rows in (1, 13):
+        check(m, w64, rows, "bf16", group)
+
+
+def test_one_scale_for_a_whole_weight_in_the_serving_import(monkeypatch):
+    multiply = ov_builders.ops.multiply
+
+    def single(a, b, **kw):
+        node = b.get_node() if hasattr(b, "get_node") else b
+        if node.get_type_name() != "Constant" or not node.get_friendly_name().endswith("/scale"):
+            return multiply(a, b, **kw)
+        return multiply(a, ov_builders.constant(np.full((1, 1, 1), 0.01, np.float16)))
+    monkeypatch.setattr(ov_builders.ops, "multiply", single)
+    cfg = SMALL.with_(group_size=0)
+    _, parts = llm_import.analyze(build_llama(cfg, llama.random_float_state(cfg, seed=1, std=0.05), compress="int8"))
+    for v in list(parts["lin"].values()) + [parts["lm_head"]]:
+        assert v.whole_rows and v.scales.shape == (v.N, 1) and bool((v.scales == float(np.float16(0.01))).all()) and v.zp.shape == (v.N, 1)
