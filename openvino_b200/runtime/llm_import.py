@@ -143,7 +143,8 @@ _DEAD_ENDS = ("Parameter", "Constant", "ReadValue", "Result", "Assign")
 def _nearest_fc_ancestor(out_port, head_size: int = 0, found: Optional[Dict] = None) -> Optional[Node]:
     """Closest FullyConnected node that feeds ``out_port`` (breadth first over all data inputs; shape plumbing, RoPE, the
     KV-state Concat and the grouped-query broadcast are walked through, parameters / constants / states end a path). With ``head_size`` the
-    path may also pass the RMS norm of heads of that size; ``found`` collects it and the RoPE node that were passed, the first of each kind."""
+    path may also pass the RMS norm of heads of that size; ``found`` collects it and the RoPE node that were passed, the first of each kind, and under "turns"
+    whether a rotation may have been passed: a RoPE node, or a product of two values, of which a rotation that is no RoPE node is made."""
     found = {} if found is None else found
     seen, frontier = set(), [out_port.get_node()]
     while frontier:
@@ -164,6 +165,8 @@ def _nearest_fc_ancestor(out_port, head_size: int = 0, found: Optional[Dict] = N
                 continue
             if t == "RoPE":
                 found.setdefault("rope", n)
+            if t == "RoPE" or (t == "Multiply" and n.get_output_element_type(0).is_real() and all(_scalar(n.input_value(i).get_node()) is None for i in range(2))):
+                found["turns"] = True
             for i in range(n.get_input_size()):
                 nxt.append(n.input_value(i).get_node())
         frontier = nxt
@@ -324,6 +327,9 @@ def analyze(model: Model) -> Tuple[LlmConfig, Dict]:
                     raise NotAnLlm("rotations that differ between layers, or between queries and keys, are not served")
         if q is None or k is None or v is None:
             raise NotAnLlm("attention %d is not fed by three projections" % l)
+        for on, what in ((on_q, "queries"), (on_k, "keys")):
+            if "turns" not in on:
+                raise NotAnLlm("attention %d has %s that the position does not rotate; such layers are not served" % (l, what))
         n1 = q.input_value(0).get_node()
         if n1.get_type_name() != "RMS" or any(x.input_value(0).get_node() != n1 for x in (k, v)):
             raise NotAnLlm("the projections of attention %d do not share one RMS input" % l)

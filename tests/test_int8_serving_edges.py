@@ -1,10 +1,12 @@
-"""8-bit products in the serving program where shares of K are uneven."""
+"""Serving program: single tokens whose products share K unevenly, decoders whose rotations are not those of all heads."""
 import pytest
 import torch
 
-from openvino_b200.models import llama
+from openvino_b200.models import llama, ov_builders
 from openvino_b200.models.llm_config import TINY_LLAMA
-from test_int8_serving import INT8_LOGITS, executor, off, prefill
+from openvino_b200.models.ov_builders import build_llama
+from openvino_b200.runtime import llm_import
+from test_int8_serving import INT8_LOGITS, SMALL, executor, off, paged, prefill
 
 
 # ------------------------------------------------------------------------------------------------ single tokens whose products share K unevenly
@@ -23,3 +25,17 @@ def test_decode_steps_with_uneven_shares(ffn):
     for i in (40, 41, 42):
         assert off(prefill(ex, ids[i:i + 1].numpy(), i), want[i]) < INT8_LOGITS
     K.check_status("executor")
+
+
+# ------------------------------------------------------------------------------------------------ heads that the position does not rotate
+# the calls of _rope while a decoder of two layers is built: queries and keys of the first, then of the second
+@pytest.mark.parametrize("left_out", [(2, 3), (0, 1), (1, 3), (0, 2), (3,), (0, 1, 2, 3)])
+@pytest.mark.parametrize("in_pages", [False, True])
+@pytest.mark.parametrize("norms", [False, True])
+def test_heads_that_do_not_turn_are_refused(left_out, in_pages, norms, monkeypatch):
+    cfg = SMALL.with_(qk_norm=norms)
+    rope, count = ov_builders._rope, iter(range(100))
+    monkeypatch.setattr(ov_builders, "_rope", lambda x, c, s, D: x if next(count) in left_out else rope(x, c, s, D))
+    m = build_llama(cfg, llama.random_float_state(cfg, seed=1, std=0.05))
+    with pytest.raises(llm_import.NotAnLlm, match="does not rotate"):
+        llm_import.analyze(paged(m) if in_pages else m)
