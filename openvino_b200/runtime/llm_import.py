@@ -203,16 +203,27 @@ def _one(nodes, what: str) -> Node:
 
 
 class _Rotation:
-    """What a RoPE node and the graph behind its cosine input say: the dimensions that turn, their pairing, the table of frequencies (None where no constant
-    looks like one) and the factor of cos and sin. Scalar factors of the angles are taken into the table."""
+    """What a RoPE node and the graph behind its cosine and sine inputs say: the dimensions that turn, their pairing, the table of frequencies (None where no
+    constant looks like one) and the factor of cos and sin. Scalar factors of the angles are taken into the table."""
 
     def __init__(self, rope: Node, head_size: int):
         at = rope.get_attributes()
         self.rot = int(at.get("rotary_ndims") or head_size)
         self.interleaved = bool(at.get("is_interleaved"))
-        self.freq, self.scale = None, 1.0
-        factor, half = 1.0, self.rot // 2
-        seen, frontier = set(), [(rope.input_value(1).get_node(), False)]
+        self.freq, factor, self.scale = self._table(rope.input_value(1).get_node())
+        freq, sine_factor, scale = self._table(rope.input_value(2 if rope.get_input_size() > 2 else 1).get_node())
+        if (freq is None) != (self.freq is None) or not np.allclose([factor, self.scale], [sine_factor, scale], rtol=1e-3) \
+                or (freq is not None and not np.allclose(freq, self.freq, rtol=1e-3)):
+            raise NotAnLlm("a rotation whose sine is not that of its cosine's angle, or has another factor, is not served")
+        if self.freq is None and abs(factor - 1.0) > 1e-6:
+            raise NotAnLlm("angles with a factor, but without a table of frequencies, are not served")
+        if self.freq is not None and self.rot > 2:
+            self.freq = self.freq * factor
+
+    def _table(self, node: Node) -> Tuple[Optional[np.ndarray], float, float]:
+        """(table of frequencies, factor of the angles, factor of their cosine or sine) behind an input of the RoPE node."""
+        half, freq, factor, scale = self.rot // 2, None, 1.0, 1.0
+        seen, frontier = set(), [(node, False)]
         while frontier:
             nxt = []
             for n, of_angle in frontier:
@@ -221,21 +232,23 @@ class _Rotation:
                 seen.add(n)
                 kind = n.get_type_name()
                 if kind == "Constant":
-                    if self.freq is None and n.get_output_element_type(0).is_real() and int(np.prod(n.get_output_shape(0) or [1])) == half:
+                    if freq is None and n.get_output_element_type(0).is_real() and int(np.prod(n.get_output_shape(0) or [1])) == half:
                         v = n.get_tensor_view().to_float32().reshape(-1).astype(np.float64)
                         if np.isfinite(v).all() and (v > 0).all() and (np.diff(v) <= 0).all():
-                            self.freq = v
+                            freq = v
                     continue
+                by = 1.0
                 if kind in ("Multiply", "Divide"):
                     for i in range(2):
                         c = _scalar(n.input_value(i).get_node())
                         if c and (kind == "Multiply" or i == 1):
-                            c = c if kind == "Multiply" else 1.0 / c
-                            factor, self.scale = (factor * c, self.scale) if of_angle else (factor, self.scale * c)
-                nxt.extend((n.input_value(i).get_node(), of_angle or kind == "Cos") for i in range(n.get_input_size()))
+                            by = by * c if kind == "Multiply" else by / c
+                elif kind == "Negative" and n.get_output_element_type(0).is_real():
+                    by = -1.0
+                factor, scale = (factor * by, scale) if of_angle else (factor, scale * by)
+                nxt.extend((n.input_value(i).get_node(), of_angle or kind in ("Cos", "Sin")) for i in range(n.get_input_size()))
             frontier = nxt
-        if self.freq is not None and half > 1:
-            self.freq = self.freq * factor
+        return freq, factor, scale
 
     def same(self, other: "_Rotation") -> bool:
         if (self.rot, self.interleaved, self.freq is None) != (other.rot, other.interleaved, other.freq is None) or abs(self.scale / other.scale - 1.0) > 1e-3:

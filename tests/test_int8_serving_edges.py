@@ -1,12 +1,14 @@
 """Serving program: single tokens whose products share K unevenly, decoders whose rotations are not those of all heads."""
+import numpy as np
 import pytest
 import torch
 
+import openvino_b200 as ov
 from openvino_b200.models import llama, ov_builders
 from openvino_b200.models.llm_config import TINY_LLAMA
 from openvino_b200.models.ov_builders import build_llama
 from openvino_b200.runtime import llm_import
-from test_int8_serving import INT8_LOGITS, SMALL, executor, off, paged, prefill
+from test_int8_serving import INT8_LOGITS, SMALL, executor, feed_of, off, paged, prefill
 
 
 # ------------------------------------------------------------------------------------------------ single tokens whose products share K unevenly
@@ -39,3 +41,37 @@ def test_heads_that_do_not_turn_are_refused(left_out, in_pages, norms, monkeypat
     m = build_llama(cfg, llama.random_float_state(cfg, seed=1, std=0.05))
     with pytest.raises(llm_import.NotAnLlm, match="does not rotate"):
         llm_import.analyze(paged(m) if in_pages else m)
+
+
+# ------------------------------------------------------------------------------------------------ cosines and sines that are not of one angle
+def with_sine(monkeypatch, change):
+    sin = ov_builders.ops.sin
+    monkeypatch.setattr(ov_builders.ops, "sin", lambda a: change(sin, a))
+
+
+@pytest.mark.parametrize("name,change", [
+    ("factor of the sine", lambda sin, a: ov_builders.ops.multiply(sin(a), ov_builders.constant(np.array(1.5, np.float32)))),
+    ("other direction", lambda sin, a: ov_builders.ops.negative(sin(a))),
+    ("factor of its angles", lambda sin, a: sin(ov_builders.ops.divide(a, ov_builders.constant(np.array(2.0, np.float32))))),
+    ("angles the other way", lambda sin, a: sin(ov_builders.ops.negative(a))),
+])
+@pytest.mark.parametrize("in_pages", [False, True])
+def test_sines_that_do_not_belong_to_the_cosines_are_refused(name, change, in_pages, monkeypatch):
+    with_sine(monkeypatch, change)
+    m = build_llama(SMALL, llama.random_float_state(SMALL, seed=1, std=0.05))
+    with pytest.raises(llm_import.NotAnLlm, match="sine"):
+        llm_import.analyze(paged(m) if in_pages else m)
+
+
+def test_rotations_the_other_way_are_read(monkeypatch):
+    """Cosines and sines of negative angles: a table of negative frequencies, as the graph computes it."""
+    cos, sin = ov_builders.ops.cos, ov_builders.ops.sin
+    monkeypatch.setattr(ov_builders.ops, "cos", lambda a: cos(ov_builders.ops.negative(a)))
+    monkeypatch.setattr(ov_builders.ops, "sin", lambda a: sin(ov_builders.ops.negative(a)))
+    state = llama.random_float_state(SMALL, seed=4, std=0.05)
+    m = build_llama(SMALL, state)
+    got, _ = llm_import.analyze(m)
+    assert np.allclose(got.inv_freq(), -np.array(SMALL.inv_freq()), rtol=1e-3) and not got.plain_rotation
+    ids = np.array([[5, 9, 200, 17, 3]], dtype=np.int64)
+    want = llama.reference_logits(SMALL.with_(rope_inv_freq=got.rope_inv_freq), {k: v.float() for k, v in state.items()}, torch.tensor(ids[0])).numpy()
+    assert np.abs(ov.Core().compile_model(m, "CPU")(feed_of(ids))[0][0] - want).max() < 1e-3 * np.abs(want).max()
