@@ -1139,12 +1139,30 @@ def _written_once(t: torch.Tensor) -> bool:
     return True
 
 
+def _same_place(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Of two tensors of one shape: every element of one is in the other's place."""
+    return a is b or (a.data_ptr() == b.data_ptr() and all(n == 1 or s == t for n, s, t in zip(a.shape, a.stride(), b.stride())))
+
+
+def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """No element of [B, S, Ha, D] shares memory with one of [B, S, Hb, D] (one type, contiguous heads), by addresses and strides alone: either all of one lies
+    behind all of the other, or both keep to columns of their own in rows whose pitch divides all steps from token to token, as the parts of a fused projection do."""
+    (B, S, Ha, D), (a0, a1, a2, _), (b0, b1, b2, _), Hb = a.shape, a.stride(), b.stride(), b.shape[2]
+    a_row, b_row = (Ha - 1) * a2 + D, (Hb - 1) * b2 + D
+    behind = (b.data_ptr() - a.data_ptr()) // a.element_size()
+    if behind >= (B - 1) * a0 + (S - 1) * a1 + a_row or -behind >= (B - 1) * b0 + (S - 1) * b1 + b_row:
+        return True
+    pitch = math.gcd(*(st for n, steps in ((B, (a0, b0)), (S, (a1, b1))) if n > 1 for st in steps))
+    return pitch > 0 and a_row <= behind % pitch <= pitch - b_row
+
+
 def qk_norm_rope(q, k, positions, inv_freq, q_norm=None, k_norm=None, eps=1e-6, interleaved=False, mult=1.0, q_out=None, k_out=None):
     """RMS norm of every query and key head (where it has weights [D]) and rotation by the position, one launch. Returns (q_out, k_out).
 
     q [B, S, Hq, D] and k [B, S, Hkv, D], bf16 or fp16 (or [S, H, D]): views with any strides whose heads are contiguous; ``positions`` int32 [B, S] or [S].
     The first 2 * len(``inv_freq``) dimensions turn by positions * inv_freq (fp32; the product is formed in 64 bits), halves paired, or neighbours with
-    ``interleaved``; cos and sin are multiplied by ``mult``. The outputs may be q and k themselves."""
+    ``interleaved``; cos and sin are multiplied by ``mult``. Outputs share no memory with one another or with q and k, except that ``q_out`` may be q itself
+    and ``k_out`` k."""
     if q.ndim == 3:
         _need(k.dim() == 3 and positions.dim() == 1, "queries [S, H, D] need keys of that form and positions [S]")
         outs = qk_norm_rope(q[None], k[None], positions, inv_freq, q_norm, k_norm, eps, interleaved, mult, None if q_out is None else q_out[None],
@@ -1162,7 +1180,8 @@ def qk_norm_rope(q, k, positions, inv_freq, q_norm=None, k_norm=None, eps=1e-6, 
     if positions.dtype is not torch.int32 or positions.shape != ((B, S) if many else (S,)) or (steps[-1] != 1 and S != 1):
         raise ValueError("positions are int32 [S] or [B, S]")
     rot = _rope_operands(dtype, D, inv_freq, q_norm, k_norm)
-    if q_out is not None or k_out is not None:
+    given = q_out is not None or k_out is not None
+    if given:
         for t, like in ((q_out, q), (k_out, k)):
             if t is not None and not (t.shape == like.shape and t.dtype is dtype and _written_once(t)):
                 raise ValueError("outputs have their inputs' shape and type, and no two elements in one place")
@@ -1178,6 +1197,10 @@ def qk_norm_rope(q, k, positions, inv_freq, q_norm=None, k_norm=None, eps=1e-6, 
     ko0, ko1, ko2, ko3 = k_out.stride()
     if not (q3 == k3 == qo3 == ko3 == 1):
         raise ValueError("heads have to be contiguous")
+    if given and B * S:
+        q_there, k_there = _same_place(q_out, q), _same_place(k_out, k)
+        if not ((q_there or _apart(q_out, q)) and (k_there or _apart(k_out, k)) and _apart(q_out, k_out) and (k_there or _apart(q_out, k)) and (q_there or _apart(k_out, q))):
+            raise ValueError("outputs must not share memory with one another, with the other's input, or with a part of their own")
     if B * S:
         _call(lib().ovb_qk_norm_rope, _QK_ROPE.pack(q.data_ptr(), k.data_ptr(), 0, q_out.data_ptr(), k_out.data_ptr(), 0, 0, 0, 0, positions.data_ptr(), 0, inv_freq.data_ptr(),
                                                     0 if q_norm is None else q_norm.data_ptr(), 0 if k_norm is None else k_norm.data_ptr(), q0, q1, q2, k0, k1, k2,
@@ -1222,6 +1245,11 @@ def qk_norm_rope_kv_write(qkv, positions, slot_map, k_cache, v_cache, inv_freq, 
         oshape, (q_pitch, step) = q_out.shape, q_out.stride() if q_out.ndim == 2 else (0, 0)
         if not (step == 1 and oshape[0] == T and oshape[1] >= queries and q_out.dtype is dtype and (q_pitch >= queries or T <= 1)):
             raise ValueError("q_out has to be [%d, %d] of the type of qkv" % (T, queries))
+        # elements that q_out begins behind qkv: other memory, the queries' own place, or columns of its rows behind the heads
+        behind = (q_out.data_ptr() - qkv.data_ptr()) // 2
+        if not (T == 0 or behind >= (T - 1) * pitch + width or -behind >= (T - 1) * q_pitch + queries or
+                ((q_pitch == pitch or T == 1) and (behind == 0 or (T > 1 and width <= behind % pitch <= pitch - queries)))):
+            raise ValueError("q_out has to be the queries' place or memory that the heads of qkv do not use")
     d = _one_device(qkv, positions, slot_map, k_cache, v_cache, inv_freq, q_norm, k_norm, q_out, k_meta if u8 else None, v_meta if u8 else None)
     if T:
         at = qkv.data_ptr()

@@ -104,3 +104,88 @@ def test_one_normed_token_with_uneven_shares(K, N, Kd):
     pick = torch.ones(1, dtype=torch.int32, device="cuda")
     assert torch.equal(K.gemm(many, pw, out_f32=True, norm=(gamma, 1e-5, pick)), got)
     K.check_status("gemm_i8")
+
+
+# ------------------------------------------------------------------------------------------------ outputs that share memory (host)
+def elements(t):
+    """Addresses of all elements, in elements of the tensor's storage."""
+    at = torch.tensor(t.storage_offset())
+    for n, st in zip(t.shape, t.stride()):
+        at = at.unsqueeze(-1) + torch.arange(n) * st
+    return set(at.reshape(-1).tolist())
+
+
+def views(B, S, D, H, other):
+    """Views [B, S, H, D] of one buffer: fused rows, in several orders of dimensions, at several places."""
+    buf = torch.zeros(4 * B * S * (H + other) * D + 64)
+    W = (H + other) * D
+    for off in (0, D, H * D, other * D, W, B * S * H * D, B * S * W, 7):
+        yield buf.as_strided((B, S, H, D), (S * W, W, D, 1), off)
+        yield buf.as_strided((B, S, H, D), (S * H * D, D, S * D, 1), off)
+        yield buf.as_strided((B, S, H, D), (S * H * D, H * D, D, 1), off)
+        yield buf.as_strided((B, S, H, D), (W, B * W, D, 1), off)
+
+
+@pytest.mark.parametrize("B,S,D", [(1, 1, 4), (1, 3, 4), (2, 1, 4), (2, 3, 4)])
+def test_places_apart_are_told_by_strides(B, S, D):
+    """`_apart` never calls views apart that share an element, and knows the parts of fused rows."""
+    from openvino_b200.ops import cuda as K
+    seen = 0
+    for a in views(B, S, D, 2, 3):
+        base = a.untyped_storage().data_ptr()
+        mine = elements(a)
+        whole = torch.empty(0).set_(a.untyped_storage())
+        for st, off in {(v.stride(), v.storage_offset()) for v in views(B, S, D, 3, 2)}:
+            b = whole.as_strided((B, S, 3, D), st, off)
+            assert b.untyped_storage().data_ptr() == base
+            if K._apart(a, b):
+                seen += 1
+                assert not mine & elements(b), (a.stride(), a.storage_offset(), st, off)
+    assert seen
+    fused = torch.zeros((B, S, 8 * D))
+    q, k, v = (fused[..., c * D:(c + n) * D].view(B, S, n, D) for c, n in ((0, 4), (4, 2), (6, 2)))
+    assert K._apart(q, k) and K._apart(k, q) and K._apart(v, q) and K._apart(k, v) and not K._apart(q, q) and not K._apart(q, fused[..., 3 * D:5 * D].view(B, S, 2, D))
+
+
+@pytest.mark.gpu
+def test_outputs_that_share_memory_are_refused(K):
+    g = gen(1)
+    rows = torch.randn((2, 5, 8 * 64), generator=g, device="cuda").bfloat16()
+    part = lambda t, c, n: t[..., c * 64:(c + n) * 64].view(2, 5, n, 64)
+    q, k = part(rows, 0, 4), part(rows, 4, 4)
+    pos, f = torch.arange(5, dtype=torch.int32, device="cuda"), torch.ones(32, device="cuda")
+    want = [t.clone() for t in K.qk_norm_rope(q, k, pos, f)]
+    other = torch.empty_like(rows)
+    for q_out, k_out in ((k, None), (None, q), (k, q), (q, q), (part(rows, 1, 4), None), (None, part(rows, 3, 4)), (part(other, 0, 4), part(other, 3, 4)), (part(other, 0, 4), part(other, 0, 4)),
+                         (q, part(rows, 3, 4)), (k.clone().flip(0)[:0], None)):
+        with pytest.raises(ValueError):
+            K.qk_norm_rope(q, k, pos, f, q_out=q_out, k_out=k_out)
+    with pytest.raises(ValueError):
+        K.qk_norm_rope(q, q, pos, f, q_out=q, k_out=part(other, 0, 4))                  # keys that are read while the queries in their place are written
+    got = K.qk_norm_rope(q, k, pos, f, q_out=part(other, 0, 4), k_out=part(other, 4, 4))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    same = rows.clone()
+    K.qk_norm_rope(part(same, 0, 4), part(same, 4, 4), pos, f, q_out=part(same, 0, 4), k_out=part(same, 4, 4))
+    assert torch.equal(part(same, 0, 4), want[0]) and torch.equal(part(same, 4, 4), want[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 6])
+def test_append_keeps_queries_off_the_heads_it_reads(K, T):
+    g, Hq, Hkv, D = gen(2), 4, 2, 64
+    wide = torch.randn((T, 16 * D), generator=g, device="cuda").bfloat16()
+    pos, slots, f = torch.arange(T, dtype=torch.int32, device="cuda"), torch.arange(T, dtype=torch.int32, device="cuda"), torch.ones(32, device="cuda")
+    kc, vc = (torch.zeros((1, Hkv, 16, D), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    run = lambda rows, q_out: K.qk_norm_rope_kv_write(rows, pos, slots, kc, vc, f, Hq, Hkv, D, 16, q_out=q_out)
+    want = torch.empty((T, Hq * D), dtype=torch.bfloat16, device="cuda")
+    run(wide[:, :8 * D], want)
+    for at in (1, 4, 6, 7):                                                             # over keys, values and a part of the queries
+        with pytest.raises(ValueError):
+            run(wide[:, :8 * D], wide[:, at * D:(at + 4) * D])
+    for at in (0, 8, 12):                                                               # the queries' place, columns behind the heads
+        rows = wide.clone()
+        run(rows[:, :8 * D], rows[:, at * D:(at + 4) * D])
+        assert torch.equal(rows[:, at * D:(at + 4) * D], want)
+    rows = torch.cat([wide, wide])
+    run(rows[:T, :8 * D], rows[T:, :4 * D])                                             # rows behind the last
+    assert torch.equal(rows[T:, :4 * D], want)
