@@ -398,13 +398,13 @@ static int launch_i8_tile(int form, const cudaLaunchConfig_t& cfg, const CUtenso
 // take a microsecond each, one behind the other (4 x 4096 x 4096 10.5 / 8.5).
 // Every CTA reads the whole row at a time of its own, so a result in the row's place has it quantised first, by a launch of its own.
 constexpr int64_t kI8FusedWeights = 64 << 20;       // bytes
+static bool i8_fused_size(int T, int N, int K) { return T == 1 && (int64_t)N * K <= kI8FusedWeights && K % 8 == 0 && K <= kI8QuantWarps * 32 * kI8Hold * 8; }
 static bool i8_fuses(const ovb_gemm_i8_args* a) {
     const auto bits = [](const void* x) { return reinterpret_cast<uintptr_t>(x); };
     const uintptr_t rows = a->row_idx != nullptr ? ((uintptr_t)(a->raw_rows - 1) * (uintptr_t)a->ld_raw + (uintptr_t)a->K) * 2 : (uintptr_t)a->K * 2;
     const uintptr_t result = (uintptr_t)(is_gated(a->act) ? a->N / 2 : a->N) * (a->out_f32 ? 4 : 2);
     const bool apart = bits(a->out) >= bits(a->raw) + rows || bits(a->raw) >= bits(a->out) + result;
-    return apart && a->raw != nullptr && a->T == 1 && (int64_t)a->N * a->K <= kI8FusedWeights && a->K % 8 == 0 && a->K <= kI8QuantWarps * 32 * kI8Hold * 8 && (a->row_idx == nullptr || a->ld_raw % 8 == 0) &&
-           ((bits(a->raw) | bits(a->gamma)) & 15) == 0;
+    return apart && a->raw != nullptr && i8_fused_size(a->T, a->N, a->K) && (a->row_idx == nullptr || a->ld_raw % 8 == 0) && ((bits(a->raw) | bits(a->gamma)) & 15) == 0;
 }
 
 // How a product is run: pairs of CTAs, or tiles of `bt` tokens whose K is shared by `splits` CTAs, with `room` KB of shared memory each (108: two to an SM).
@@ -531,6 +531,8 @@ int ovb_pack_i8(const void* w, int is_unsigned, void* w_out, int N, int K, int64
     OVB_CHECK_CUDA(launch_serial(pack_i8_kernel, dim3((unsigned)chunks), dim3(256), 0, stream, (const uint8_t*)w, (uint4*)w_out, N, K, ldw, KB, is_unsigned ? 0x80 : 0));
     return 0;
 }
+
+int ovb_gemm_i8_launches(int T, int N, int K) { return ovb::i8_fused_size(T, N, K) ? 1 : 2; }
 
 int ovb_gemm_i8(const ovb_gemm_i8_args* a, ovb_stream_t stream_) {
     using namespace ovb;

@@ -178,6 +178,8 @@ typedef struct {
     float act_limit, act_slope, act_shift, eps;
 } ovb_gemm_i8_args;
 int ovb_gemm_i8(const ovb_gemm_i8_args* a, ovb_stream_t stream);
+// Kernels that a product of 16-bit rows launches: one where it quantises a single row itself (rows and norm 16-byte aligned, the result in another place), else two.
+int ovb_gemm_i8_launches(int T, int N, int K);
 
 // ---------------------------------------------------------------------------------------------
 // Normalisation / elementwise

@@ -483,6 +483,11 @@ def quantize_rows(x: torch.Tensor, norm=None) -> QuantizedRows:
     return QuantizedRows(q, scales, sums, x.dtype)
 
 
+def gemm_i8_launches(T: int, w: "PackedWeight") -> int:
+    """Kernels that ``gemm`` launches for ``T`` 16-bit rows (16-byte aligned, not in the result's place) and a weight of ``from_ir_i8``."""
+    return lib().ovb_gemm_i8_launches(C.c_int(T), C.c_int(w.N), C.c_int(w.K))
+
+
 def _gemm_i8(x, w: "PackedWeight", out, residual, act, out_f32, glu, cap, norm) -> torch.Tensor:
     N, Kd, wt, bias, zps = w.N, w.K, w.w, w.bias, w.zps
     gamma = idx = None

@@ -425,6 +425,11 @@ class CudaLlmExecutor(LlmExecutor):
         self.int8 = any(p is not None and p.mode == K.W_I8 for lw in weights.layers for p in (lw.qkv, lw.o, lw.gate_up, lw.down)) or weights.lm_head.mode == K.W_I8
         if self.int8 and self.tp_size > 1:
             raise ValueError("products of whole numbers are not summed over tensor-parallel ranks: compile the model without DYNAMIC_QUANTIZATION_GROUP_SIZE")
+        # Launches that products of whole numbers add to (or take from) the sequence of norms and products that `_forward` counts, for one row and for several. Rows
+        # are quantised with their norm in one launch, or in the product's; the vocabulary's product also gathers its rows.
+        counts = [(p, normed) for lw in weights.layers for p, normed in ((lw.qkv, 1), (lw.o, 0), (lw.gate_up, int(not cfg.num_experts)), (lw.down, 0)) if p is not None and p.mode == K.W_I8]
+        self.int8_layer_launches = [sum(K.gemm_i8_launches(rows, p) - 1 - normed for p, normed in counts) for rows in (1, 2)]
+        self.int8_head_launches = [K.gemm_i8_launches(rows, weights.lm_head) - 3 if weights.lm_head.mode == K.W_I8 else 0 for rows in (1, 2)]
         # frequencies of the rotation, for the models that the rotation of whole heads by powers of one base does not serve
         self.inv_freq = None if cfg.plain_rotation else torch.tensor(cfg.inv_freq(), dtype=torch.float32, device=self.device)
         # KV_CACHE_PRECISION = u8: rows are stored as bytes with one fp16 (scale, zero point) pair per (block, head, slot):
@@ -520,10 +525,7 @@ class CudaLlmExecutor(LlmExecutor):
             K.rmsnorm(last_h, w.final_norm, cfg.rms_eps, out=last_x)
             K.gemm(last_x, w.lm_head, out=logits, ws=ws)
         self._sample(sb, B)
-        # with products of whole numbers: rows are quantised with their norm in one launch (the output and down projections need one more each); a single
-        # token's rows in none
-        n += 0 if not self.int8 else (2 if T > 1 else -2) * cfg.num_layers - 1 - (B == 1)
-        self.kernel_launches += n + 5
+        self.kernel_launches += n + 5 + self.int8_layer_launches[T > 1] + self.int8_head_launches[B > 1]
 
     def _normed(self, h: torch.Tensor, norm: torch.Tensor, x: torch.Tensor, wt: K.PackedWeight, out: torch.Tensor, act: int = K.ACT_NONE) -> None:
         """The product of the normed rows of ``h``; ``x``: room for them where the product does not norm them itself."""

@@ -189,3 +189,31 @@ def test_append_keeps_queries_off_the_heads_it_reads(K, T):
     rows = torch.cat([wide, wide])
     run(rows[:T, :8 * D], rows[T:, :4 * D])                                             # rows behind the last
     assert torch.equal(rows[T:, :4 * D], want)
+
+
+# ------------------------------------------------------------------------------------------------ launches that are counted
+def kernels_of(call):
+    """Kernel nodes of a captured call."""
+    from cuda.bindings import runtime as rt
+    call()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(g):
+        call()
+    raw = rt.cudaGraph_t(g.raw_cuda_graph())
+    err, nodes, n = rt.cudaGraphGetNodes(raw, 0)
+    assert int(err) == 0
+    err, nodes, n = rt.cudaGraphGetNodes(raw, n)
+    assert int(err) == 0
+    kinds = [rt.cudaGraphNodeGetType(node) for node in nodes[:n]]
+    return sum(kind == rt.cudaGraphNodeType.cudaGraphNodeTypeKernel for _, kind in kinds)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,Kd", [(256, 512), (4096, 16384), (4224, 16384), (28672, 4096), (128, 500), (128, 16392)])
+@pytest.mark.parametrize("T", [1, 2, 300])
+def test_launches_are_told(K, T, N, Kd):
+    w = torch.randint(-128, 128, (N, Kd), generator=gen(1), device="cuda", dtype=torch.int8)
+    pw = K.PackedWeight.from_ir_i8(w, torch.full((N,), 0.01, device="cuda"))
+    x = torch.randn((T, Kd), generator=gen(2), device="cuda").bfloat16()
+    assert kernels_of(lambda: K.gemm(x, pw)) == K.gemm_i8_launches(T, pw)

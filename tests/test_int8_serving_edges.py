@@ -75,3 +75,28 @@ def test_rotations_the_other_way_are_read(monkeypatch):
     ids = np.array([[5, 9, 200, 17, 3]], dtype=np.int64)
     want = llama.reference_logits(SMALL.with_(rope_inv_freq=got.rope_inv_freq), {k: v.float() for k, v in state.items()}, torch.tensor(ids[0])).numpy()
     assert np.abs(ov.Core().compile_model(m, "CPU")(feed_of(ids))[0][0] - want).max() < 1e-3 * np.abs(want).max()
+
+
+# ------------------------------------------------------------------------------------------------ launches of a step
+@pytest.mark.gpu
+@pytest.mark.parametrize("hidden,ffn,vocab", [(256, 512, 512), (4096, 8448, 512), (256, 512, 262208)])
+def test_launches_of_a_step_are_counted(hidden, ffn, vocab):
+    """The kernels of a step of one token and of several: those of the same decoder in 16 bits, and what its products launch more or less. Weights above 64 MB are
+    not multiplied in the launch that quantises their row. (The attention is the same in both: its launches cancel.)"""
+    from openvino_b200.ops import cuda as K
+    from openvino_b200.runtime.cuda_llm import CudaLlmExecutor, LlmWeights, StepShape
+    from test_int8_edges import kernels_of
+    kernels, counted = {}, {}
+    for name, more in (("whole numbers", dict(weight_format="int8", int8_activations=True, group_size=0)), ("16 bits", dict(weight_format="bf16"))):
+        cfg = TINY_LLAMA.with_(qk_norm=True, hidden_size=hidden, ffn_size=ffn, vocab_size=vocab, **more)
+        ex = CudaLlmExecutor(cfg, LlmWeights.random(cfg, "cuda"), num_kv_blocks=64, max_batch_tokens=16, max_seqs=4, use_cuda_graphs=False)
+        for n in (1, 9):
+            ids = np.arange(n)
+            prefill(ex, ids)
+            before = ex.kernel_launches
+            ex._forward(ex.prefill, StepShape(n, 1, n, n))
+            counted[name, n] = ex.kernel_launches - before
+            kernels[name, n] = kernels_of(lambda: ex._forward(ex.prefill, StepShape(n, 1, n, n)))
+    for n in (1, 9):
+        assert counted["whole numbers", n] - counted["16 bits", n] == kernels["whole numbers", n] - kernels["16 bits", n]
+    K.check_status("executor")
