@@ -472,6 +472,7 @@ def quantize_rows(x: torch.Tensor, norm=None) -> QuantizedRows:
 
     ``norm`` (weights, eps[, row indices]): RMS norm of the rows (of the indexed rows) of ``x`` first, in 32 bits. A row without a value of at least 2^-119 is
     zero; one with a value that is not finite has the scale NaN, and so have all products with it (with a norm: a value of the row times its weight)."""
+    _need(isinstance(x, torch.Tensor), "rows of 16-bit values are expected, not %s", type(x).__name__)
     T, gamma, eps, idx = _raw_rows(x, norm)
     d = _one_device(x, gamma, idx)
     cols = x.shape[1]
@@ -575,6 +576,7 @@ def gemm(x: torch.Tensor, w: PackedWeight, out: Optional[torch.Tensor] = None, r
     if w.mode == W_I8:
         _need(comm is None and not splits and not block_t, "products of whole numbers take no communicator, split count or token tile")
         return _gemm_i8(x, w, out, residual, act, out_f32, glu, cap, norm)
+    _need(not isinstance(x, QuantizedRows), "quantised rows are for weights of from_ir_i8")
     assert x.dim() == 2 and x.stride(1) == 1
     if norm is not None and len(norm) > 2:
         T, K = norm[2].numel(), x.shape[1]

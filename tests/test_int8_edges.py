@@ -217,3 +217,14 @@ def test_launches_are_told(K, T, N, Kd):
     pw = K.PackedWeight.from_ir_i8(w, torch.full((N,), 0.01, device="cuda"))
     x = torch.randn((T, Kd), generator=gen(2), device="cuda").bfloat16()
     assert kernels_of(lambda: K.gemm(x, pw)) == K.gemm_i8_launches(T, pw)
+
+
+# ------------------------------------------------------------------------------------------------ operands that do not belong together (host)
+def test_quantised_rows_are_refused_where_rows_are_expected():
+    from openvino_b200.ops import cuda as K
+    rows = K.QuantizedRows(torch.zeros((4, 64), dtype=torch.int8), torch.ones(4), torch.zeros(4, dtype=torch.int32), torch.bfloat16)
+    for mode in (K.W_BF16, K.W_U8, K.W_F32):
+        with pytest.raises(ValueError):
+            K.gemm(rows, K.PackedWeight(mode, torch.zeros((128, 64)).bfloat16(), 128, 64))
+    with pytest.raises(ValueError):
+        K.quantize_rows(rows)
