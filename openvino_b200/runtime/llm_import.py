@@ -42,6 +42,10 @@ class _Linear:
             w = w.input_value(0).get_node()
         if w.get_type_name() != "Constant":
             raise NotAnLlm("weight of %s is not a constant" % fc.get_friendly_name())
+        bias = fc.input_value(2).get_node() if fc.get_input_size() > 2 else None
+        adds = [c for c in _consumers(fc) if c.get_type_name() == "Add"]
+        if bias is not None and (bias.get_type_name() != "Constant" or _adds_something(bias)) or any(_adds_something(c.input_value(i).get_node()) for c in adds for i in range(2)):
+            raise NotAnLlm("the bias of %s is not served" % fc.get_friendly_name())
         self.compressed = t == "FullyConnectedCompressed"
         view = w.get_tensor_view()
         self.N = view.shape[0]
@@ -143,8 +147,9 @@ _DEAD_ENDS = ("Parameter", "Constant", "ReadValue", "Result", "Assign")
 def _nearest_fc_ancestor(out_port, head_size: int = 0, found: Optional[Dict] = None) -> Optional[Node]:
     """Closest FullyConnected node that feeds ``out_port`` (breadth first over all data inputs; shape plumbing, RoPE, the
     KV-state Concat and the grouped-query broadcast are walked through, parameters / constants / states end a path). With ``head_size`` the
-    path may also pass the RMS norm of heads of that size; ``found`` collects it and the RoPE node that were passed, the first of each kind, and under "turns"
-    whether a rotation may have been passed: a RoPE node, or a product of two values, of which a rotation that is no RoPE node is made."""
+    path may also pass the RMS norm of heads of that size; ``found`` collects it and the RoPE node that were passed, the first of each kind, under "turns"
+    whether a rotation may have been passed (a RoPE node, or a product of two values, of which a rotation that is no RoPE node is made), and under "added" an
+    Add of a constant."""
     found = {} if found is None else found
     seen, frontier = set(), [out_port.get_node()]
     while frontier:
@@ -167,10 +172,19 @@ def _nearest_fc_ancestor(out_port, head_size: int = 0, found: Optional[Dict] = N
                 found.setdefault("rope", n)
             if t == "RoPE" or (t == "Multiply" and n.get_output_element_type(0).is_real() and all(_scalar(n.input_value(i).get_node()) is None for i in range(2))):
                 found["turns"] = True
+            if t == "Add" and n.get_output_element_type(0).is_real() and any(_adds_something(n.input_value(i).get_node()) for i in range(2)):
+                found["added"] = n
             for i in range(n.get_input_size()):
                 nxt.append(n.input_value(i).get_node())
         frontier = nxt
     return None
+
+
+def _adds_something(n: Node) -> bool:
+    """A constant (behind a Convert) that is not zero."""
+    if n.get_type_name() == "Convert":
+        n = n.input_value(0).get_node()
+    return n.get_type_name() == "Constant" and bool(np.any(n.get_tensor_view().to_float32()))
 
 
 def _consumers(node: Node, port: int = 0):
@@ -327,7 +341,8 @@ def analyze(model: Model) -> Tuple[LlmConfig, Dict]:
         D = _head_size(a)
         on_q: Dict = {}
         on_k: Dict = {}
-        q, k, v = _nearest_fc_ancestor(a.input_value(0), D, on_q), _nearest_fc_ancestor(a.input_value(1), D, on_k), _nearest_fc_ancestor(a.input_value(2))
+        on_v: Dict = {}
+        q, k, v = _nearest_fc_ancestor(a.input_value(0), D, on_q), _nearest_fc_ancestor(a.input_value(1), D, on_k), _nearest_fc_ancestor(a.input_value(2), 0, on_v)
         for key, on, projection in (("q_norm", on_q, q), ("k_norm", on_k, k)):
             norm = _head_norm(on, projection)
             if norm is not None:
@@ -340,6 +355,8 @@ def analyze(model: Model) -> Tuple[LlmConfig, Dict]:
                     raise NotAnLlm("rotations that differ between layers, or between queries and keys, are not served")
         if q is None or k is None or v is None:
             raise NotAnLlm("attention %d is not fed by three projections" % l)
+        if any("added" in on for on in (on_q, on_k, on_v)):
+            raise NotAnLlm("attention %d has projections with biases, which are not served" % l)
         for on, what in ((on_q, "queries"), (on_k, "keys")):
             if "turns" not in on:
                 raise NotAnLlm("attention %d has %s that the position does not rotate; such layers are not served" % (l, what))

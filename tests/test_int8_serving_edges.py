@@ -100,3 +100,25 @@ def test_launches_of_a_step_are_counted(hidden, ffn, vocab):
     for n in (1, 9):
         assert counted["whole numbers", n] - counted["16 bits", n] == kernels["whole numbers", n] - kernels["16 bits", n]
     K.check_status("executor")
+
+
+# ------------------------------------------------------------------------------------------------ biases
+@pytest.mark.parametrize("which", ["q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj", "down_proj"])
+@pytest.mark.parametrize("compress", [None, "int8"])
+@pytest.mark.parametrize("value", [0.0, 0.7])
+def test_projections_with_biases_are_refused(which, compress, value, monkeypatch):
+    """The serving program adds none; one of zeros adds nothing, where the graph's form lets it be seen."""
+    matmul = ov_builders.ops.matmul
+
+    def biased(*a, **kw):
+        r = matmul(*a, **kw)
+        if not str(kw.get("name") or "").endswith(which):
+            return r
+        return ov_builders.ops.add(r, ov_builders.constant(np.full((1, 1, r.output(0).get_partial_shape()[2].get_length()), value, np.float32)))
+    monkeypatch.setattr(ov_builders.ops, "matmul", biased)
+    m = build_llama(SMALL.with_(group_size=0), llama.random_float_state(SMALL, seed=1, std=0.05), compress=compress)
+    if value == 0.0 and which in ("q_proj", "k_proj", "v_proj"):
+        assert llm_import.analyze(m)[0].num_layers == 2
+    elif value:
+        with pytest.raises(llm_import.NotAnLlm):
+            llm_import.analyze(m)
