@@ -144,3 +144,26 @@ def test_one_scale_for_a_whole_weight_in_the_serving_import(monkeypatch):
     _, parts = llm_import.analyze(build_llama(cfg, llama.random_float_state(cfg, seed=1, std=0.05), compress="int8"))
     for v in list(parts["lin"].values()) + [parts["lm_head"]]:
         assert v.whole_rows and v.scales.shape == (v.N, 1) and bool((v.scales == float(np.float16(0.01))).all()) and v.zp.shape == (v.N, 1)
+
+
+# ------------------------------------------------------------------------------------------------ weights, scales and zero points that are inputs
+@pytest.mark.parametrize("inputs", [("w",), ("s",), ("z",), ("w", "s", "z"), ()])
+def test_inputs_of_compressed_products_are_those_of_the_call(inputs):
+    """The body of a folded block is called with the weights of one block after the other; nothing that was expanded for one call serves another."""
+    from openvino_b200.runtime.cuda_plugin import GraphProgram
+    rng = np.random.default_rng(5)
+    N, Kd = 24, 64
+
+    def values():
+        return {"w": rng.integers(0, 256, (N, Kd)).astype(np.uint8), "s": (rng.random((N, 1)) / 50).astype(np.float32), "z": rng.integers(100, 150, (N, 1)).astype(np.uint8)}
+    fixed = values()
+    x = ops.parameter([-1, Kd], "f32", "x")
+    nodes = {n: ops.parameter(list(v.shape), "f32" if n == "s" else "u8", n) if n in inputs else ops.constant(v) for n, v in fixed.items()}
+    fc = ops.fully_connected_compressed(x, nodes["w"], ops.constant(np.zeros(0, np.float32)), nodes["s"], nodes["z"])
+    prog = GraphProgram(ov.Model([ops.result(fc)], [x] + [nodes[n] for n in inputs], "block"), "cpu")
+    for _ in range(3):
+        v = {**fixed, **{n: t for n, t in values().items() if n in inputs}}
+        a = rng.standard_normal((5, Kd)).astype(np.float32)
+        got = prog.run([torch.from_numpy(a)] + [torch.from_numpy(v[n]) for n in inputs])[0].numpy()
+        w64 = (v["w"].astype(np.float64) - v["z"]) * v["s"]
+        assert np.abs(got - a @ w64.T).max() <= (Kd + 4) * 2.0 ** -24 * (np.abs(a) @ np.abs(w64).T).max()
