@@ -470,7 +470,8 @@ def _raw_rows(x: torch.Tensor, norm):
 def quantize_rows(x: torch.Tensor, norm=None) -> QuantizedRows:
     """bf16 or fp16 rows -> signed bytes: with a = max |row|, code = round(value * (127 / a)), halves to even, scale = a / 127.
 
-    ``norm`` (weights, eps[, row indices]): RMS norm of the rows (of the indexed rows) of ``x`` first, in 32 bits. A row without a value of at least 2^-119 is
+    ``norm`` (weights, eps[, row indices]): RMS norm of the rows (of the indexed rows) of ``x`` first, in 32 bits; its sum of squares is taken in an order that goes by the
+    width and the number of rows, so the scales (not the codes) of one row may differ in their last bits between calls of other sizes. A row without a value of at least 2^-119 is
     zero; one with a value that is not finite has the scale NaN, and so have all products with it (with a norm: a value of the row times its weight)."""
     _need(isinstance(x, torch.Tensor), "rows of 16-bit values are expected, not %s", type(x).__name__)
     T, gamma, eps, idx = _raw_rows(x, norm)
@@ -1244,23 +1245,24 @@ def qk_norm_rope_kv_write(qkv, positions, slot_map, k_cache, v_cache, inv_freq, 
             _need(t is not None and t.dtype == torch.float16 and t.shape == (blocks, Hkv, block_size, 2) and t.is_contiguous(),
                   "a uint8 cache needs fp16 tables [num_blocks, %d, %d, 2]", Hkv, block_size)
     rot = _rope_operands(dtype, D, inv_freq, q_norm, k_norm)
+    at = qkv.data_ptr()
     if q_out is None:
         if T > 1 and pitch < width:
             raise ValueError("rows that are written in place must not overlap")
-        q_out, q_pitch = qkv, pitch
+        q_out, q_pitch, q_at = qkv, pitch, at
     else:
         oshape, (q_pitch, step) = q_out.shape, q_out.stride() if q_out.ndim == 2 else (0, 0)
         if not (step == 1 and oshape[0] == T and oshape[1] >= queries and q_out.dtype is dtype and (q_pitch >= queries or T <= 1)):
             raise ValueError("q_out has to be [%d, %d] of the type of qkv" % (T, queries))
         # elements that q_out begins behind qkv: other memory, the queries' own place, or columns of its rows behind the heads
-        behind = (q_out.data_ptr() - qkv.data_ptr()) // 2
+        q_at = q_out.data_ptr()
+        behind = (q_at - at) // 2
         if not (T == 0 or behind >= (T - 1) * pitch + width or -behind >= (T - 1) * q_pitch + queries or
                 ((q_pitch == pitch or T == 1) and (behind == 0 or (T > 1 and width <= behind % pitch <= pitch - queries)))):
             raise ValueError("q_out has to be the queries' place or memory that the heads of qkv do not use")
     d = _one_device(qkv, positions, slot_map, k_cache, v_cache, inv_freq, q_norm, k_norm, q_out, k_meta if u8 else None, v_meta if u8 else None)
     if T:
-        at = qkv.data_ptr()
-        _call(lib().ovb_qk_norm_rope, _QK_ROPE.pack(at, at + queries * 2, at + (Hq + Hkv) * D * 2, q_out.data_ptr(), 0, k_cache.data_ptr(), v_cache.data_ptr(),
+        _call(lib().ovb_qk_norm_rope, _QK_ROPE.pack(at, at + queries * 2, at + (Hq + Hkv) * D * 2, q_at, 0, k_cache.data_ptr(), v_cache.data_ptr(),
                                                     k_meta.data_ptr() if u8 else 0, v_meta.data_ptr() if u8 else 0, positions.data_ptr(), slot_map.data_ptr(), inv_freq.data_ptr(),
                                                     0 if q_norm is None else q_norm.data_ptr(), 0 if k_norm is None else k_norm.data_ptr(), 0, pitch, D, 0, pitch, D, 0, pitch, D,
                                                     0, q_pitch, D, 0, 0, 0, 0, blocks * block_size, 1, T, Hq, Hkv, D, rot, block_size, 1 if interleaved else 0,
