@@ -57,7 +57,8 @@ __device__ __forceinline__ void i8_quantize_row(const I8TileParams& p, uint8_t* 
         x[h] = at < pieces ? __ldcg(src + at) : make_uint4(0, 0, 0, 0);
         g[h] = p.gamma != nullptr && at < pieces ? __ldg(static_cast<const uint4*>(p.gamma) + at) : make_uint4(0, 0, 0, 0);
     }
-    // sums in the order of ovb_quantize_rows for few rows of up to 4096 columns
+    // The sum of squares has the order of ovb_quantize_rows for few rows of 1025 to 4096 columns. Narrower and wider rows are shared by other numbers of warps there: the
+    // codes are the same, the norm's factor and with it the row's scale may differ in their last bits.
     const bool norm = p.gamma != nullptr;
     uint32_t top = 0;
     uint64_t ss2 = pair_of(0.f);

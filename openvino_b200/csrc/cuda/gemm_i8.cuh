@@ -3,7 +3,7 @@
 //   out[t, n] = act((sum_k x[t, k] w[n, k] - zp[n] * sum_k x[t, k]) * x_scale[t] * w_scale[n] + bias[n]) + residual[t, n]
 //
 // x and w are signed bytes, zp is a byte's zero point in the same signed form. The sums are exact: with K <= kI8MaxK both terms together stay below 2^31
-// (|x| <= 127, |w|, |zp| <= 128), so a sum that is split over CTAs has the same value in any order, and every kernel of this family gives the same integers.
+// (|x| <= 127, |w|, |zp| <= 128), so a sum that is split over CTAs has the same value in any order, and every kernel of this family gives the same integers for the same codes.
 #pragma once
 #include "gemm_common.cuh"
 

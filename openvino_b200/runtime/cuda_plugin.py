@@ -1806,7 +1806,7 @@ class CudaConfig(PluginConfig):
         self.register(ConfigOption(props.hint.kv_cache_precision, "bf16", "element type of the paged KV cache: bf16 | f16 | u8",
                                    lambda v: str(v).lower() in ("bf16", "f16", "u8", "dynamic"), R))
         self.register(ConfigOption(props.hint.dynamic_quantization_group_size, 0, "activations that share a scale in products with 8-bit weights of one scale per channel, "
-                                   "which then run in whole numbers: 0 = off, -1 or a size that covers the row = one scale per row", lambda v: v >= -1, R))
+                                   "which then run in whole numbers: 0 = off, -1 or a size that covers the row (the serving program: the longest row of all weights) = one scale per row", lambda v: v >= -1, R))
         self.register(ConfigOption(props.cuda.use_cuda_graphs, True, "capture decode steps of the serving program in CUDA graphs", None, R))
         self.register(ConfigOption(props.cuda.serving_program, False, "compile a decoder-only LLM graph into the serving program", None, R))
         self.register(ConfigOption(props.cuda.tensor_parallel_size, 0, "ranks of the tensor-parallel group (0 = the process group's size)", lambda v: 0 <= v <= 8, R))

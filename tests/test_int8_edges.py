@@ -228,3 +228,32 @@ def test_quantised_rows_are_refused_where_rows_are_expected():
             K.gemm(rows, K.PackedWeight(mode, torch.zeros((128, 64)).bfloat16(), 128, 64))
     with pytest.raises(ValueError):
         K.quantize_rows(rows)
+
+
+def test_packed_structures_are_as_long_as_the_librarys():
+    """The formats that calls are packed with, and the same structures field by field."""
+    import ctypes as C
+    from openvino_b200.ops import cuda as K
+    for packed, fields in ((K._QUANT_ROWS, K.QuantRowsArgs), (K._GEMM_I8, K.GemmI8Args), (K._QK_ROPE, K.QkRopeArgs)):
+        assert packed.size == C.sizeof(fields)
+        values = [i + 1 for i in range(len(fields._fields_))]
+        raw = fields.from_buffer_copy(packed.pack(*values))
+        assert [getattr(raw, f[0]) for f in fields._fields_] == values
+
+
+# ------------------------------------------------------------------------------------------------ rows whichever kernel quantises them
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", [700, 2048, 4100, 8192, 14336])
+def test_rows_among_few_and_many(K, cols):
+    """From 512 rows on other kernels quantise them. Without a norm the bits are the same; with one the codes and their sums are, and the scales are as far apart as two
+    sums of squares of `cols` terms may be, 2 cols U, half of that behind the root, next to eight roundings on each side."""
+    x = torch.randn((512, cols), generator=gen(cols), device="cuda").bfloat16()
+    gamma = (1 + 0.3 * torch.randn(cols, generator=gen(2), device="cuda")).bfloat16()
+    for norm in (None, (gamma, 1e-5)):
+        few, many, one = K.quantize_rows(x[:511], norm=norm), K.quantize_rows(x, norm=norm), K.quantize_rows(x[7:8], norm=norm)
+        assert torch.equal(few.q, many.q[:511]) and torch.equal(few.sums, many.sums[:511]) and torch.equal(one.q, many.q[7:8])
+        if norm is None:
+            assert torch.equal(few.scales, many.scales[:511])
+        else:
+            assert bool(((few.scales - many.scales[:511]).double().abs() <= (cols + 16) * U * few.scales.double()).all())
+    K.check_status("quantize_rows")
