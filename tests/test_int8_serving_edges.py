@@ -122,3 +122,35 @@ def test_projections_with_biases_are_refused(which, compress, value, monkeypatch
     elif value:
         with pytest.raises(llm_import.NotAnLlm):
             llm_import.analyze(m)
+
+
+# ------------------------------------------------------------------------------------------------ neighbours paired
+def neighbours(x, cos, sin, D):
+    """The rotation of neighbouring pairs as graphs write it, from the builder's tables of halves side by side."""
+    ops, _i64 = ov_builders.ops, ov_builders._i64
+    cut = lambda t, b, e, step=1: ops.slice(t, _i64([b]), _i64([e]), _i64([step]), _i64([3])).output(0)
+    S = x.get_partial_shape()[3].get_length()
+    if D < S:
+        return ops.concat([neighbours(cut(x, 0, D), cos, sin, D), cut(x, D, S)], 3).output(0)
+
+    def spread(t):                              # [f0, f1, ..] -> [f0, f0, f1, f1, ..]
+        half = ops.unsqueeze(cut(t, 0, D // 2), _i64([4])).output(0)
+        return ops.reshape(ops.concat([half, half], 4), _i64([0, 0, 0, D]), True).output(0)
+    odd, even = cut(x, 1, D, 2), cut(x, 0, D, 2)
+    turned = ops.concat([ops.unsqueeze(ops.negative(odd), _i64([4])).output(0), ops.unsqueeze(even, _i64([4])).output(0)], 4)
+    return ops.add(ops.multiply(x, spread(cos)), ops.multiply(ops.reshape(turned, _i64([0, x.get_partial_shape()[1].get_length(), -1, D]), True), spread(sin))).output(0)
+
+
+@pytest.mark.parametrize("more", [{}, dict(rotary_dim=64), dict(qk_norm=True, rope_scale=1.25)])
+@pytest.mark.parametrize("in_pages", [False, True])
+def test_rotations_of_neighbours_are_recognised(more, in_pages, monkeypatch):
+    monkeypatch.setattr(ov_builders, "_rope", neighbours)
+    cfg = SMALL.with_(**more)
+    state = llama.random_float_state(cfg, seed=4, std=0.05)
+    m = build_llama(cfg, state)
+    ids = np.array([[5, 9, 200, 17, 3]], dtype=np.int64)
+    want = llama.reference_logits(cfg.with_(rope_interleaved=True), {k: v.float() for k, v in state.items()}, torch.tensor(ids[0])).numpy()
+    assert np.abs(ov.Core().compile_model(m, "CPU")(feed_of(ids))[0][0] - want).max() < 1e-3 * np.abs(want).max()
+    got, _ = llm_import.analyze(paged(m) if in_pages else m)
+    assert got.rope_interleaved and got.rotary_dim == cfg.rotary_dim and got.qk_norm == cfg.qk_norm and abs(got.rope_scale - cfg.rope_scale) < 1e-6
+    assert np.allclose(got.inv_freq(), cfg.inv_freq(), rtol=1e-3)
