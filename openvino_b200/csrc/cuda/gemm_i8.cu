@@ -7,7 +7,7 @@
 // the kernel that wrote the tokens has finished. The partial sums are integers: they go to shared memory as [token][channel], every CTA of the cluster
 // adds up its share of the tokens over all partials and finishes them, lanes along the channels.
 //
-// What bounds it: the weights' way from memory, 1 x 6144 x 4096 6.9 us (3.7 TB/s with its start-up of about 3), 7 x 4096 x 14336 11.8 us (5.0), 64 x 28672 x 4096
+// What bounds it: the weights' way from memory, 1 x 6144 x 4096 6.9 us (3.7 TB/s with its start-up of about 3), 1 x 4096 x 11008 10.8 us, 7 x 4096 x 14336 11.8 us (5.0), 64 x 28672 x 4096
 // 21.5 us (5.5), 128256 x 4096 for one token 76.7 us (6.85); with some hundred tokens the rate at which MMAs are issued, 65 cycles each with 128 rows.
 #include <atomic>
 #include <type_traits>
